@@ -7,9 +7,9 @@
 // reduction, arithmetic intensity ~100 FLOP/B -> fp32 VALU bound, not HBM and not MFMA (relu sits between the two
 // contractions).  The forward kernel writes relu(x) = (x + |x|) / 2: the linear half separates,
 //     M_ij = sum_k h_k |P_ik + Q_jk|  +  (sum_k h_k P_ik)  +  (sum_k h_k Q_jk) + b2,      h = w2 / 2,
-// so the (i,j,k) loop is one packed add (v_pk_add_f32, two k per instruction) and one fma with the |.| source
-// modifier: 1.5 VALU instructions per (i,j,k) instead of 3 (add, max, fma); the two row sums ride along with the
-// LDS staging (+2 % work).
+// so the (i,j,k) loop is one add and one fma with the |.| source modifier: 2 VALU instructions per (i,j,k) instead of 3
+// (add, max, fma; packed fp32 instructions are off, see the Makefile); the two row sums ride along with the LDS staging
+// (+2 % work).
 //
 // Forward:  workgroup = 64(i) x 64(j) outputs x one K slice, 256 threads, 4x4 register tile per thread
 //           (rows ty+16a, cols tx+16b so that the LDS row stride of 36 words is conflict-free for
@@ -25,15 +25,19 @@
 #define LDK (BK + 4)  // 36-word row stride: 16 rows x 4 words hit 64 distinct banks
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// acc + w * |x| in ONE instruction.  Left to itself hipcc materialises |x| with v_and_b32 so that it can pair the
-// multiply-adds into v_pk_fma_f32 (packed operands have no abs modifier): 2 instructions per element instead of 1.5.
-// exact 0/1 step of a packed pair: 1 where d > 0 (down to the smallest denormal), else 0 -- two packed multiplies whose
+// acc + w * |x| in ONE instruction (fma_abs).
+// exact 0/1 step of a pair: 1 where d > 0 (down to the smallest denormal), else 0 -- two multiplies per element whose
 // [0,1] output clamp is a free modifier
 __device__ __forceinline__ f32x2 relu_step2(f32x2 d) {
-  const f32x2 big = {8.507059173023462e37f, 8.507059173023462e37f};     // 2^126
+  const float big = 8.507059173023462e37f;     // 2^126
   f32x2 t;
-  asm("v_pk_mul_f32 %0, %1, %2 clamp" : "=v"(t) : "v"(d), "v"(big));
-  asm("v_pk_mul_f32 %0, %1, %2 clamp" : "=v"(t) : "v"(t), "v"(big));
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    float x = d[e];
+    asm("v_mul_f32_e64 %0, %1, %2 clamp" : "=v"(x) : "v"(x), "v"(big));
+    asm("v_mul_f32_e64 %0, %1, %2 clamp" : "=v"(x) : "v"(x), "v"(big));
+    t[e] = x;
+  }
   return t;
 }
 
@@ -133,7 +137,7 @@ __global__ __launch_bounds__(256) void affinity_fwd_kernel(const float* __restri
       for (int a = 0; a < 4; ++a)
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          const f32x2 x0 = p[a][0] + q[b][0], x1 = p[a][1] + q[b][1];      // v_pk_add_f32
+          const f32x2 x0 = p[a][0] + q[b][0], x1 = p[a][1] + q[b][1];
           acc[a][b] = fma_abs(w.x, x0.x, acc[a][b]);                       // |.| is a free VOP3 source modifier
           acc[a][b] = fma_abs(w.y, x0.y, acc[a][b]);
           acc[a][b] = fma_abs(w.z, x1.x, acc[a][b]);
