@@ -165,6 +165,78 @@ int ttdg_sinkhorn_batched_bwd(const float* s, int64_t sb, int64_t sr, int64_t sc
 int ttdg_mha_adjacency(const float* q, const float* k, int d, ttdg_graphs_t gr, float scale, float drop_p,
                        uint64_t seed, int zero_diag, float* Apack, ttdg_stream_t stream);
 
+/* ---- multi-head cross attention (the operator beside ttdg_mha_adjacency: utils/attentions.py:44-116 with queries of one set and
+ *      keys / values of another, several heads, batches) -----------------------------------------------------------------------
+ * q (B, Tq, H, D), k and v (B, Tk, Hkv, D): element strides per batch / position / head, the last dimension dense; H % Hkv == 0 (query
+ * head h reads key head h / (H / Hkv)); D % 8 == 0, 8 <= D <= 256; strides multiples of 16 bytes, pointers 16-byte aligned.
+ * Key j of sample b exists when j < k_lens[b] (k_lens may be NULL: all Tk; values are clamped to 0 .. Tk) and key_mask[b * m_sb + j * m_st]
+ * != 0 (bytes; NULL: all).  What stands at keys that do not exist never reaches a result, infinities and NaN included; a sample without
+ * any key gives zeros and no gradient.
+ *     out[b,i,h,:] = sum_j softmax_j(scale * q[b,i,h,:] . k[b,j,h',:]) v[b,j,h',:]        out (B, Tq, H, D) contiguous
+ * dtype TTDG_F32: products in fp32 on the matrix unit; TTDG_BF16: products of bf16 with fp32 sums, probabilities (and, backward, the
+ * score gradients) rounded to bf16 between the two products.  Softmax statistics are fp32.
+ * For a backward pass later: lse (B, Hkv, Tq * H / Hkv) fp32 (log2 of the sums) and, bf16 only, out_lo (like out: what the rounding of
+ * out dropped) are written when not NULL, and the backward reads q, k, v, out, out_lo, lse, dout (contiguous like out) and writes dq like
+ * out, dk / dv (B, Tk, Hkv, D) contiguous (zeros at keys that do not exist; both NULL: not wanted).  No atomics: results do not change from run to run.
+ * ws / ws_bytes: at least ttdg_attention_{fwd,bwd}_workspace_bytes(a), 16-byte aligned (0 bytes: NULL is fine); nothing in it outlives the call.
+ * TTDG_EINVAL for anything outside this; nothing is launched then. */
+#define TTDG_F32 0
+#define TTDG_BF16 1
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;
+  const int32_t* k_lens;
+  const uint8_t* key_mask;
+  int64_t m_sb, m_st;
+  int32_t B, Tq, Tk, H, Hkv, D, dtype;
+  float scale;
+  void *out, *out_lo;
+  float* lse;
+  const void* dout;
+  void *dq, *dk, *dv;
+  void* ws;
+  size_t ws_bytes;
+} ttdg_attention_t;
+size_t ttdg_attention_fwd_workspace_bytes(const ttdg_attention_t* a);
+size_t ttdg_attention_bwd_workspace_bytes(const ttdg_attention_t* a);
+int ttdg_attention_fwd(const ttdg_attention_t* a, ttdg_stream_t stream);
+int ttdg_attention_bwd(const ttdg_attention_t* a, ttdg_stream_t stream);
+
+/* ---- norm of queries and keys for each head with the position rotation in the same pass (the step between the projections of an
+ *      attention layer, utils/attentions.py:72-74, and its scores) ---------------------------------------------------------------
+ * Two sides, queries and keys (k.H = 0: queries only).  x (B, T, H, D): element strides per batch / position / head, last dimension
+ * dense, strides multiples of 16 bytes, 16-byte aligned; w (D) fp32; y, dy, dx (B, T, H, D) contiguous; dw (D) fp32.
+ *     n = x / sqrt(mean(x^2) + eps),  u = n * w,  y = u with the pairs of its first R channels turned by pos[axis] * freq[pair]
+ * Pair i of R / 2: channels (i, i + R / 2), or (2 i, 2 i + 1) when interleaved; axis i / (R / 2 / axes) of pos (B, T, axes), int32 or
+ * (pos64) int64, element strides p_sb / p_st / p_sa; freq (R / 2) fp64 on the device; angles are formed and reduced in 64 bits.
+ * R = 0: no rotation (pos / freq may be NULL).  D and R multiples of 8, D <= 256.
+ * bwd reads x, w, pos, dy and writes dx and dw of both sides; ws: ttdg_qk_norm_rope_bwd_workspace_bytes(a).  No atomics. */
+typedef struct {
+  const void* x;
+  int64_t sb, st, sh;
+  int32_t T, H;
+  const float* w;
+  const void* pos;
+  int64_t p_sb, p_st, p_sa;
+  void* y;
+  const void* dy;
+  void* dx;
+  float* dw;
+} ttdg_norm_rope_side_t;
+typedef struct {
+  ttdg_norm_rope_side_t q, k;
+  const double* freq;
+  int32_t B, D, R, axes, interleaved, pos64, dtype;
+  float eps;
+  void* ws;
+  size_t ws_bytes;
+} ttdg_qk_norm_rope_t;
+int ttdg_qk_norm_rope_fwd(const ttdg_qk_norm_rope_t* a, ttdg_stream_t stream);
+size_t ttdg_qk_norm_rope_bwd_workspace_bytes(const ttdg_qk_norm_rope_t* a);
+int ttdg_qk_norm_rope_bwd(const ttdg_qk_norm_rope_t* a, ttdg_stream_t stream);
+
+
+
 /* ---- A6+A7 graduated-assignment multi-graph matching, whole solve on device ------
  * (multi_graph_matching.py:223-244, 300-389 with num_clusters == 1; utils/hungarian.py:8-66 ->
  * scipy.optimize.linear_sum_assignment [3P] re-implemented on device, one wavefront per LAP.)

@@ -81,6 +81,31 @@ class Mm(C.Structure):
                 ("C2", C.c_void_p), ("ldc2", C.c_int64), ("nsplit", C.c_int32)]
 
 
+class Attention(C.Structure):
+    """ttdg_attention_t: one cross-attention call, forward or backward (csrc/attention.hip); strides in elements."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p)] + \
+               [(n, C.c_int64) for n in ("q_sb", "q_st", "q_sh", "k_sb", "k_st", "k_sh", "v_sb", "v_st", "v_sh")] + \
+               [("k_lens", C.c_void_p), ("key_mask", C.c_void_p), ("m_sb", C.c_int64), ("m_st", C.c_int64)] + \
+               [(n, C.c_int32) for n in ("B", "Tq", "Tk", "H", "Hkv", "D", "dtype")] + \
+               [("scale", C.c_float), ("out", C.c_void_p), ("out_lo", C.c_void_p), ("lse", C.c_void_p), ("dout", C.c_void_p),
+                ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
+class NormRopeSide(C.Structure):
+    """ttdg_norm_rope_side_t: the queries or the keys of ttdg_qk_norm_rope_t."""
+    _fields_ = [("x", C.c_void_p), ("sb", C.c_int64), ("st", C.c_int64), ("sh", C.c_int64), ("T", C.c_int32), ("H", C.c_int32), ("w", C.c_void_p),
+                ("pos", C.c_void_p), ("p_sb", C.c_int64), ("p_st", C.c_int64), ("p_sa", C.c_int64), ("y", C.c_void_p), ("dy", C.c_void_p),
+                ("dx", C.c_void_p), ("dw", C.c_void_p)]
+
+
+class QkNormRope(C.Structure):
+    """ttdg_qk_norm_rope_t: one call of the per-head norm with rotation, forward or backward (csrc/qk_norm.hip)."""
+    _fields_ = [("q", NormRopeSide), ("k", NormRopeSide), ("freq", C.c_void_p)] + \
+               [(n, C.c_int32) for n in ("B", "D", "R", "axes", "interleaved", "pos64", "dtype")] + \
+               [("eps", C.c_float), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
+
+
+F32, BF16 = 0, 1          # TTDG_F32, TTDG_BF16
 GEMM_GROUP_MAX = 8
 ROW_SCALE_MAX = 64
 RPN_LEVELS_MAX = 8
@@ -107,6 +132,13 @@ SIGNATURES = {
     "ttdg_sinkhorn_batched_fwd": (C.c_int, [_P, _L, _L, _L, _I, _I, _I, _P, _P, _I, _F, _I, _P, _P, _S]),
     "ttdg_sinkhorn_batched_bwd": (C.c_int, [_P, _L, _L, _L, _I, _I, _I, _P, _P, _I, _F, _I, _P, _P, _P, _S]),
     "ttdg_mha_adjacency": (C.c_int, [_P, _P, _I, Graphs, _F, _F, C.c_uint64, _I, _P, _S]),
+    "ttdg_attention_fwd_workspace_bytes": (C.c_size_t, [C.POINTER(Attention)]),
+    "ttdg_attention_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(Attention)]),
+    "ttdg_attention_fwd": (C.c_int, [C.POINTER(Attention), _S]),
+    "ttdg_attention_bwd": (C.c_int, [C.POINTER(Attention), _S]),
+    "ttdg_qk_norm_rope_fwd": (C.c_int, [C.POINTER(QkNormRope), _S]),
+    "ttdg_qk_norm_rope_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(QkNormRope)]),
+    "ttdg_qk_norm_rope_bwd": (C.c_int, [C.POINTER(QkNormRope), _S]),
     "ttdg_gagm_workspace_bytes": (C.c_size_t, [_I]),
     "ttdg_gagm_solve": (C.c_int, [_P, _P, _P, Graphs, GagmCfg, _P, _P, _P, _S]),
     "ttdg_lap_batched": (C.c_int, [_P, _I, _I, _I, _P, _S]),

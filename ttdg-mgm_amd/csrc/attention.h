@@ -1,0 +1,286 @@
+// Device building blocks of the attention kernels (attention.hip): operand fragments, LDS tiles, LDS-DMA, row / key bookkeeping.
+#pragma once
+#include "common.h"
+
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) float f32x8;
+
+struct attn_args {
+  const void *q, *k, *v;
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;     // elements
+  const int32_t* k_lens;
+  const uint8_t* key_mask;
+  int64_t m_sb, m_st;
+  int B, Tq, Tk, H, Hk, D, G, R;                                    // G = H / Hk query heads per key head, R = Tq G rows per problem
+  int row_tiles, key_tiles, splits;
+  float scale, scale_log2;                                          // scale, scale * log2(e)
+  void *out, *out_lo;
+  float* lse;                                                       // (problem, row): log2 of the row's sum of exponentials
+  const void* dout;
+  void *dq, *dk, *dv;
+  float *delta, *part_o, *part_lse;
+};
+
+__device__ __forceinline__ f32x16 f32x16_zero() {
+  f32x16 z;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) z[e] = 0.f;
+  return z;
+}
+
+// register e of a 32 x 32 accumulator holds tile row attn_reg_row(e) + 4 (lane >> 5), tile column lane & 31
+__device__ __forceinline__ constexpr int attn_reg_row(int e) { return (e & 3) + 8 * (e >> 2); }
+
+// value of the own lane and of the lane 32 away, joined
+__device__ __forceinline__ float attn_half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float attn_half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ void attn_wait_dma() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int BN>
+__device__ __forceinline__ constexpr uint64_t attn_all() { return BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1; }
+
+#define ATTN_OOB 0x7ffffff0u          // behind the end of every buffer resource below: reads as zero
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t attn_rsrc(const void* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, 0x7fffff00, 0x00020000);
+}
+__device__ __forceinline__ void attn_dma16(__amdgpu_buffer_rsrc_t r, char* lds_wave_base, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds_wave_base, 16, off, 0, 0, 0);
+}
+__device__ __forceinline__ void attn_dma4(__amdgpu_buffer_rsrc_t r, char* lds_wave_base, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds_wave_base, 4, off, 0, 0, 0);
+}
+
+__device__ __forceinline__ void attn_store4(float* out, f32x4 x) { *(f32x4*)out = x; }
+__device__ __forceinline__ void attn_store4(__bf16* out, f32x4 x) { *(bf16x4*)out = __builtin_convertvector(x, bf16x4); }
+__device__ __forceinline__ void attn_store1(float* out, float*, int64_t i, float x) { out[i] = x; }
+__device__ __forceinline__ void attn_store1(__bf16* out, __bf16* lo, int64_t i, float x) {
+  const __bf16 hi = (__bf16)x;
+  out[i] = hi;
+  if (lo) lo[i] = (__bf16)(x - (float)hi);
+}
+
+// workgroup -> (problem, tile, split).  Consecutive tiles of one split read the same keys; workgroups are dealt to the eight XCDs in turn,
+// so XCD x takes a contiguous run of that order and its L2 sees each key tile once.
+__device__ __forceinline__ void attn_block(const attn_args& p, int tiles, int& prob, int& tile, int& split) {
+  const int T = gridDim.x, q = T >> 3, r = T & 7, x = blockIdx.x & 7, i = blockIdx.x >> 3;
+  const int L = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + i;
+  const int per = tiles * p.splits;
+  prob = L / per;
+  const int rem = L - prob * per;
+  split = rem / tiles;
+  tile = rem - split * tiles;
+}
+
+// row of a problem -> query position and head (rows behind the last one are clamped to it: they are computed and not stored)
+struct attn_row {
+  int row, t, head;
+  __device__ __forceinline__ attn_row(const attn_args& p, int hk, int r) {
+    row = min(r, p.R - 1);
+    t = row / p.G;
+    head = hk * p.G + row - t * p.G;
+  }
+};
+
+// the keys of a sample: how many, and which of a tile exist
+struct attn_keys {
+  int n;
+  const uint8_t* mask;
+  int64_t m_st;
+  __device__ __forceinline__ attn_keys(const attn_args& p, int b) {
+    n = p.k_lens ? max(0, min(p.k_lens[b], p.Tk)) : p.Tk;
+    mask = p.key_mask ? p.key_mask + b * p.m_sb : nullptr;
+    m_st = p.m_st;
+  }
+  __device__ __forceinline__ bool alive(int key) const { return key < n && (!mask || mask[key * m_st]); }
+  template <int BN>
+  __device__ __forceinline__ uint64_t live(int t, int lane) const {      // bit j: key t BN + j exists
+    return __ballot(lane < BN && alive(t * BN + lane));
+  }
+};
+
+// position of 16-byte chunk c of a tile row.  Eight consecutive rows XOR with eight different numbers (row reads: eight lanes of
+// consecutive rows read the same c), and the four rows of a transposing read's 16-lane group land in four different 32-byte windows.
+__device__ __forceinline__ int attn_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+
+template <typename T, int DP>
+struct attn_tile {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int ES = sizeof(T), CE = 16 / ES;      // element size, elements per chunk
+  static constexpr int RB = DP * ES;                      // bytes of a tile row
+  static constexpr int NC = RB / 16, NP = NC / 2;         // chunks per row; chunk pairs: the wavefront's halves take one chunk each
+  static constexpr int bytes(int rows) { return rows * RB; }
+  typedef __attribute__((ext_vector_type(16 / sizeof(T)))) T frag;
+
+  // a row of the second operand: half h holds chunks 2 i + h; zeros behind D
+  static __device__ __forceinline__ void load_row(frag* f, const T* row, int D, int h) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int c = (2 * i + h) * CE;
+      frag z = {};
+      f[i] = c < D ? *(const frag*)(row + c) : z;
+    }
+  }
+  // sum over this half's chunks of f * (a + lo)
+  static __device__ __forceinline__ float row_dot(const frag* f, const T* a, const T* lo, int D, int h) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int c = (2 * i + h) * CE;
+      if (c < D) {
+        const frag x = *(const frag*)(a + c);
+        frag y = {};
+        if (lo) y = *(const frag*)(lo + c);
+#pragma unroll
+        for (int e = 0; e < CE; ++e) s = fmaf((float)f[i][e], (float)x[e] + (float)y[e], s);
+      }
+    }
+    return s;
+  }
+
+  // tile rows [0, ROWS) from base (row stride st elements) into LDS; rows whose bit in `live` is off, and chunks behind D, become zeros
+  template <int ROWS, int WM>
+  static __device__ __forceinline__ void issue(char* lds, const T* base, int64_t st, int D, uint64_t live, int wave, int lane) {
+    const auto r = attn_rsrc(base);
+    const uint32_t stb = (uint32_t)(st * ES);
+#pragma unroll
+    for (int i = 0; i < ROWS * NC / 64 / WM; ++i) {
+      const int lin = (i * WM + wave) * 64 + lane, row = lin / NC, c = (lin % NC) ^ attn_swz(row);
+      const uint32_t off = ((live >> row) & 1) && c * CE < D ? row * stb + c * 16 : ATTN_OOB;
+      attn_dma16(r, lds + (i * WM + wave) * 1024, off);
+    }
+  }
+
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+      return c;
+    } else {
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+  }
+
+  // acc[tile row][lane's row of f] += sum_d tile[row0 + .][d] f[d]
+  static __device__ __forceinline__ void row_product(f32x16& acc, const char* tile, int row0, const frag* f, int l32, int h) {
+    const int base = l32 * RB + ((h ^ attn_swz(l32)) << 4);
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      acc = mma(*(const frag*)(tile + row0 * RB + (base ^ (32 * (i & 3))) + 128 * (i >> 2)), f[i], acc);
+  }
+  // the same with the second operand read from memory
+  static __device__ __forceinline__ void row_product_mem(f32x16& acc, const char* tile, int row0, const T* row, int D, int l32, int h) {
+    const int base = l32 * RB + ((h ^ attn_swz(l32)) << 4);
+#pragma unroll 4
+    for (int i = 0; i < NP; ++i) {
+      const int c = (2 * i + h) * CE;
+      frag f = {};
+      if (c < D) f = *(const frag*)(row + c);
+      acc = mma(*(const frag*)(tile + row0 * RB + (base ^ (32 * (i & 3))) + 128 * (i >> 2)), f, acc);
+    }
+  }
+
+  // acc[d][lane's column] += sum over the 32 tile rows from row0 of tile[.][d] p[.], p in accumulator layout.  For 16-bit types p is
+  // rounded to the inputs' type (round to nearest even, as every operand of the matrix unit is): an error of at most half a step per
+  // term, independent from term to term, while the sums stay in 32 bits.
+  static __device__ __forceinline__ void col_product(f32x16* acc, const char* tile, int row0, const f32x16& p, int lane) {
+    const int h = lane >> 5;
+    if constexpr (F32) {
+      const int l32 = lane & 31;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int row = attn_reg_row(e) + 4 * h;
+        const char* a = tile + (row0 + row) * RB + (((l32 >> 2) ^ (((e & 3) << 1) | h)) << 4) + 4 * (l32 & 3);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*(const float*)(a + 128 * d), p[e], acc[d], 0, 0, 0);
+      }
+    } else {
+      const int i = lane & 15, blk = (lane >> 4) & 1, row = 4 * h + (i >> 2);
+      const int base = row * RB + (((2 * blk + ((i & 3) >> 1)) ^ attn_swz(row)) << 4) + 8 * (i & 1);
+#pragma unroll
+      for (int kg = 0; kg < 2; ++kg) {
+        f32x8 x;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = p[8 * kg + e];
+        const bf16x8 b = __builtin_convertvector(x, bf16x8);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          const char* a = tile + (row0 + 16 * kg) * RB + (base ^ (64 * (d & 1))) + 128 * (d >> 1);
+          const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)a);
+          const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(a + 8 * RB));
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b, acc[d], 0, 0, 0);
+        }
+      }
+    }
+  }
+
+  // the lane's row: channels 32 d + 8 g + 4 h + (0 .. 3) are four consecutive registers.  `lo`: what the rounding of `out` dropped.
+  template <typename O>
+  static __device__ __forceinline__ void store_row(const f32x16* acc, float factor, O* out, O* lo, int D, int h) {
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * d + 8 * g + 4 * h;
+        if (c < D) {
+          f32x4 x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = acc[d][4 * g + e] * factor;
+          attn_store4(out + c, x);
+          if (lo) {
+            if constexpr (sizeof(O) == 2) {
+              const bf16x4 hi = __builtin_convertvector(x, bf16x4);
+              attn_store4(lo + c, x - __builtin_convertvector(hi, f32x4));
+            }
+          }
+        }
+      }
+  }
+};
+
+// row tiles of the dk / dv kernel: q, do, lse and delta of BQ rows of a problem
+struct attn_rows {
+  const char *q, *g;
+  const float *lse, *delta;
+  __device__ __forceinline__ attn_rows(const attn_args& p, int b, int hk, int prob) {
+    q = (const char*)p.q;
+    g = (const char*)p.dout;
+    lse = p.lse + (int64_t)prob * p.R;
+    delta = p.delta + (int64_t)prob * p.R;
+    q_off = b * p.q_sb + (int64_t)hk * p.G * p.q_sh;
+    g_off = ((int64_t)b * p.Tq * p.H + (int64_t)hk * p.G) * p.D;
+  }
+  int64_t q_off, g_off;
+  template <typename T, int DP, int BQ, int WM>
+  __device__ __forceinline__ void issue(const attn_args& p, char* lds, int tile_bytes, int t, int wave, int lane) const {
+    typedef attn_tile<T, DP> tile_t;
+    const int r0 = t * BQ, tb = r0 / p.G, left = p.R - r0;
+    const auto rq = attn_rsrc((const T*)q + q_off + (int64_t)tb * p.q_st);
+    const auto rg = attn_rsrc((const T*)g + g_off + (int64_t)tb * p.H * p.D);
+    const uint32_t qst = (uint32_t)(p.q_st * tile_t::ES), qsh = (uint32_t)(p.q_sh * tile_t::ES);
+    const uint32_t gst = (uint32_t)(p.H * p.D * tile_t::ES), gsh = (uint32_t)(p.D * tile_t::ES);
+#pragma unroll
+    for (int i = 0; i < BQ * tile_t::NC / 64 / WM; ++i) {
+      const int lin = (i * WM + wave) * 64 + lane, row = lin / tile_t::NC, c = (lin % tile_t::NC) ^ attn_swz(row);
+      const int r = r0 + row, tt = r / p.G, gg = r - tt * p.G;
+      const bool ok = row < left && c * tile_t::CE < p.D;
+      attn_dma16(rq, lds + (i * WM + wave) * 1024, ok ? (tt - tb) * qst + gg * qsh + c * 16 : ATTN_OOB);
+      attn_dma16(rg, lds + tile_bytes + (i * WM + wave) * 1024, ok ? (tt - tb) * gst + gg * gsh + c * 16 : ATTN_OOB);
+    }
+    if (wave == WM - 1) {
+      const uint32_t off = lane < BQ && lane < left ? lane * 4 : ATTN_OOB;
+      attn_dma4(attn_rsrc(lse + r0), lds + 2 * tile_bytes, off);
+      attn_dma4(attn_rsrc(delta + r0), lds + 2 * tile_bytes + 256, off);
+    }
+  }
+};

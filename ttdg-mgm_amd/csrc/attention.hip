@@ -1,0 +1,519 @@
+// Multi-head cross attention: queries of one set attend to keys / values of another (an encoder's states), forward and backward.
+//
+//   s_ij = scale q_i . k_j        p_ij = exp(s_ij) / sum_j exp(s_ij)  over the keys j that exist (j < k_lens[b], key_mask[b, j] != 0)
+//   o_i  = sum_j p_ij v_j         (a row without any key: o_i = 0, no gradient)
+//   delta_i = o_i . do_i          ds_ij = p_ij (v_j . do_i - delta_i)
+//   dv_j = sum_i p_ij do_i        dk_j = scale sum_i ds_ij q_i        dq_i = scale sum_j ds_ij k_j
+//
+// Shared key heads: the G = H / Hkv query heads of a key head and the Tq queries form ONE list of R = Tq G rows, row r = t G + g, so a
+// problem is (batch, key head): R rows against Tk keys, and nothing below knows about heads.
+//
+// Everything is computed transposed, S^T = K Q^T with v_mfma 32 x 32 tiles: a lane then owns one row (column of the tile) and 16 of the
+// 32 keys, so the softmax is in-lane plus one exchange between the wavefront's halves, and the probabilities already lie in the registers
+// the way the next product O^T = V^T P^T wants its second operand (which keys sit in which of the operand's slots is free as long as V^T
+// uses the same order).  V^T is read from the row-major V tile by the transposing LDS read (16-bit types) or by plain column reads
+// (32-bit).  One body serves both types: bfloat16 through v_mfma_f32_32x32x16_bf16, float32 through v_mfma_f32_32x32x2_f32 (exact products).
+//
+// Tiles go memory -> LDS by LDS-DMA, double-buffered, in 16-byte chunks whose position in the row is XORed with a function of the row
+// (conflict-free for row reads and for the transposing reads).  A chunk that must not be read - a row behind the last key, a masked
+// key, a channel behind D - gets an offset behind the end of the buffer resource: the hardware then stores zeros, so whatever stands in
+// masked places (infinities, NaN) never reaches a product.  The resource starts at the tile, so 32-bit offsets are relative to the tile
+// and a cache may be longer than 4 GiB.
+#include "attention.h"
+
+// ---------------------------------------------------------------------------------------------------------------- forward
+template <typename T, int DP, int BN, int WM>
+__global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) void attn_fwd_kernel(attn_args p) {
+  typedef attn_tile<T, DP> tile_t;
+  typedef typename tile_t::frag frag;
+  extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
+  constexpr int TB = tile_t::bytes(BN);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = lane >> 5, l32 = lane & 31;
+  int prob, tile, split;
+  attn_block(p, p.row_tiles, prob, tile, split);
+  const int b = prob / p.Hk, hk = prob - b * p.Hk;
+
+  const int row = (tile * WM + wave) * 32 + l32;
+  const attn_row rw(p, hk, row);
+  frag qf[tile_t::NP];
+  tile_t::load_row(qf, (const T*)p.q + b * p.q_sb + (int64_t)rw.t * p.q_st + (int64_t)rw.head * p.q_sh, p.D, h);
+
+  f32x16 o[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) o[d] = f32x16_zero();
+  float m = -INFINITY, l = 0.f;
+
+  const attn_keys keys(p, b);
+  const int nt = (keys.n + BN - 1) / BN;
+  const int t0 = (int)((int64_t)nt * split / p.splits), t1 = (int)((int64_t)nt * (split + 1) / p.splits);
+  const T* kb = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh;
+  const T* vb = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh;
+  uint64_t live_next = t0 < t1 ? keys.live<BN>(t0, lane) : 0;
+  if (live_next) {
+    tile_t::template issue<BN, WM>(attn_smem, kb + (int64_t)t0 * BN * p.k_st, p.k_st, p.D, live_next, wave, lane);
+    tile_t::template issue<BN, WM>(attn_smem + TB, vb + (int64_t)t0 * BN * p.v_st, p.v_st, p.D, live_next, wave, lane);
+  }
+  for (int t = t0; t < t1; ++t) {
+    const char* kt = attn_smem + ((t - t0) & 1) * 2 * TB;
+    const char* vt = kt + TB;
+    const uint64_t live = live_next;
+    attn_wait_dma();                 // this wavefront's share of tile t has landed
+    __syncthreads();                 // ... everybody's has, and nobody still reads the other buffer
+    if (t + 1 < t1) {
+      live_next = keys.live<BN>(t + 1, lane);
+      if (live_next) {
+        char* nx = attn_smem + ((t + 1 - t0) & 1) * 2 * TB;
+        tile_t::template issue<BN, WM>(nx, kb + (int64_t)(t + 1) * BN * p.k_st, p.k_st, p.D, live_next, wave, lane);
+        tile_t::template issue<BN, WM>(nx + TB, vb + (int64_t)(t + 1) * BN * p.v_st, p.v_st, p.D, live_next, wave, lane);
+      }
+    }
+    if (live == 0) continue;         // (the same for every wavefront of the workgroup)
+    f32x16 s[BN / 32];
+#pragma unroll
+    for (int kk = 0; kk < BN / 32; ++kk) {
+      s[kk] = f32x16_zero();
+      tile_t::row_product(s[kk], kt, 32 * kk, qf, l32, h);
+    }
+    if (live != attn_all<BN>()) {
+#pragma unroll
+      for (int kk = 0; kk < BN / 32; ++kk) {
+        const uint32_t bits = (uint32_t)(live >> (32 * kk)) >> (4 * h);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!((bits >> attn_reg_row(e)) & 1)) s[kk][e] = -INFINITY;
+      }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int kk = 0; kk < BN / 32; ++kk)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kk][e]);
+    mx = attn_half_max(mx);
+    const float mn = fmaxf(m, mx * p.scale_log2);
+    if (__any(mn > m)) {             // the running maximum grew somewhere: rescale what has been summed
+      const float a = fast_exp2(m - mn);
+      l *= a;
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) o[d] *= a;
+      m = mn;
+    }
+#pragma unroll
+    for (int kk = 0; kk < BN / 32; ++kk) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float x = fast_exp2(fmaf(s[kk][e], p.scale_log2, -m));
+        s[kk][e] = x;
+        l += x;
+      }
+      tile_t::col_product(o, vt, 32 * kk, s[kk], lane);
+    }
+  }
+  l = attn_half_sum(l);
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;      // no key at all: zeros
+  const float lse = l > 0.f || l != l ? m + fast_log2(l) : -INFINITY;
+  if (row >= p.R) return;
+  if (p.splits > 1) {
+    const int64_t pr = ((int64_t)prob * p.splits + split) * p.R + row;
+    if (h == 0) p.part_lse[pr] = lse;
+    tile_t::store_row(o, inv, p.part_o + pr * p.D, (float*)nullptr, p.D, h);
+  } else {
+    if (h == 0 && p.lse) p.lse[(int64_t)prob * p.R + row] = lse;
+    const int64_t off = (((int64_t)b * p.Tq + rw.t) * p.H + rw.head) * p.D;
+    tile_t::store_row(o, inv, (T*)p.out + off, p.out_lo ? (T*)p.out_lo + off : (T*)nullptr, p.D, h);
+  }
+}
+
+// joins the splits of a row: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max); one wavefront per row
+template <typename T>
+__global__ __launch_bounds__(256) void attn_combine_kernel(attn_args p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= (int64_t)p.B * p.Hk * p.R) return;
+  const int prob = (int)(id / p.R), row = (int)(id - (int64_t)prob * p.R);
+  const int b = prob / p.Hk, hk = prob - b * p.Hk;
+  const int64_t pr = (int64_t)prob * p.splits * p.R + row;
+  float mx = -INFINITY;
+  for (int s = lane; s < p.splits; s += 64) mx = fmaxf(mx, p.part_lse[pr + (int64_t)s * p.R]);
+  mx = wave_max(mx);
+  const bool any = mx > -INFINITY || mx != mx;
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, z = 0.f;
+  if (any)
+    for (int s = 0; s < p.splits; ++s) {
+      const int64_t ps = pr + (int64_t)s * p.R;
+      const float w = fast_exp2(p.part_lse[ps] - mx);
+      z += w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (lane + 64 * e < p.D) o[e] = fmaf(w, p.part_o[ps * p.D + lane + 64 * e], o[e]);
+    }
+  const float inv = any ? 1.f / z : 0.f;
+  const attn_row rw(p, hk, row);
+  const int64_t off = (((int64_t)b * p.Tq + rw.t) * p.H + rw.head) * p.D;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (lane + 64 * e < p.D) attn_store1((T*)p.out, p.out_lo ? (T*)p.out_lo : nullptr, off + lane + 64 * e, o[e] * inv);
+  if (lane == 0 && p.lse) p.lse[(int64_t)prob * p.R + row] = any ? mx + fast_log2(z) : -INFINITY;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- backward
+// dq, and delta_i = do_i . o_i on the way (the dk / dv kernel reads it).  o is taken as out + out_lo: with the output rounded to bfloat16
+// alone the error of delta (2^-9 |o| |do|, the same for every key of a row) would reach dq times the mean key.
+template <typename T, int DP, int BN, int WM>
+__global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) void attn_bwd_dq_kernel(attn_args p) {
+  typedef attn_tile<T, DP> tile_t;
+  typedef typename tile_t::frag frag;
+  extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
+  constexpr int TB = tile_t::bytes(BN);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = lane >> 5, l32 = lane & 31;
+  int prob, tile, split;
+  attn_block(p, p.row_tiles, prob, tile, split);
+  const int b = prob / p.Hk, hk = prob - b * p.Hk;
+
+  const int row = (tile * WM + wave) * 32 + l32;
+  const attn_row rw(p, hk, row);
+  frag qf[tile_t::NP], gf[tile_t::NP];
+  tile_t::load_row(qf, (const T*)p.q + b * p.q_sb + (int64_t)rw.t * p.q_st + (int64_t)rw.head * p.q_sh, p.D, h);
+  const int64_t off = (((int64_t)b * p.Tq + rw.t) * p.H + rw.head) * p.D;
+  tile_t::load_row(gf, (const T*)p.dout + off, p.D, h);
+  float delta = tile_t::row_dot(gf, (const T*)p.out + off, p.out_lo ? (const T*)p.out_lo + off : (const T*)nullptr, p.D, h);
+  delta = attn_half_sum(delta);
+  float lse = p.lse[(int64_t)prob * p.R + rw.row];
+  if (split == 0 && h == 0 && row < p.R) p.delta[(int64_t)prob * p.R + row] = delta;
+  if (lse == -INFINITY) lse = INFINITY;       // a row without any key: p = 0
+
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) acc[d] = f32x16_zero();
+
+  const attn_keys keys(p, b);
+  const int nt = (keys.n + BN - 1) / BN;
+  const int t0 = (int)((int64_t)nt * split / p.splits), t1 = (int)((int64_t)nt * (split + 1) / p.splits);
+  const T* kb = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh;
+  const T* vb = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh;
+  uint64_t live_next = t0 < t1 ? keys.live<BN>(t0, lane) : 0;
+  if (live_next) {
+    tile_t::template issue<BN, WM>(attn_smem, kb + (int64_t)t0 * BN * p.k_st, p.k_st, p.D, live_next, wave, lane);
+    tile_t::template issue<BN, WM>(attn_smem + TB, vb + (int64_t)t0 * BN * p.v_st, p.v_st, p.D, live_next, wave, lane);
+  }
+  for (int t = t0; t < t1; ++t) {
+    const char* kt = attn_smem + ((t - t0) & 1) * 2 * TB;
+    const char* vt = kt + TB;
+    const uint64_t live = live_next;
+    attn_wait_dma();
+    __syncthreads();
+    if (t + 1 < t1) {
+      live_next = keys.live<BN>(t + 1, lane);
+      if (live_next) {
+        char* nx = attn_smem + ((t + 1 - t0) & 1) * 2 * TB;
+        tile_t::template issue<BN, WM>(nx, kb + (int64_t)(t + 1) * BN * p.k_st, p.k_st, p.D, live_next, wave, lane);
+        tile_t::template issue<BN, WM>(nx + TB, vb + (int64_t)(t + 1) * BN * p.v_st, p.v_st, p.D, live_next, wave, lane);
+      }
+    }
+    if (live == 0) continue;
+#pragma unroll
+    for (int kk = 0; kk < BN / 32; ++kk) {
+      f32x16 s = f32x16_zero(), dp = f32x16_zero();
+      tile_t::row_product(s, kt, 32 * kk, qf, l32, h);
+      tile_t::row_product(dp, vt, 32 * kk, gf, l32, h);
+      const uint32_t bits = (uint32_t)(live >> (32 * kk)) >> (4 * h);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float pr = fast_exp2(fmaf(s[e], p.scale_log2, -lse));
+        s[e] = ((bits >> attn_reg_row(e)) & 1) ? pr * (dp[e] - delta) : 0.f;
+      }
+      tile_t::col_product(acc, kt, 32 * kk, s, lane);
+    }
+  }
+  if (row >= p.R) return;
+  if (p.splits > 1) tile_t::store_row(acc, 1.f, p.part_o + (int64_t)split * p.B * p.Tq * p.H * p.D + off, (float*)nullptr, p.D, h);
+  else tile_t::store_row(acc, p.scale, (T*)p.dq + off, (T*)nullptr, p.D, h);
+}
+
+// dk and dv: a wavefront owns 32 keys, their k and v rows in registers (REGS) or re-read through the caches (the registers of float32 with
+// 256 channels are full of the two sums), and walks over the rows; q and do tiles in LDS serve both as rows (scores) and, transposed, as
+// the second products' first operand.
+template <typename T, int DP, int BQ, int WM, bool REGS>
+__global__ __launch_bounds__(64 * WM, 1) void attn_bwd_dkv_kernel(attn_args p) {
+  typedef attn_tile<T, DP> tile_t;
+  typedef typename tile_t::frag frag;
+  extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
+  constexpr int TB = tile_t::bytes(BQ);
+  constexpr int STAGE = 2 * TB + 1024;        // q tile, do tile, lse (64 floats), delta (64 floats), padding
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = lane >> 5, l32 = lane & 31;
+  int prob, tile, split;
+  attn_block(p, p.key_tiles, prob, tile, split);
+  const int b = prob / p.Hk, hk = prob - b * p.Hk;
+
+  const int key = (tile * WM + wave) * 32 + l32;
+  const attn_keys keys(p, b);
+  const bool mine = keys.alive(key);
+  const int64_t kr = min(key, p.Tk - 1);
+  const T* kp = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh + kr * p.k_st;
+  const T* vp = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh + kr * p.v_st;
+  frag kf[REGS ? tile_t::NP : 1], vf[REGS ? tile_t::NP : 1];
+  if (REGS) {
+    tile_t::load_row(kf, kp, p.D, h);
+    tile_t::load_row(vf, vp, p.D, h);
+  }
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) { dk[d] = f32x16_zero(); dv[d] = f32x16_zero(); }
+
+  const int nt = __syncthreads_or(mine) ? (p.R + BQ - 1) / BQ : 0;      // no key of this workgroup exists: zeros
+  const int t0 = (int)((int64_t)nt * split / p.splits), t1 = (int)((int64_t)nt * (split + 1) / p.splits);
+  const attn_rows rows(p, b, hk, prob);
+  if (t0 < t1) rows.template issue<T, DP, BQ, WM>(p, attn_smem, TB, t0, wave, lane);
+  for (int t = t0; t < t1; ++t) {
+    const char* qt = attn_smem + ((t - t0) & 1) * STAGE;
+    const char* gt = qt + TB;
+    attn_wait_dma();
+    __syncthreads();
+    if (t + 1 < t1) rows.template issue<T, DP, BQ, WM>(p, attn_smem + ((t + 1 - t0) & 1) * STAGE, TB, t + 1, wave, lane);
+#pragma unroll
+    for (int qq = 0; qq < BQ / 32; ++qq) {
+      f32x16 s = f32x16_zero(), dp = f32x16_zero();
+      if (REGS) {
+        tile_t::row_product(s, qt, 32 * qq, kf, l32, h);
+        tile_t::row_product(dp, gt, 32 * qq, vf, l32, h);
+      } else {
+        tile_t::row_product_mem(s, qt, 32 * qq, kp, p.D, l32, h);
+        tile_t::row_product_mem(dp, gt, 32 * qq, vp, p.D, l32, h);
+      }
+      const float* st = (const float*)(qt + 2 * TB) + 32 * qq + 4 * h;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 ls = *(const f32x4*)(st + 8 * g), de = *(const f32x4*)(st + 64 + 8 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float pr = fast_exp2(fmaf(s[4 * g + e], p.scale_log2, -ls[e]));
+          s[4 * g + e] = pr;
+          dp[4 * g + e] = pr * (dp[4 * g + e] - de[e]);
+        }
+      }
+      tile_t::col_product(dv, gt, 32 * qq, s, lane);
+      tile_t::col_product(dk, qt, 32 * qq, dp, lane);
+    }
+  }
+  if (key >= p.Tk) return;
+  const int64_t off = (((int64_t)b * p.Tk + key) * p.Hk + hk) * p.D;
+  if (!mine) {                        // (a select, not a factor: the sums of a key that does not exist may be anything)
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) { dk[d] = f32x16_zero(); dv[d] = f32x16_zero(); }
+  }
+  if (p.splits > 1) {
+    const int64_t plane = (int64_t)p.B * p.Tk * p.Hk * p.D;
+    tile_t::store_row(dk, 1.f, p.part_o + 2 * split * plane + off, (float*)nullptr, p.D, h);
+    tile_t::store_row(dv, 1.f, p.part_o + (2 * split + 1) * plane + off, (float*)nullptr, p.D, h);
+  } else {
+    tile_t::store_row(dk, p.scale, (T*)p.dk + off, (T*)nullptr, p.D, h);
+    tile_t::store_row(dv, 1.f, (T*)p.dv + off, (T*)nullptr, p.D, h);
+  }
+}
+
+// adds the planes of a split in their order: out[i] = factor * sum_s part[s * stride + i], four values per thread (n % 4 == 0: D is)
+template <typename T>
+__global__ __launch_bounds__(256) void attn_reduce_kernel(const float* __restrict__ part, int64_t stride, int splits, float factor,
+                                                          T* __restrict__ out, int64_t n) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  f32x4 a = *(const f32x4*)(part + i);
+  for (int s = 1; s < splits; ++s) a += *(const f32x4*)(part + s * stride + i);
+  attn_store4(out + i, a * factor);
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+static int attn_check(const ttdg_attention_t* a, const char* what) {
+  static thread_local char msg[160];
+#define ATTN_REQUIRE(cond, text)                                        \
+  do {                                                                  \
+    if (!(cond)) {                                                      \
+      snprintf(msg, sizeof(msg), "%s: %s", what, text);                 \
+      return ttdg_fail(TTDG_EINVAL, msg);                               \
+    }                                                                   \
+  } while (0)
+  ATTN_REQUIRE(a->dtype == TTDG_F32 || a->dtype == TTDG_BF16, "dtype must be TTDG_F32 or TTDG_BF16");
+  ATTN_REQUIRE(a->B >= 0 && a->Tq >= 0 && a->Tk >= 0 && a->H >= 1 && a->Hkv >= 1, "negative size or no head");
+  ATTN_REQUIRE(a->H % a->Hkv == 0, "the number of query heads must be a multiple of the number of key heads");
+  const int ce = a->dtype == TTDG_F32 ? 4 : 8, es = a->dtype == TTDG_F32 ? 4 : 2;
+  ATTN_REQUIRE(a->D >= 8 && a->D <= 256 && a->D % 8 == 0, "the head dimension must be a multiple of 8 up to 256");
+  ATTN_REQUIRE(a->scale > 0.f && a->scale < 1e30f, "the scale must be positive and finite");
+  if (a->B == 0 || a->Tq == 0) return 0;
+  ATTN_REQUIRE(a->q && (a->Tk == 0 || (a->k && a->v)), "null pointer");
+  const int64_t st[9] = {a->q_sb, a->q_st, a->q_sh, a->k_sb, a->k_st, a->k_sh, a->v_sb, a->v_st, a->v_sh};
+  for (int i = 0; i < 9; ++i) ATTN_REQUIRE(st[i] >= 0 && st[i] % ce == 0, "strides must be multiples of 16 bytes");
+  ATTN_REQUIRE(((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) % 16 == 0, "q, k and v must be 16-byte aligned");
+  // offsets inside a tile are 32-bit: 64 rows, of the queries spread over the G heads of a key head
+  const int64_t lim = (int64_t)0x7f000000 / es;
+  ATTN_REQUIRE(a->k_st <= lim / 64 && a->v_st <= lim / 64, "key / value rows too far apart");
+  ATTN_REQUIRE(a->q_st <= lim / 130 && a->q_sh <= lim / 2 / (a->H / a->Hkv), "query rows or heads too far apart");
+  const int64_t R = (int64_t)a->Tq * (a->H / a->Hkv);
+  ATTN_REQUIRE(R < (1 << 30) && a->Tk < (1 << 30) && (int64_t)a->B * a->Hkv < (1 << 24), "too many rows, keys or heads");
+  ATTN_REQUIRE((int64_t)a->H * a->D <= (1 << 20), "more than 2^20 channels in all heads");
+  ATTN_REQUIRE(a->m_sb >= 0 && a->m_st >= 0, "negative mask stride");
+#undef ATTN_REQUIRE
+  return 0;
+}
+
+static attn_args attn_make(const ttdg_attention_t* a) {
+  attn_args p = {};
+  p.q = a->q; p.k = a->k; p.v = a->v;
+  p.q_sb = a->q_sb; p.q_st = a->q_st; p.q_sh = a->q_sh;
+  p.k_sb = a->k_sb; p.k_st = a->k_st; p.k_sh = a->k_sh;
+  p.v_sb = a->v_sb; p.v_st = a->v_st; p.v_sh = a->v_sh;
+  p.k_lens = a->k_lens; p.key_mask = a->key_mask; p.m_sb = a->m_sb; p.m_st = a->m_st;
+  p.B = a->B; p.Tq = a->Tq; p.Tk = a->Tk; p.H = a->H; p.Hk = a->Hkv; p.D = a->D;
+  p.G = a->H / a->Hkv; p.R = a->Tq * p.G;
+  p.scale = a->scale; p.scale_log2 = a->scale * TTDG_LOG2E;
+  p.out = a->out; p.out_lo = a->out_lo; p.lse = a->lse;
+  p.dout = a->dout; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
+  p.splits = 1;
+  return p;
+}
+
+// How many workgroups share one (problem, tile): the long axis (`units` tiles of it) is split until the launch fills the chip - 512
+// workgroups, two per CU - but a part keeps at least `least` tiles, below which the join costs more than the part saves.
+static int attn_splits(int64_t blocks, int units, int least) {
+  if (blocks >= 384 || units < 2 * least) return 1;
+  int64_t s = (512 + blocks - 1) / blocks;
+  if (s > units / least) s = units / least;
+  if (s > 256) s = 256;
+  return s < 1 ? 1 : (int)s;
+}
+
+struct attn_plan {
+  int dp, wm, bn, row_tiles, fwd_splits, dq_splits, key_tiles, bq, dkv_splits;
+  size_t fwd_ws, bwd_ws;
+};
+
+static attn_plan attn_planned(const ttdg_attention_t* a) {
+  attn_plan q;
+  const bool f32 = a->dtype == TTDG_F32;
+  const int64_t probs = (int64_t)a->B * a->Hkv;
+  const int64_t R = (int64_t)a->Tq * (a->H / a->Hkv);
+  q.dp = a->D <= 64 ? 64 : a->D <= 128 ? 128 : 256;
+  q.bn = q.dp == 64 || (q.dp == 128 && !f32) ? 64 : 32;
+  q.wm = R <= 32 ? 1 : 4;
+  q.row_tiles = (int)((R + 32 * q.wm - 1) / (32 * q.wm));
+  const int kt = (a->Tk + q.bn - 1) / q.bn;
+  q.fwd_splits = attn_splits(probs * q.row_tiles * q.wm / 4 + 1, kt, 2);
+  q.dq_splits = attn_splits(probs * q.row_tiles * q.wm / 4 + 1, kt, 2);
+  q.key_tiles = (a->Tk + 127) / 128;
+  q.bq = q.bn;
+  const int qt = (int)((R + q.bq - 1) / q.bq);
+  q.dkv_splits = attn_splits(probs * q.key_tiles, qt, 2);
+  const size_t rows = (size_t)probs * R;
+  q.fwd_ws = q.fwd_splits > 1 ? (size_t)q.fwd_splits * rows * (a->D + 1) * 4 : 0;
+  const size_t kv = (size_t)a->B * a->Tk * a->Hkv * a->D * 4;
+  size_t w = q.dq_splits > 1 ? (size_t)q.dq_splits * rows * a->D * 4 : 0;
+  if (q.dkv_splits > 1 && 2 * kv * q.dkv_splits > w) w = 2 * kv * q.dkv_splits;
+  q.bwd_ws = rows * 4 + 16 + w;
+  return q;
+}
+
+extern "C" size_t ttdg_attention_fwd_workspace_bytes(const ttdg_attention_t* a) {
+  if (!a || attn_check(a, "attention_fwd_workspace_bytes")) return 0;
+  return a->B && a->Tq ? attn_planned(a).fwd_ws : 0;
+}
+
+extern "C" size_t ttdg_attention_bwd_workspace_bytes(const ttdg_attention_t* a) {
+  if (!a || attn_check(a, "attention_bwd_workspace_bytes")) return 0;
+  return a->B && a->Tq ? attn_planned(a).bwd_ws : 0;
+}
+
+#define ATTN_LAUNCH(kernel, grid, threads, lds, stream, args)                              \
+  do {                                                                                     \
+    TTDG_ALLOW_LDS((kernel), (lds));                                                       \
+    hipLaunchKernelGGL((kernel), dim3((unsigned)(grid)), dim3(threads), (lds), (hipStream_t)(stream), args); \
+    if (int e_ = ttdg_launch_status(#kernel)) return e_;                                   \
+  } while (0)
+
+template <typename T, int DP, int BN>
+static int attn_fwd_launch(const attn_args& p, const attn_plan& q, ttdg_stream_t stream) {
+  constexpr int lds = 4 * attn_tile<T, DP>::bytes(BN);
+  const int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;
+  TTDG_LIMIT(grid < (1ll << 31), "attention_fwd: too many workgroups");
+  if (q.wm == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 1>), grid, 64, lds, stream, p);
+  else ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 4>), grid, 256, lds, stream, p);
+  if (p.splits > 1) ATTN_LAUNCH((attn_combine_kernel<T>), ((int64_t)p.B * p.Hk * p.R + 3) / 4, 256, 0, stream, p);
+  return 0;
+}
+
+template <typename T, int DP, int BN>
+static int attn_bwd_launch(attn_args p, const attn_plan& q, ttdg_stream_t stream) {
+  constexpr int lds = 4 * attn_tile<T, DP>::bytes(BN);
+  p.splits = q.dq_splits;
+  int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;
+  TTDG_LIMIT(grid < (1ll << 31), "attention_bwd: too many workgroups");
+  if (q.wm == 1) ATTN_LAUNCH((attn_bwd_dq_kernel<T, DP, BN, 1>), grid, 64, lds, stream, p);
+  else ATTN_LAUNCH((attn_bwd_dq_kernel<T, DP, BN, 4>), grid, 256, lds, stream, p);
+  const int64_t nq = (int64_t)p.B * p.Tq * p.H * p.D, nk = (int64_t)p.B * p.Tk * p.Hk * p.D;
+  if (p.splits > 1) {
+    hipLaunchKernelGGL(attn_reduce_kernel<T>, dim3((unsigned)((nq / 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p.part_o, nq, p.splits, p.scale, (T*)p.dq, nq);
+    if (int e = ttdg_launch_status("attn_reduce")) return e;
+  }
+  if (p.Tk == 0 || !p.dk) return 0;
+  p.splits = q.dkv_splits;
+  grid = (int64_t)p.B * p.Hk * p.key_tiles * p.splits;
+  TTDG_LIMIT(grid < (1ll << 31), "attention_bwd: too many workgroups");
+  constexpr bool regs = !(sizeof(T) == 4 && DP == 256);
+  constexpr int lds2 = 4 * attn_tile<T, DP>::bytes(BN) + 2048;
+  ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, 4, regs>), grid, 256, lds2, stream, p);
+  if (p.splits > 1) {
+    for (int w = 0; w < 2; ++w) {
+      hipLaunchKernelGGL(attn_reduce_kernel<T>, dim3((unsigned)((nk / 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p.part_o + w * nk, 2 * nk, p.splits,
+                         w == 0 ? p.scale : 1.f, (T*)(w == 0 ? p.dk : p.dv), nk);
+      if (int e = ttdg_launch_status("attn_reduce")) return e;
+    }
+  }
+  return 0;
+}
+
+#define ATTN_DISPATCH(fn, a, ...)                                                                  \
+  do {                                                                                             \
+    if ((a)->dtype == TTDG_F32) {                                                                  \
+      if (q.dp == 64) return fn<float, 64, 64>(__VA_ARGS__);                                       \
+      if (q.dp == 128) return fn<float, 128, 32>(__VA_ARGS__);                                     \
+      return fn<float, 256, 32>(__VA_ARGS__);                                                      \
+    }                                                                                              \
+    if (q.dp == 64) return fn<__bf16, 64, 64>(__VA_ARGS__);                                        \
+    if (q.dp == 128) return fn<__bf16, 128, 64>(__VA_ARGS__);                                      \
+    return fn<__bf16, 256, 32>(__VA_ARGS__);                                                       \
+  } while (0)
+
+extern "C" int ttdg_attention_fwd(const ttdg_attention_t* a, ttdg_stream_t stream) {
+  TTDG_REQUIRE(a, "attention_fwd: null pointer");
+  if (int e = attn_check(a, "attention_fwd")) return e;
+  if (a->B == 0 || a->Tq == 0) return 0;
+  TTDG_REQUIRE(a->out && (uintptr_t)a->out % 16 == 0 && (uintptr_t)a->out_lo % 16 == 0, "attention_fwd: out must be a 16-byte aligned pointer");
+  const attn_plan q = attn_planned(a);
+  TTDG_REQUIRE(q.fwd_ws == 0 || (a->ws && (uintptr_t)a->ws % 16 == 0 && a->ws_bytes >= q.fwd_ws), "attention_fwd: workspace too small or misaligned");
+  attn_args p = attn_make(a);
+  p.row_tiles = q.row_tiles;
+  p.splits = q.fwd_splits;
+  p.part_o = (float*)a->ws;
+  p.part_lse = (float*)a->ws + (size_t)q.fwd_splits * p.B * p.Hk * p.R * p.D;
+  ATTN_DISPATCH(attn_fwd_launch, a, p, q, stream);
+}
+
+extern "C" int ttdg_attention_bwd(const ttdg_attention_t* a, ttdg_stream_t stream) {
+  TTDG_REQUIRE(a, "attention_bwd: null pointer");
+  if (int e = attn_check(a, "attention_bwd")) return e;
+  if (a->B == 0 || a->Tq == 0) {
+    TTDG_REQUIRE(a->B == 0 || a->Tk == 0 || !a->dk, "attention_bwd: without queries dk and dv are zeros; fill them");
+    return 0;
+  }
+  TTDG_REQUIRE(a->out && a->lse && a->dout && a->dq && (!a->dk == !a->dv), "attention_bwd: null pointer (dk and dv: both or none)");
+  TTDG_REQUIRE(((uintptr_t)a->out | (uintptr_t)a->out_lo | (uintptr_t)a->dout | (uintptr_t)a->dq | (uintptr_t)a->dk | (uintptr_t)a->dv) % 16 == 0,
+               "attention_bwd: out, dout and the gradients must be 16-byte aligned");
+  const attn_plan q = attn_planned(a);
+  TTDG_REQUIRE(a->ws && (uintptr_t)a->ws % 16 == 0 && a->ws_bytes >= q.bwd_ws, "attention_bwd: workspace too small or misaligned");
+  attn_args p = attn_make(a);
+  p.row_tiles = q.row_tiles;
+  p.key_tiles = q.key_tiles;
+  p.delta = (float*)a->ws;
+  p.part_o = (float*)a->ws + (((size_t)p.B * p.Hk * p.R + 3) & ~(size_t)3);
+  ATTN_DISPATCH(attn_bwd_launch, a, p, q, stream);
+}

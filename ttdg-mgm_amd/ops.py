@@ -410,6 +410,315 @@ def mha_adjacency(q, k, gr, sizes, scale, drop_p=0.0, seed=0, zero_diag=True):
     return apack
 
 
+# ------------------------------------------------------------------------------------------- attention between two sets
+_ATTN_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
+def _on_device_of(t):
+    """The kernels run on the current stream of the device the tensors live on, whatever device is current."""
+    return torch.cuda.device(t.device) if t.is_cuda and t.device.index != torch.cuda.current_device() else _NO_DEVICE
+
+
+class _NoDevice:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NO_DEVICE = _NoDevice()
+
+
+def _dense_rows(t):
+    """``t`` (B, T, H, D) as the kernels read it: dense channels, every other stride a multiple of 16 bytes and short enough for 32-bit
+    offsets inside a tile, 16-byte aligned; anything else is copied once."""
+    e = 16 // t.element_size()
+    sb, st, sh, sd = t.stride()
+    if t.numel() == 0:
+        return t
+    if (sd != 1 and t.shape[3] > 1) or sb % e or st % e or sh % e or t.data_ptr() % 16 or st > 1 << 21 or sh * t.shape[2] > 1 << 27:
+        return t.contiguous()
+    return t
+
+
+def _attn_check(q, k, v, k_lens, key_mask):
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError("cross_attention: %s must be (batch, positions, heads, channels), got %s" % (name, tuple(t.shape)))
+        if t.dtype != q.dtype or q.dtype not in _ATTN_DTYPES:
+            raise TypeError("cross_attention: float32 or bfloat16 tensors of one type, got %s" % ", ".join(str(x.dtype) for x in (q, k, v)))
+        if t.device != q.device:
+            raise ValueError("cross_attention: tensors on different devices")
+    B, Tq, H, D = q.shape
+    Hk = k.shape[2]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError("cross_attention: q %s, k %s, v %s do not belong together" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if H < 1 or Hk < 1 or H % Hk:
+        raise ValueError("cross_attention: %d query heads do not share %d key heads evenly" % (H, Hk))
+    if D % 8 or not 8 <= D <= 256:
+        raise ValueError("cross_attention: %d channels per head; a multiple of 8 up to 256 is supported" % D)
+    if k_lens is not None:
+        if k_lens.dtype not in (torch.int32, torch.int64):
+            raise TypeError("cross_attention: k_lens must be int32 or int64, got %s" % k_lens.dtype)
+        if tuple(k_lens.shape) != (B,) or k_lens.device != q.device:
+            raise ValueError("cross_attention: k_lens must be (%d,) on %s" % (B, q.device))
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool:
+            raise TypeError("cross_attention: key_mask must be bool (True = the key exists), got %s" % key_mask.dtype)
+        if key_mask.dim() != 2 or key_mask.shape[0] not in (1, B) or key_mask.shape[1] != k.shape[1] or key_mask.device != q.device:
+            raise ValueError("cross_attention: key_mask must be (%d or 1, %d) on %s" % (B, k.shape[1], q.device))
+    ptr(q)                              # (refuses CPU tensors)
+
+
+def _attn_desc(q, k, v, scale, k_lens, key_mask):
+    """ttdg_attention_t without outputs, backward fields and workspace."""
+    a = _lib.Attention()
+    a.q, a.k, a.v = ptr(q), ptr(k), ptr(v)
+    a.q_sb, a.q_st, a.q_sh, _ = q.stride()
+    a.k_sb, a.k_st, a.k_sh, _ = k.stride()
+    a.v_sb, a.v_st, a.v_sh, _ = v.stride()
+    if k_lens is not None:
+        a.k_lens = ptr(k_lens)
+    if key_mask is not None:
+        a.key_mask = ptr(key_mask)
+        a.m_sb, a.m_st = (0 if key_mask.shape[0] == 1 else key_mask.stride(0)), key_mask.stride(1)
+    a.B, a.Tq, a.H, a.D = q.shape
+    a.Tk, a.Hkv, a.dtype, a.scale = k.shape[1], k.shape[2], _ATTN_DTYPES[q.dtype], scale
+    return a
+
+
+def _attn_workspace(a, nbytes, device):
+    if nbytes == 0:
+        return None
+    ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
+    a.ws, a.ws_bytes = ptr(ws), nbytes
+    return ws
+
+
+def _attn_forward(q, k, v, scale, k_lens, key_mask, keep):
+    """-> (out, out_lo, lse); the last two (what a backward needs) are None unless ``keep``."""
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    lse = lo = None
+    if q.numel() == 0:
+        return out, lo, lse
+    a = _attn_desc(q, k, v, scale, k_lens, key_mask)
+    a.out = ptr(out)
+    if keep:
+        lse = torch.empty(a.B * a.Tq * a.H, device=q.device, dtype=torch.float32)
+        a.lse = ptr(lse)
+        if q.dtype != torch.float32:
+            lo = torch.empty_like(out)
+            a.out_lo = ptr(lo)
+    ws = _attn_workspace(a, _lib.load().ttdg_attention_fwd_workspace_bytes(C.byref(a)), q.device)    # noqa: F841 (alive until enqueued)
+    with _timed("attention_fwd", (a.B, a.Tq, a.Tk, a.H, a.Hkv, a.D)):
+        call("ttdg_attention_fwd", C.byref(a), stream())
+    return out, lo, lse
+
+
+class CrossAttentionFn(torch.autograd.Function):
+    """cross_attention with gradients.  Saved: the inputs, the output (with what its rounding dropped) and one float per row."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, scale, k_lens, key_mask):
+        with _on_device_of(q):
+            out, lo, lse = _attn_forward(q, k, v, scale, k_lens, key_mask, True)
+        ctx.save_for_backward(q, k, v, out, lo, lse, k_lens, key_mask)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lo, lse, k_lens, key_mask = ctx.saved_tensors
+        kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        if q.numel() == 0:
+            return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), None, None, None
+        with _on_device_of(q):
+            dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+            dk, dv = (torch.empty(k.shape, device=q.device, dtype=q.dtype) for _ in range(2)) if kv else (None, None)
+            dout = dout.contiguous()
+            if dout.data_ptr() % 16:
+                dout = dout.clone()
+            a = _attn_desc(q, k, v, ctx.scale, k_lens, key_mask)
+            a.out, a.out_lo, a.lse, a.dout, a.dq, a.dk, a.dv = ptr(out), ptr(lo), ptr(lse), ptr(dout), ptr(dq), ptr(dk), ptr(dv)
+            ws = _attn_workspace(a, _lib.load().ttdg_attention_bwd_workspace_bytes(C.byref(a)), q.device)    # noqa: F841
+            with _timed("attention_bwd", (a.B, a.Tq, a.Tk, a.H, a.Hkv, a.D)):
+                call("ttdg_attention_bwd", C.byref(a), stream())
+        return dq, dk, dv, None, None, None
+
+
+def cross_attention(q, k, v, scale=None, k_lens=None, key_mask=None):
+    """Multi-head attention of queries over another set's keys and values (csrc/attention.hip), with gradients.
+
+    q (B, Tq, H, D); k, v (B, Tk, Hk, D), H a multiple of Hk (query head h reads key head h // (H // Hk)); float32 or bfloat16; D a multiple
+    of 8 up to 256; Tq, Tk and B may be zero.  Any strides: slices of a fused projection are read in place (channels dense and every stride
+    a multiple of 16 bytes), other layouts are copied first.  ``scale`` defaults to D ** -0.5.
+    ``k_lens`` (B,) int32 / int64: the keys j < k_lens[b] exist (values are clamped to 0 .. Tk); ``key_mask`` (B or 1, Tk) bool: the keys with
+    True exist.  What stands at other keys - padding, infinities, NaN - never reaches a result; they get zero gradients, and a sample
+    without any key gives zeros.  Returns (B, Tq, H, D), contiguous.  One query per sample (a decoding step) and few queries over many keys
+    take the same call: the keys are then split over the chip and joined.  No second derivatives."""
+    _attn_check(q, k, v, k_lens, key_mask)
+    scale = q.shape[3] ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError("cross_attention: the scale must be positive and finite, got %r" % scale)
+    if k_lens is not None:
+        k_lens = k_lens.to(torch.int32).contiguous()
+    q, k, v = _dense_rows(q), _dense_rows(k), _dense_rows(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return CrossAttentionFn.apply(q, k, v, scale, k_lens, key_mask)
+    with _on_device_of(q):
+        return _attn_forward(q, k, v, scale, k_lens, key_mask, False)[0]
+
+
+# ------------------------------------------------------------------------------------------- per-head norm + rotation
+def rope_frequencies(rot_dim, base=10000.0, axes=1, device=None):
+    """Rotation frequencies of qk_norm_rope: (rot_dim / 2,) float64, one geometric sequence 1 ... base^-1 per position axis."""
+    if rot_dim <= 0 or rot_dim % 8 or axes not in (1, 2):
+        raise ValueError("rope_frequencies: a positive multiple of 8 channels over one or two axes, got %r over %r" % (rot_dim, axes))
+    n = rot_dim // 2 // axes
+    f = float(base) ** (-torch.arange(n, device=device, dtype=torch.float64) / n)
+    return f.repeat(axes)
+
+
+def _qkn_check(q, k, q_weight, k_weight, freq, q_pos, k_pos):
+    R = 0 if freq is None else 2 * freq.numel()
+    axes = 1
+    if freq is not None:
+        if freq.dtype != torch.float64 or freq.dim() != 1 or freq.device != q.device:
+            raise TypeError("qk_norm_rope: frequencies must be a float64 vector on %s" % q.device)
+        if q_pos is None:
+            raise ValueError("qk_norm_rope: a rotation needs positions")
+        axes = 1 if q_pos.dim() == 2 else 2
+    for name, x, w, pos in (("q", q, q_weight, q_pos), ("k", k, k_weight, k_pos)):
+        if x is None:
+            if w is not None or (pos is not None and name == "k" and pos is not q_pos):
+                raise ValueError("qk_norm_rope: a weight or positions for keys, but no keys")
+            continue
+        if x.dim() != 4:
+            raise ValueError("qk_norm_rope: %s must be (batch, positions, heads, channels), got %s" % (name, tuple(x.shape)))
+        if x.dtype != q.dtype or q.dtype not in _ATTN_DTYPES:
+            raise TypeError("qk_norm_rope: float32 or bfloat16 tensors of one type, got %s and %s" % (q.dtype, x.dtype))
+        if x.device != q.device or x.shape[0] != q.shape[0] or x.shape[3] != q.shape[3]:
+            raise ValueError("qk_norm_rope: q %s and k %s do not belong together" % (tuple(q.shape), tuple(x.shape)))
+        D = x.shape[3]
+        if D % 8 or not 8 <= D <= 256 or R > D or R % 8:
+            raise ValueError("qk_norm_rope: %d channels per head, %d of them rotated; multiples of 8 up to 256 are supported" % (D, R))
+        if w is None or w.dtype != torch.float32 or tuple(w.shape) != (D,) or w.device != q.device:
+            raise TypeError("qk_norm_rope: the weight of %s must be float32 (%d,) on %s" % (name, D, q.device))
+        if freq is None:
+            continue
+        if pos is None or pos.dtype not in (torch.int32, torch.int64) or pos.dtype != q_pos.dtype:
+            raise TypeError("qk_norm_rope: positions must be int32 or int64, the same for queries and keys")
+        if pos.dim() != q_pos.dim() or pos.dim() not in (2, 3) or pos.shape[0] not in (1, x.shape[0]) or pos.shape[1] != x.shape[1] or \
+                (pos.dim() == 3 and pos.shape[2] != 2) or pos.device != q.device:
+            raise ValueError("qk_norm_rope: positions of %s must be (%d or 1, %d) or (.., .., 2) on %s, got %s" %
+                             (name, x.shape[0], x.shape[1], q.device, tuple(pos.shape)))
+    ptr(q)                              # (refuses CPU tensors)
+    return axes
+
+
+def _qkn_side(s, x, w, pos):
+    s.x, s.T, s.H, s.w = ptr(x), x.shape[1], x.shape[2], ptr(w)
+    s.sb, s.st, s.sh, _ = x.stride()
+    if pos is not None:
+        s.pos = ptr(pos)
+        s.p_sb, s.p_st = (0 if pos.shape[0] == 1 else pos.stride(0)), pos.stride(1)
+        s.p_sa = pos.stride(2) if pos.dim() == 3 else 0
+
+
+def _qkn_desc(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, eps, interleaved):
+    a = _lib.QkNormRope()
+    _qkn_side(a.q, q, q_weight, q_pos)
+    if k is not None:
+        _qkn_side(a.k, k, k_weight, k_pos)
+    a.B, a.D, a.axes, a.interleaved, a.dtype, a.eps = q.shape[0], q.shape[3], axes, int(bool(interleaved)), _ATTN_DTYPES[q.dtype], eps
+    if freq is not None:
+        a.R, a.freq, a.pos64 = 2 * freq.numel(), ptr(freq), int(q_pos.dtype == torch.int64)
+    return a
+
+
+def _qkn_forward(a, q, k):
+    yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    yk = None if k is None else torch.empty(k.shape, device=q.device, dtype=q.dtype)
+    a.q.y, a.k.y = ptr(yq), ptr(yk)
+    with _timed("qk_norm_rope_fwd", 2 * (yq.numel() + (0 if yk is None else yk.numel())) * yq.element_size()):      # algorithmic bytes
+        call("ttdg_qk_norm_rope_fwd", C.byref(a), stream())
+    return yq, yk
+
+
+class QkNormRopeFn(torch.autograd.Function):
+    """qk_norm_rope with gradients; the backward recomputes the norms from the saved inputs."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, eps, interleaved):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(q, k, q_weight, k_weight, freq, q_pos, k_pos)
+        ctx.args = (axes, eps, interleaved)
+        with _on_device_of(q):
+            return _qkn_forward(_qkn_desc(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, eps, interleaved), q, k)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, q_weight, k_weight, freq, q_pos, k_pos = ctx.saved_tensors
+        with _on_device_of(q):
+            a = _qkn_desc(q, k, q_weight, k_weight, freq, q_pos, k_pos, *ctx.args)
+            keep = []
+
+            def side(s, x, g):
+                if x is None:
+                    return None, None
+                if g is None:
+                    g = torch.zeros(x.shape, device=x.device, dtype=x.dtype)
+                g = g.contiguous()
+                if g.data_ptr() % 16:
+                    g = g.clone()
+                dx, dw = torch.empty(x.shape, device=x.device, dtype=x.dtype), torch.empty(x.shape[3], device=x.device, dtype=torch.float32)
+                s.dy, s.dx, s.dw = ptr(g), ptr(dx), ptr(dw)
+                keep.append(g)
+                return dx, dw
+
+            dq, dwq = side(a.q, q, gq)
+            dk, dwk = side(a.k, k, gk)
+            ws = _attn_workspace(a, _lib.load().ttdg_qk_norm_rope_bwd_workspace_bytes(C.byref(a)), q.device)      # noqa: F841
+            with _timed("qk_norm_rope_bwd", 3 * (q.numel() + (0 if k is None else k.numel())) * q.element_size()):
+                call("ttdg_qk_norm_rope_bwd", C.byref(a), stream())
+        return dq, dk, dwq, dwk, None, None, None, None, None, None
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, freq=None, q_pos=None, k_pos=None, eps=1e-6, interleaved=False):
+    """RMS norm of every head of the queries and keys, scaled by a weight per channel, then rotated by their positions, in one pass over
+    both (csrc/qk_norm.hip), with gradients.
+
+    q (B, Tq, H, D) and k (B, Tk, Hk, D) or None (a decoding step over keys that are kept: then k_weight is None too), float32 or bfloat16,
+    any strides (see cross_attention); weights (D,) float32.  ``freq`` (R / 2,) float64, see ``rope_frequencies``: the pairs of the first R
+    channels - (i, i + R / 2), or (2 i, 2 i + 1) with ``interleaved`` - turn by position * freq[i]; None: no rotation.  Positions
+    (B or 1, T) int32 / int64, or (B or 1, T, 2) for two coordinates: the first half of the pairs turns by the first one.  ``k_pos`` defaults
+    to ``q_pos``.  D and R are multiples of 8, D up to 256.  Returns (q', k'), contiguous; k' is None without k.  No second derivatives."""
+    if freq is not None and k is not None and k_pos is None:
+        k_pos = q_pos
+    axes = _qkn_check(q, k, q_weight, k_weight, freq, q_pos, k_pos)
+    if not eps >= 0.0:
+        raise ValueError("qk_norm_rope: eps must not be negative, got %r" % eps)
+    if freq is None:
+        q_pos = k_pos = None
+    else:
+        freq = freq.contiguous()
+    q, k = _dense_rows(q), None if k is None else _dense_rows(k)
+    q_weight, k_weight = _dense_weight(q_weight), None if k is None else _dense_weight(k_weight)
+    ts = (q, k, q_weight, k_weight)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        return QkNormRopeFn.apply(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, float(eps), interleaved)
+    with _on_device_of(q):
+        return _qkn_forward(_qkn_desc(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, float(eps), interleaved), q, k)
+
+
+def _dense_weight(w):
+    w = w.contiguous()
+    return w if w.data_ptr() % 16 == 0 else w.clone()
+
+
 def gagm_cfg(tau0=0.1, gamma=0.5, min_tau=1e-2, tol=1e-3, quad_weight=0.5, max_iter=200, sk_iter=20,
              max_stages=0, start_hungarian=False, profile=False, no_cycle_skip=False, variant=0):
     c = _lib.GagmCfg()
