@@ -224,7 +224,8 @@ def ptr(t):
 
 
 def stream():
-    return torch.cuda.current_stream().cuda_stream
+    """torch's current stream of the current device as a hipStream_t (the raw handle: 0.2 us instead of 2.8 us for a Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def call(name, *args):

@@ -414,11 +414,6 @@ def mha_adjacency(q, k, gr, sizes, scale, drop_p=0.0, seed=0, zero_diag=True):
 _ATTN_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
 
-def _on_device_of(t):
-    """The kernels run on the current stream of the device the tensors live on, whatever device is current."""
-    return torch.cuda.device(t.device) if t.is_cuda and t.device.index != torch.cuda.current_device() else _NO_DEVICE
-
-
 class _NoDevice:
     def __enter__(self):
         return self
@@ -430,29 +425,44 @@ class _NoDevice:
 _NO_DEVICE = _NoDevice()
 
 
+def _on_device_of(t):
+    """The kernels run on the current stream of the device the tensors live on, whatever device is current."""
+    return _NO_DEVICE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def _timed_call(name, arg, timer, meta):
+    """call(name, byref(arg), stream()), stamped when bench.py asks for it (the usual case stays free of the context manager)."""
+    if KERNEL_TIMERS is None:
+        call(name, C.byref(arg), stream())
+    else:
+        with _timed(timer, meta):
+            call(name, C.byref(arg), stream())
+
+
+def _like(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _dense_rows(t):
     """``t`` (B, T, H, D) as the kernels read it: dense channels, every other stride a multiple of 16 bytes and short enough for 32-bit
     offsets inside a tile, 16-byte aligned; anything else is copied once."""
-    e = 16 // t.element_size()
     sb, st, sh, sd = t.stride()
-    if t.numel() == 0:
-        return t
-    if (sd != 1 and t.shape[3] > 1) or sb % e or st % e or sh % e or t.data_ptr() % 16 or st > 1 << 21 or sh * t.shape[2] > 1 << 27:
-        return t.contiguous()
+    if sd != 1 or (sb | st | sh) * t.element_size() & 15 or t.data_ptr() & 15 or st > 1 << 21 or sh * t.shape[2] > 1 << 27:
+        return t if t.numel() == 0 else t.contiguous()
     return t
 
 
 def _attn_check(q, k, v, k_lens, key_mask):
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
-            raise ValueError("cross_attention: %s must be (batch, positions, heads, channels), got %s" % (name, tuple(t.shape)))
-        if t.dtype != q.dtype or q.dtype not in _ATTN_DTYPES:
-            raise TypeError("cross_attention: float32 or bfloat16 tensors of one type, got %s" % ", ".join(str(x.dtype) for x in (q, k, v)))
-        if t.device != q.device:
-            raise ValueError("cross_attention: tensors on different devices")
-    B, Tq, H, D = q.shape
-    Hk = k.shape[2]
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+    dt, dev = q.dtype, q.device
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("cross_attention: q, k and v must be (batch, positions, heads, channels), got %s" % (tuple(tuple(t.shape) for t in (q, k, v)),))
+    if dt not in _ATTN_DTYPES or k.dtype != dt or v.dtype != dt:
+        raise TypeError("cross_attention: float32 or bfloat16 tensors of one type, got %s" % ", ".join(str(x.dtype) for x in (q, k, v)))
+    if k.device != dev or v.device != dev:
+        raise ValueError("cross_attention: tensors on different devices")
+    B, _, H, D = q.shape
+    Bk, Tk, Hk, Dk = k.shape
+    if k.shape != v.shape or Bk != B or Dk != D:
         raise ValueError("cross_attention: q %s, k %s, v %s do not belong together" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     if H < 1 or Hk < 1 or H % Hk:
         raise ValueError("cross_attention: %d query heads do not share %d key heads evenly" % (H, Hk))
@@ -461,59 +471,57 @@ def _attn_check(q, k, v, k_lens, key_mask):
     if k_lens is not None:
         if k_lens.dtype not in (torch.int32, torch.int64):
             raise TypeError("cross_attention: k_lens must be int32 or int64, got %s" % k_lens.dtype)
-        if tuple(k_lens.shape) != (B,) or k_lens.device != q.device:
-            raise ValueError("cross_attention: k_lens must be (%d,) on %s" % (B, q.device))
+        if k_lens.dim() != 1 or k_lens.shape[0] != B or k_lens.device != dev:
+            raise ValueError("cross_attention: k_lens must be (%d,) on %s" % (B, dev))
     if key_mask is not None:
         if key_mask.dtype != torch.bool:
             raise TypeError("cross_attention: key_mask must be bool (True = the key exists), got %s" % key_mask.dtype)
-        if key_mask.dim() != 2 or key_mask.shape[0] not in (1, B) or key_mask.shape[1] != k.shape[1] or key_mask.device != q.device:
-            raise ValueError("cross_attention: key_mask must be (%d or 1, %d) on %s" % (B, k.shape[1], q.device))
-    ptr(q)                              # (refuses CPU tensors)
+        if key_mask.dim() != 2 or key_mask.shape[0] not in (1, B) or key_mask.shape[1] != Tk or key_mask.device != dev:
+            raise ValueError("cross_attention: key_mask must be (%d or 1, %d) on %s" % (B, Tk, dev))
+    if not q.is_cuda:
+        ptr(q)                          # raises: no CPU fallback
 
 
-def _attn_desc(q, k, v, scale, k_lens, key_mask):
-    """ttdg_attention_t without outputs, backward fields and workspace."""
-    a = _lib.Attention()
-    a.q, a.k, a.v = ptr(q), ptr(k), ptr(v)
-    a.q_sb, a.q_st, a.q_sh, _ = q.stride()
-    a.k_sb, a.k_st, a.k_sh, _ = k.stride()
-    a.v_sb, a.v_st, a.v_sh, _ = v.stride()
-    if k_lens is not None:
-        a.k_lens = ptr(k_lens)
+def _attn_desc(q, k, v, scale, k_lens, key_mask, out=None, out_lo=None, lse=None, dout=None, dq=None, dk=None, dv=None):
+    """ttdg_attention_t without a workspace (positional: the field order of the struct)."""
+    B, Tq, H, D = q.shape
+    qb, qt, qh, _ = q.stride()
+    kb, kt, kh, _ = k.stride()
+    vb, vt, vh, _ = v.stride()
+    mask, mb, mt = None, 0, 0
     if key_mask is not None:
-        a.key_mask = ptr(key_mask)
-        a.m_sb, a.m_st = (0 if key_mask.shape[0] == 1 else key_mask.stride(0)), key_mask.stride(1)
-    a.B, a.Tq, a.H, a.D = q.shape
-    a.Tk, a.Hkv, a.dtype, a.scale = k.shape[1], k.shape[2], _ATTN_DTYPES[q.dtype], scale
-    return a
+        mask, mb, mt = key_mask.data_ptr(), (0 if key_mask.shape[0] == 1 else key_mask.stride(0)), key_mask.stride(1)
+    return _lib.Attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), qb, qt, qh, kb, kt, kh, vb, vt, vh, None if k_lens is None else k_lens.data_ptr(),
+                          mask, mb, mt, B, Tq, k.shape[1], H, k.shape[2], D, _ATTN_DTYPES[q.dtype], scale, ptr(out), ptr(out_lo), ptr(lse), ptr(dout),
+                          ptr(dq), ptr(dk), ptr(dv))
 
 
 def _attn_workspace(a, nbytes, device):
     if nbytes == 0:
         return None
     ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
-    a.ws, a.ws_bytes = ptr(ws), nbytes
+    a.ws, a.ws_bytes = ws.data_ptr(), nbytes
     return ws
 
 
 def _attn_forward(q, k, v, scale, k_lens, key_mask, keep):
     """-> (out, out_lo, lse); the last two (what a backward needs) are None unless ``keep``."""
-    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    out = _like(q)
     lse = lo = None
     if q.numel() == 0:
         return out, lo, lse
-    a = _attn_desc(q, k, v, scale, k_lens, key_mask)
-    a.out = ptr(out)
     if keep:
-        lse = torch.empty(a.B * a.Tq * a.H, device=q.device, dtype=torch.float32)
-        a.lse = ptr(lse)
-        if q.dtype != torch.float32:
-            lo = torch.empty_like(out)
-            a.out_lo = ptr(lo)
+        lse = torch.empty(q.shape[0] * q.shape[1] * q.shape[2], device=q.device, dtype=torch.float32)
+        lo = None if q.dtype == torch.float32 else _like(q)
+    a = _attn_desc(q, k, v, scale, k_lens, key_mask, out, lo, lse)
     ws = _attn_workspace(a, _lib.load().ttdg_attention_fwd_workspace_bytes(C.byref(a)), q.device)    # noqa: F841 (alive until enqueued)
-    with _timed("attention_fwd", (a.B, a.Tq, a.Tk, a.H, a.Hkv, a.D)):
-        call("ttdg_attention_fwd", C.byref(a), stream())
+    _timed_call("ttdg_attention_fwd", a, "attention_fwd", q.shape + k.shape[1:3])
     return out, lo, lse
+
+
+def _dense_grad(g):
+    g = g.contiguous()
+    return g.clone() if g.data_ptr() & 15 else g
 
 
 class CrossAttentionFn(torch.autograd.Function):
@@ -535,16 +543,12 @@ class CrossAttentionFn(torch.autograd.Function):
         if q.numel() == 0:
             return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), None, None, None
         with _on_device_of(q):
-            dq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-            dk, dv = (torch.empty(k.shape, device=q.device, dtype=q.dtype) for _ in range(2)) if kv else (None, None)
-            dout = dout.contiguous()
-            if dout.data_ptr() % 16:
-                dout = dout.clone()
-            a = _attn_desc(q, k, v, ctx.scale, k_lens, key_mask)
-            a.out, a.out_lo, a.lse, a.dout, a.dq, a.dk, a.dv = ptr(out), ptr(lo), ptr(lse), ptr(dout), ptr(dq), ptr(dk), ptr(dv)
+            dq = _like(q)
+            dk, dv = (_like(k), _like(k)) if kv else (None, None)
+            dout = _dense_grad(dout)
+            a = _attn_desc(q, k, v, ctx.scale, k_lens, key_mask, out, lo, lse, dout, dq, dk, dv)
             ws = _attn_workspace(a, _lib.load().ttdg_attention_bwd_workspace_bytes(C.byref(a)), q.device)    # noqa: F841
-            with _timed("attention_bwd", (a.B, a.Tq, a.Tk, a.H, a.Hkv, a.D)):
-                call("ttdg_attention_bwd", C.byref(a), stream())
+            _timed_call("ttdg_attention_bwd", a, "attention_bwd", q.shape + k.shape[1:3])
         return dq, dk, dv, None, None, None
 
 
@@ -562,7 +566,7 @@ def cross_attention(q, k, v, scale=None, k_lens=None, key_mask=None):
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
         raise ValueError("cross_attention: the scale must be positive and finite, got %r" % scale)
-    if k_lens is not None:
+    if k_lens is not None and (k_lens.dtype != torch.int32 or not k_lens.is_contiguous()):
         k_lens = k_lens.to(torch.int32).contiguous()
     q, k, v = _dense_rows(q), _dense_rows(k), _dense_rows(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -618,32 +622,31 @@ def _qkn_check(q, k, q_weight, k_weight, freq, q_pos, k_pos):
     return axes
 
 
-def _qkn_side(s, x, w, pos):
-    s.x, s.T, s.H, s.w = ptr(x), x.shape[1], x.shape[2], ptr(w)
-    s.sb, s.st, s.sh, _ = x.stride()
+def _qkn_side(x, w, pos, y, dy, dx, dw):
+    """ttdg_norm_rope_side_t (positional)"""
+    if x is None:
+        return _lib.NormRopeSide()
+    _, T, H, _ = x.shape
+    sb, st, sh, _ = x.stride()
+    at, pb, pt, pa = None, 0, 0, 0
     if pos is not None:
-        s.pos = ptr(pos)
-        s.p_sb, s.p_st = (0 if pos.shape[0] == 1 else pos.stride(0)), pos.stride(1)
-        s.p_sa = pos.stride(2) if pos.dim() == 3 else 0
+        at, pb, pt = pos.data_ptr(), (0 if pos.shape[0] == 1 else pos.stride(0)), pos.stride(1)
+        pa = pos.stride(2) if pos.dim() == 3 else 0
+    return _lib.NormRopeSide(x.data_ptr(), sb, st, sh, T, H, w.data_ptr(), at, pb, pt, pa, ptr(y), ptr(dy), ptr(dx), ptr(dw))
 
 
-def _qkn_desc(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, eps, interleaved):
-    a = _lib.QkNormRope()
-    _qkn_side(a.q, q, q_weight, q_pos)
-    if k is not None:
-        _qkn_side(a.k, k, k_weight, k_pos)
-    a.B, a.D, a.axes, a.interleaved, a.dtype, a.eps = q.shape[0], q.shape[3], axes, int(bool(interleaved)), _ATTN_DTYPES[q.dtype], eps
-    if freq is not None:
-        a.R, a.freq, a.pos64 = 2 * freq.numel(), ptr(freq), int(q_pos.dtype == torch.int64)
-    return a
+def _qkn_desc(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, eps, interleaved, outs=(None, None), grads=(None,) * 6):
+    """ttdg_qk_norm_rope_t without a workspace; grads: dy, dx, dw of the queries, then of the keys"""
+    R, at, wide = (0, None, 0) if freq is None else (2 * freq.numel(), freq.data_ptr(), int(q_pos.dtype == torch.int64))
+    return _lib.QkNormRope(_qkn_side(q, q_weight, q_pos, outs[0], *grads[:3]), _qkn_side(k, k_weight, k_pos, outs[1], *grads[3:]), at, q.shape[0],
+                           q.shape[3], R, axes, interleaved, wide, _ATTN_DTYPES[q.dtype], eps)
 
 
-def _qkn_forward(a, q, k):
-    yq = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    yk = None if k is None else torch.empty(k.shape, device=q.device, dtype=q.dtype)
-    a.q.y, a.k.y = ptr(yq), ptr(yk)
-    with _timed("qk_norm_rope_fwd", 2 * (yq.numel() + (0 if yk is None else yk.numel())) * yq.element_size()):      # algorithmic bytes
-        call("ttdg_qk_norm_rope_fwd", C.byref(a), stream())
+def _qkn_forward(q, k, *args):
+    yq = _like(q)
+    yk = None if k is None else _like(k)
+    a = _qkn_desc(q, k, *args, outs=(yq, yk))
+    _timed_call("ttdg_qk_norm_rope_fwd", a, "qk_norm_rope_fwd", 2 * (yq.numel() + (0 if yk is None else yk.numel())) * yq.element_size())   # algorithmic bytes
     return yq, yk
 
 
@@ -656,34 +659,22 @@ class QkNormRopeFn(torch.autograd.Function):
         ctx.save_for_backward(q, k, q_weight, k_weight, freq, q_pos, k_pos)
         ctx.args = (axes, eps, interleaved)
         with _on_device_of(q):
-            return _qkn_forward(_qkn_desc(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, eps, interleaved), q, k)
+            return _qkn_forward(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, eps, interleaved)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, freq, q_pos, k_pos = ctx.saved_tensors
+        dq = dk = dwq = dwk = None
         with _on_device_of(q):
-            a = _qkn_desc(q, k, q_weight, k_weight, freq, q_pos, k_pos, *ctx.args)
-            keep = []
-
-            def side(s, x, g):
-                if x is None:
-                    return None, None
-                if g is None:
-                    g = torch.zeros(x.shape, device=x.device, dtype=x.dtype)
-                g = g.contiguous()
-                if g.data_ptr() % 16:
-                    g = g.clone()
-                dx, dw = torch.empty(x.shape, device=x.device, dtype=x.dtype), torch.empty(x.shape[3], device=x.device, dtype=torch.float32)
-                s.dy, s.dx, s.dw = ptr(g), ptr(dx), ptr(dw)
-                keep.append(g)
-                return dx, dw
-
-            dq, dwq = side(a.q, q, gq)
-            dk, dwk = side(a.k, k, gk)
+            gq = _dense_grad(gq) if gq is not None else torch.zeros(q.shape, device=q.device, dtype=q.dtype)     # (an output nobody used)
+            dq, dwq = _like(q), _like(q_weight)
+            if k is not None:
+                gk = _dense_grad(gk) if gk is not None else torch.zeros(k.shape, device=k.device, dtype=k.dtype)
+                dk, dwk = _like(k), _like(k_weight)
+            a = _qkn_desc(q, k, q_weight, k_weight, freq, q_pos, k_pos, *ctx.args, grads=(gq, dq, dwq, gk, dk, dwk))
             ws = _attn_workspace(a, _lib.load().ttdg_qk_norm_rope_bwd_workspace_bytes(C.byref(a)), q.device)      # noqa: F841
-            with _timed("qk_norm_rope_bwd", 3 * (q.numel() + (0 if k is None else k.numel())) * q.element_size()):
-                call("ttdg_qk_norm_rope_bwd", C.byref(a), stream())
+            _timed_call("ttdg_qk_norm_rope_bwd", a, "qk_norm_rope_bwd", 3 * (q.numel() + (0 if k is None else k.numel())) * q.element_size())
         return dq, dk, dwq, dwk, None, None, None, None, None, None
 
 
@@ -707,16 +698,16 @@ def qk_norm_rope(q, k, q_weight, k_weight, freq=None, q_pos=None, k_pos=None, ep
         freq = freq.contiguous()
     q, k = _dense_rows(q), None if k is None else _dense_rows(k)
     q_weight, k_weight = _dense_weight(q_weight), None if k is None else _dense_weight(k_weight)
-    ts = (q, k, q_weight, k_weight)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        return QkNormRopeFn.apply(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, float(eps), interleaved)
+    args = (q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, float(eps), int(bool(interleaved)))
+    if torch.is_grad_enabled() and (q.requires_grad or q_weight.requires_grad or (k is not None and (k.requires_grad or k_weight.requires_grad))):
+        return QkNormRopeFn.apply(*args)
     with _on_device_of(q):
-        return _qkn_forward(_qkn_desc(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, float(eps), interleaved), q, k)
+        return _qkn_forward(*args)
 
 
 def _dense_weight(w):
     w = w.contiguous()
-    return w if w.data_ptr() % 16 == 0 else w.clone()
+    return w.clone() if w.data_ptr() & 15 else w
 
 
 def gagm_cfg(tau0=0.1, gamma=0.5, min_tau=1e-2, tol=1e-3, quad_weight=0.5, max_iter=200, sk_iter=20,
