@@ -62,12 +62,6 @@ __device__ __forceinline__ void attn_dma4(__amdgpu_buffer_rsrc_t r, char* lds_wa
 
 __device__ __forceinline__ void attn_store4(float* out, f32x4 x) { *(f32x4*)out = x; }
 __device__ __forceinline__ void attn_store4(__bf16* out, f32x4 x) { *(bf16x4*)out = __builtin_convertvector(x, bf16x4); }
-__device__ __forceinline__ void attn_store1(float* out, float*, int64_t i, float x) { out[i] = x; }
-__device__ __forceinline__ void attn_store1(__bf16* out, __bf16* lo, int64_t i, float x) {
-  const __bf16 hi = (__bf16)x;
-  out[i] = hi;
-  if (lo) lo[i] = (__bf16)(x - (float)hi);
-}
 
 // workgroup -> (problem, tile, split).  Consecutive tiles of one split read the same keys; workgroups are dealt to the eight XCDs in turn,
 // so XCD x takes a contiguous run of that order and its L2 sees each key tile once.

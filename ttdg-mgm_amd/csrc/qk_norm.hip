@@ -29,6 +29,8 @@ struct qkn_vec {
   static __device__ __forceinline__ void store(T* p, f32 x) { *(mem*)p = __builtin_convertvector(x, mem); }
 };
 
+#define QKN_MAX_BLOCKS 1024           // persistent workgroups of the backward, per side
+
 struct qkn_side {
   const void *x, *pos, *dy;
   int64_t sb, st, sh, p_sb, p_st, p_sa;
@@ -232,27 +234,25 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(qkn_args p) {
   }
 }
 
-// dw[c] = sum over the workgroups' partial rows, in a fixed order: 16 threads per channel, then their sums
+// dw[c] = sum over the workgroups' partial rows, in a fixed order: a workgroup takes four channels, a thread every 256th row of them
 __global__ __launch_bounds__(256) void qk_norm_rope_dw_kernel(const float* __restrict__ part, int nq, int nk, int D, float* __restrict__ dwq,
                                                               float* __restrict__ dwk) {
-  __shared__ float red[256];
-  const int side = blockIdx.y, c = blockIdx.x * 16 + (threadIdx.x & 15), k = threadIdx.x >> 4;
+  __shared__ f32x4 red[4];
+  const int side = blockIdx.y, c = blockIdx.x * 4;
   const int n = side ? nk : nq;
-  const float* p = part + (side ? (int64_t)nq * D : 0);
-  float a = 0.f;
-  if (c < D)
-    for (int i = k; i < n; i += 16) a += p[(int64_t)i * D + c];
-  red[threadIdx.x] = a;
+  const float* p = part + (side ? (int64_t)nq * D : 0) + c;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < QKN_MAX_BLOCKS; i += 256)
+    if (i + threadIdx.x < n) a += *(const f32x4*)(p + (int64_t)(i + threadIdx.x) * D);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) a[e] = wave_sum(a[e]);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
   __syncthreads();
-  if (k == 0 && c < D) {
-    for (int i = 1; i < 16; ++i) a += red[i * 16 + (threadIdx.x & 15)];
-    (side ? dwk : dwq)[c] = a;
-  }
+  if (threadIdx.x < 4) (side ? dwk : dwq)[c + threadIdx.x] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
-#define QKN_MAX_BLOCKS 1024           // persistent workgroups of the backward: four per CU
-
 static int qkn_check(const ttdg_qk_norm_rope_t* a) {
   TTDG_REQUIRE(a->dtype == TTDG_F32 || a->dtype == TTDG_BF16, "qk_norm_rope: dtype must be TTDG_F32 or TTDG_BF16");
   TTDG_REQUIRE(a->B >= 0 && a->D >= 8 && a->D <= 256 && a->D % 8 == 0, "qk_norm_rope: the head dimension must be a multiple of 8 up to 256");
@@ -346,7 +346,7 @@ extern "C" int ttdg_qk_norm_rope_bwd(const ttdg_qk_norm_rope_t* a, ttdg_stream_t
     if (int e = ttdg_launch_status("qk_norm_rope_bwd")) return e;
   }
   const int sides = a->k.H ? 2 : 1;
-  hipLaunchKernelGGL(qk_norm_rope_dw_kernel, dim3((a->D + 15) / 16, sides), dim3(256), 0, (hipStream_t)stream, p.part, p.s[0].blocks, p.s[1].blocks, a->D,
+  hipLaunchKernelGGL(qk_norm_rope_dw_kernel, dim3(a->D / 4, sides), dim3(256), 0, (hipStream_t)stream, p.part, p.s[0].blocks, p.s[1].blocks, a->D,
                      a->q.dw, a->k.dw);
   return ttdg_launch_status("qk_norm_rope_dw");
 }
