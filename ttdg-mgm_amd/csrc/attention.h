@@ -164,12 +164,16 @@ struct attn_tile {
     }
   }
 
-  // acc[tile row][lane's row of f] += sum_d tile[row0 + .][d] f[d]
-  static __device__ __forceinline__ void row_product(f32x16& acc, const char* tile, int row0, const frag* f, int l32, int h) {
+  // acc[n][tile row][lane's row of f[n]] += sum_d tile[row0 + .][d] f[n][d]: every chunk read from LDS serves the NB blocks of columns
+  template <int NB>
+  static __device__ __forceinline__ void row_product(f32x16* acc, const char* tile, int row0, const frag (*f)[NP], int l32, int h) {
     const int base = l32 * RB + ((h ^ attn_swz(l32)) << 4);
 #pragma unroll
-    for (int i = 0; i < NP; ++i)
-      acc = mma(*(const frag*)(tile + row0 * RB + (base ^ (32 * (i & 3))) + 128 * (i >> 2)), f[i], acc);
+    for (int i = 0; i < NP; ++i) {
+      const frag a = *(const frag*)(tile + row0 * RB + (base ^ (32 * (i & 3))) + 128 * (i >> 2));
+#pragma unroll
+      for (int n = 0; n < NB; ++n) acc[n] = mma(a, f[n][i], acc[n]);
+    }
   }
   // the same with the second operand read from memory
   static __device__ __forceinline__ void row_product_mem(f32x16& acc, const char* tile, int row0, const T* row, int D, int l32, int h) {
@@ -183,10 +187,11 @@ struct attn_tile {
     }
   }
 
-  // acc[d][lane's column] += sum over the 32 tile rows from row0 of tile[.][d] p[.], p in accumulator layout.  For 16-bit types p is
+  // acc[n][d][lane's column] += sum over the 32 tile rows from row0 of tile[.][d] p[n][.], p in accumulator layout.  For 16-bit types p is
   // rounded to the inputs' type (round to nearest even, as every operand of the matrix unit is): an error of at most half a step per
   // term, independent from term to term, while the sums stay in 32 bits.
-  static __device__ __forceinline__ void col_product(f32x16* acc, const char* tile, int row0, const f32x16& p, int lane) {
+  template <int NB>
+  static __device__ __forceinline__ void col_product(f32x16 (*acc)[DP / 32], const char* tile, int row0, const f32x16* p, int lane) {
     const int h = lane >> 5;
     if constexpr (F32) {
       const int l32 = lane & 31;
@@ -195,24 +200,33 @@ struct attn_tile {
         const int row = attn_reg_row(e) + 4 * h;
         const char* a = tile + (row0 + row) * RB + (((l32 >> 2) ^ (((e & 3) << 1) | h)) << 4) + 4 * (l32 & 3);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*(const float*)(a + 128 * d), p[e], acc[d], 0, 0, 0);
+        for (int d = 0; d < DP / 32; ++d) {
+          const float x = *(const float*)(a + 128 * d);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) acc[n][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[n][e], acc[n][d], 0, 0, 0);
+        }
       }
     } else {
       const int i = lane & 15, blk = (lane >> 4) & 1, row = 4 * h + (i >> 2);
       const int base = row * RB + (((2 * blk + ((i & 3) >> 1)) ^ attn_swz(row)) << 4) + 8 * (i & 1);
 #pragma unroll
       for (int kg = 0; kg < 2; ++kg) {
-        f32x8 x;
+        bf16x8 b[NB];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = p[8 * kg + e];
-        const bf16x8 b = __builtin_convertvector(x, bf16x8);
+        for (int n = 0; n < NB; ++n) {
+          f32x8 x;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = p[n][8 * kg + e];
+          b[n] = __builtin_convertvector(x, bf16x8);
+        }
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
           const char* a = tile + (row0 + 16 * kg) * RB + (base ^ (64 * (d & 1))) + 128 * (d >> 1);
           const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)a);
           const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(a + 8 * RB));
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b, acc[d], 0, 0, 0);
+          const bf16x8 f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) acc[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, b[n], acc[n][d], 0, 0, 0);
         }
       }
     }

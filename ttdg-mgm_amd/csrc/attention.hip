@@ -73,7 +73,7 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
 #pragma unroll
     for (int kk = 0; kk < BN / 32; ++kk) {
       s[kk] = f32x16_zero();
-      tile_t::row_product(s[kk], kt, 32 * kk, qf, l32, h);
+      tile_t::template row_product<1>(&s[kk], kt, 32 * kk, &qf, l32, h);
     }
     if (live != attn_all<BN>()) {
 #pragma unroll
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
         s[kk][e] = x;
         l += x;
       }
-      tile_t::col_product(o, vt, 32 * kk, s[kk], lane);
+      tile_t::template col_product<1>(&o, vt, 32 * kk, &s[kk], lane);
     }
   }
   l = attn_half_sum(l);
@@ -243,15 +243,15 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
 #pragma unroll
     for (int kk = 0; kk < BN / 32; ++kk) {
       f32x16 s = f32x16_zero(), dp = f32x16_zero();
-      tile_t::row_product(s, kt, 32 * kk, qf, l32, h);
-      tile_t::row_product(dp, vt, 32 * kk, gf, l32, h);
+      tile_t::template row_product<1>(&s, kt, 32 * kk, &qf, l32, h);
+      tile_t::template row_product<1>(&dp, vt, 32 * kk, &gf, l32, h);
       const uint32_t bits = (uint32_t)(live >> (32 * kk)) >> (4 * h);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const float pr = fast_exp2(fmaf(s[e], p.scale_log2, -lse));
         s[e] = ((bits >> attn_reg_row(e)) & 1) ? pr * (dp[e] - delta) : 0.f;
       }
-      tile_t::col_product(acc, kt, 32 * kk, s, lane);
+      tile_t::template col_product<1>(&acc, kt, 32 * kk, &s, lane);
     }
   }
   if (row >= p.R) return;
@@ -259,11 +259,11 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
   else tile_t::store_row(acc, p.scale, (T*)p.dq + off, (T*)nullptr, p.D, h);
 }
 
-// dk and dv: a wavefront owns 32 keys, their k and v rows in registers (REGS) or re-read through the caches (the registers of float32 with
-// 256 channels are full of the two sums), and walks over the rows; q and do tiles in LDS serve both as rows (scores) and, transposed, as
-// the second products' first operand.
-template <typename T, int DP, int BQ, int WM, bool REGS>
-__global__ __launch_bounds__(64 * WM, 1) void attn_bwd_dkv_kernel(attn_args p) {
+// dk and dv: a wavefront owns 32 NB keys, their k and v rows in registers (REGS) or re-read through the caches (the registers of float32
+// with 256 channels are full of the two sums), and walks over the rows; q and do tiles in LDS serve both as rows (scores) and, transposed,
+// as the second products' first operand.
+template <typename T, int DP, int BQ, int WM, int NB, bool REGS>
+__global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) void attn_bwd_dkv_kernel(attn_args p) {
   typedef attn_tile<T, DP> tile_t;
   typedef typename tile_t::frag frag;
   extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
@@ -275,22 +275,31 @@ __global__ __launch_bounds__(64 * WM, 1) void attn_bwd_dkv_kernel(attn_args p) {
   attn_block(p, p.key_tiles, prob, tile, split);
   const int b = prob / p.Hk, hk = prob - b * p.Hk;
 
-  const int key = (tile * WM + wave) * 32 + l32;
+  const int key0 = (tile * WM + wave) * 32 * NB + l32;      // block n of this lane: key0 + 32 n
   const attn_keys keys(p, b);
-  const bool mine = keys.alive(key);
-  const int64_t kr = min(key, p.Tk - 1);
-  const T* kp = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh + kr * p.k_st;
-  const T* vp = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh + kr * p.v_st;
-  frag kf[REGS ? tile_t::NP : 1], vf[REGS ? tile_t::NP : 1];
-  if (REGS) {
-    tile_t::load_row(kf, kp, p.D, h);
-    tile_t::load_row(vf, vp, p.D, h);
-  }
-  f32x16 dk[DP / 32], dv[DP / 32];
+  const T* kb = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh;
+  const T* vb = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh;
+  const T *kp[NB], *vp[NB];
+  frag kf[NB][REGS ? tile_t::NP : 1], vf[NB][REGS ? tile_t::NP : 1];
+  f32x16 dk[NB][DP / 32], dv[NB][DP / 32];
+  bool mine[NB], any = false;
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d) { dk[d] = f32x16_zero(); dv[d] = f32x16_zero(); }
+  for (int n = 0; n < NB; ++n) {
+    const int key = key0 + 32 * n;
+    mine[n] = keys.alive(key);
+    any |= mine[n];
+    const int64_t kr = min(key, p.Tk - 1);
+    kp[n] = kb + kr * p.k_st;
+    vp[n] = vb + kr * p.v_st;
+    if constexpr (REGS) {
+      tile_t::load_row(kf[n], kp[n], p.D, h);
+      tile_t::load_row(vf[n], vp[n], p.D, h);
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) { dk[n][d] = f32x16_zero(); dv[n][d] = f32x16_zero(); }
+  }
 
-  const int nt = __syncthreads_or(mine) ? (p.R + BQ - 1) / BQ : 0;      // no key of this workgroup exists: zeros
+  const int nt = __syncthreads_or(any) ? (p.R + BQ - 1) / BQ : 0;      // no key of this workgroup exists: zeros
   const int t0 = (int)((int64_t)nt * split / p.splits), t1 = (int)((int64_t)nt * (split + 1) / p.splits);
   const attn_rows rows(p, b, hk, prob);
   if (t0 < t1) rows.template issue<T, DP, BQ, WM>(p, attn_smem, TB, t0, wave, lane);
@@ -300,44 +309,53 @@ __global__ __launch_bounds__(64 * WM, 1) void attn_bwd_dkv_kernel(attn_args p) {
     attn_wait_dma();
     __syncthreads();
     if (t + 1 < t1) rows.template issue<T, DP, BQ, WM>(p, attn_smem + ((t + 1 - t0) & 1) * STAGE, TB, t + 1, wave, lane);
-#pragma unroll
+#pragma unroll 1
     for (int qq = 0; qq < BQ / 32; ++qq) {
-      f32x16 s = f32x16_zero(), dp = f32x16_zero();
-      if (REGS) {
-        tile_t::row_product(s, qt, 32 * qq, kf, l32, h);
-        tile_t::row_product(dp, gt, 32 * qq, vf, l32, h);
+      f32x16 s[NB], dp[NB];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) { s[n] = f32x16_zero(); dp[n] = f32x16_zero(); }
+      if constexpr (REGS) {
+        tile_t::template row_product<NB>(s, qt, 32 * qq, kf, l32, h);
+        tile_t::template row_product<NB>(dp, gt, 32 * qq, vf, l32, h);
       } else {
-        tile_t::row_product_mem(s, qt, 32 * qq, kp, p.D, l32, h);
-        tile_t::row_product_mem(dp, gt, 32 * qq, vp, p.D, l32, h);
+        static_assert(REGS || NB == 1, "keys re-read from memory: one block");
+        tile_t::row_product_mem(s[0], qt, 32 * qq, kp[0], p.D, l32, h);
+        tile_t::row_product_mem(dp[0], gt, 32 * qq, vp[0], p.D, l32, h);
       }
       const float* st = (const float*)(qt + 2 * TB) + 32 * qq + 4 * h;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 ls = *(const f32x4*)(st + 8 * g), de = *(const f32x4*)(st + 64 + 8 * g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float pr = fast_exp2(fmaf(s[4 * g + e], p.scale_log2, -ls[e]));
-          s[4 * g + e] = pr;
-          dp[4 * g + e] = pr * (dp[4 * g + e] - de[e]);
-        }
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float pr = fast_exp2(fmaf(s[n][4 * g + e], p.scale_log2, -ls[e]));
+            s[n][4 * g + e] = pr;
+            dp[n][4 * g + e] = pr * (dp[n][4 * g + e] - de[e]);
+          }
       }
-      tile_t::col_product(dv, gt, 32 * qq, s, lane);
-      tile_t::col_product(dk, qt, 32 * qq, dp, lane);
+      tile_t::template col_product<NB>(dv, gt, 32 * qq, s, lane);
+      tile_t::template col_product<NB>(dk, qt, 32 * qq, dp, lane);
     }
   }
-  if (key >= p.Tk) return;
-  const int64_t off = (((int64_t)b * p.Tk + key) * p.Hk + hk) * p.D;
-  if (!mine) {                        // (a select, not a factor: the sums of a key that does not exist may be anything)
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) { dk[d] = f32x16_zero(); dv[d] = f32x16_zero(); }
-  }
-  if (p.splits > 1) {
-    const int64_t plane = (int64_t)p.B * p.Tk * p.Hk * p.D;
-    tile_t::store_row(dk, 1.f, p.part_o + 2 * split * plane + off, (float*)nullptr, p.D, h);
-    tile_t::store_row(dv, 1.f, p.part_o + (2 * split + 1) * plane + off, (float*)nullptr, p.D, h);
-  } else {
-    tile_t::store_row(dk, p.scale, (T*)p.dk + off, (T*)nullptr, p.D, h);
-    tile_t::store_row(dv, 1.f, (T*)p.dv + off, (T*)nullptr, p.D, h);
+  for (int n = 0; n < NB; ++n) {
+    const int key = key0 + 32 * n;
+    if (key >= p.Tk) continue;
+    const int64_t off = (((int64_t)b * p.Tk + key) * p.Hk + hk) * p.D;
+    if (!mine[n]) {                        // (a select, not a factor: the sums of a key that does not exist may be anything)
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d) { dk[n][d] = f32x16_zero(); dv[n][d] = f32x16_zero(); }
+    }
+    if (p.splits > 1) {
+      const int64_t plane = (int64_t)p.B * p.Tk * p.Hk * p.D;
+      tile_t::store_row(dk[n], 1.f, p.part_o + 2 * split * plane + off, (float*)nullptr, p.D, h);
+      tile_t::store_row(dv[n], 1.f, p.part_o + (2 * split + 1) * plane + off, (float*)nullptr, p.D, h);
+    } else {
+      tile_t::store_row(dk[n], p.scale, (T*)p.dk + off, (T*)nullptr, p.D, h);
+      tile_t::store_row(dv[n], 1.f, (T*)p.dv + off, (T*)nullptr, p.D, h);
+    }
   }
 }
 
@@ -412,7 +430,7 @@ static int attn_splits(int64_t blocks, int units, int least) {
 }
 
 struct attn_plan {
-  int dp, wm, bn, row_tiles, fwd_splits, dq_splits, key_tiles, bq, dkv_splits;
+  int dp, wm, bn, row_tiles, fwd_splits, dq_splits, key_tiles, nb, bq, dkv_splits;
   size_t fwd_ws, bwd_ws;
 };
 
@@ -428,7 +446,8 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   const int kt = (a->Tk + q.bn - 1) / q.bn;
   q.fwd_splits = attn_splits(probs * q.row_tiles * q.wm / 4 + 1, kt, 2);
   q.dq_splits = attn_splits(probs * q.row_tiles * q.wm / 4 + 1, kt, 2);
-  q.key_tiles = (a->Tk + 127) / 128;
+  q.nb = 1;
+  q.key_tiles = (a->Tk + 128 * q.nb - 1) / (128 * q.nb);
   q.bq = q.bn;
   const int qt = (int)((R + q.bq - 1) / q.bq);
   q.dkv_splits = attn_splits(probs * q.key_tiles, qt, 2);
@@ -492,7 +511,8 @@ static int attn_bwd_launch(attn_args p, const attn_plan& q, ttdg_stream_t stream
   TTDG_LIMIT(grid < (1ll << 31), "attention_bwd: too many workgroups");
   constexpr bool regs = !(sizeof(T) == 4 && DP == 256);
   constexpr int lds2 = 4 * attn_tile<T, DP>::bytes(BN) + 2048;
-  ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, 4, regs>), grid, 256, lds2, stream, p);
+  constexpr int nb = 1;
+  ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, 4, nb, regs>), grid, 256, lds2, stream, p);
   if (p.splits > 1) {
     for (int w = 0; w < 2; ++w) {
       hipLaunchKernelGGL(attn_reduce_kernel<T>, dim3((unsigned)((nk / 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p.part_o + w * nk, 2 * nk, p.splits,
