@@ -63,12 +63,9 @@ __device__ __forceinline__ void attn_dma4(__amdgpu_buffer_rsrc_t r, char* lds_wa
 __device__ __forceinline__ void attn_store4(float* out, f32x4 x) { *(f32x4*)out = x; }
 __device__ __forceinline__ void attn_store4(__bf16* out, f32x4 x) { *(bf16x4*)out = __builtin_convertvector(x, bf16x4); }
 
-// workgroup -> (problem, tile, split).  Consecutive tiles of one split read the same keys; workgroups are dealt to the eight XCDs in turn,
-// so XCD x takes a contiguous run of that order and its L2 sees each key tile once.
+// workgroup -> (problem, tile, split), tiles of one split next to each other
 __device__ __forceinline__ void attn_block(const attn_args& p, int tiles, int& prob, int& tile, int& split) {
-  const int T = gridDim.x, q = T >> 3, r = T & 7, x = blockIdx.x & 7, i = blockIdx.x >> 3;
-  const int L = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + i;
-  const int per = tiles * p.splits;
+  const int L = blockIdx.x, per = tiles * p.splits;
   prob = L / per;
   const int rem = L - prob * per;
   split = rem / tiles;
