@@ -1,10 +1,13 @@
 // Device building blocks of the attention kernels (attention.hip): operand fragments, LDS tiles, LDS-DMA, row / key bookkeeping.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) float f32x8;
@@ -46,8 +49,6 @@ __device__ __forceinline__ float attn_half_sum(float x) {
 }
 
 __device__ __forceinline__ void attn_wait_dma() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-template <int BN>
-__device__ __forceinline__ constexpr uint64_t attn_all() { return BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1; }
 
 #define ATTN_OOB 0x7ffffff0u          // behind the end of every buffer resource below: reads as zero
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t attn_rsrc(const void* base) {
@@ -72,6 +73,12 @@ __device__ __forceinline__ void attn_block(const attn_args& p, int tiles, int& p
   tile = rem - split * tiles;
 }
 
+// the part [t0, t1) of n tiles that falls to one of the splits
+__device__ __forceinline__ void attn_part(int n, int split, int splits, int& t0, int& t1) {
+  t0 = (int)((int64_t)n * split / splits);
+  t1 = (int)((int64_t)n * (split + 1) / splits);
+}
+
 // row of a problem -> query position and head (rows behind the last one are clamped to it: they are computed and not stored)
 struct attn_row {
   int row, t, head;
@@ -93,10 +100,6 @@ struct attn_keys {
     m_st = p.m_st;
   }
   __device__ __forceinline__ bool alive(int key) const { return key < n && (!mask || mask[key * m_st]); }
-  template <int BN>
-  __device__ __forceinline__ uint64_t live(int t, int lane) const {      // bit j: key t BN + j exists
-    return __ballot(lane < BN && alive(t * BN + lane));
-  }
 };
 
 // position of 16-byte chunk c of a tile row.  Eight consecutive rows XOR with eight different numbers (row reads: eight lanes of
@@ -138,19 +141,6 @@ struct attn_tile {
     return s;
   }
 
-  // tile rows [0, ROWS) from base (row stride st elements) into LDS; rows whose bit in `live` is off, and chunks behind D, become zeros
-  template <int ROWS, int WM>
-  static __device__ __forceinline__ void issue(char* lds, const T* base, int64_t st, int D, uint64_t live, int wave, int lane) {
-    const auto r = attn_rsrc(base);
-    const uint32_t stb = (uint32_t)(st * ES);
-#pragma unroll
-    for (int i = 0; i < ROWS * NC / 64 / WM; ++i) {
-      const int lin = (i * WM + wave) * 64 + lane, row = lin / NC, c = (lin % NC) ^ attn_swz(row);
-      const uint32_t off = ((live >> row) & 1) && c * CE < D ? row * stb + c * 16 : ATTN_OOB;
-      attn_dma16(r, lds + (i * WM + wave) * 1024, off);
-    }
-  }
-
   static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
     if constexpr (F32) {
 #pragma unroll
@@ -161,16 +151,15 @@ struct attn_tile {
     }
   }
 
-  // acc[n][tile row][lane's row of f[n]] += sum_d tile[row0 + .][d] f[n][d]: every chunk read from LDS serves the NB blocks of columns
-  template <int NB>
-  static __device__ __forceinline__ void row_product(f32x16* acc, const char* tile, int row0, const frag (*f)[NP], int l32, int h) {
+  // acc[n][tile row][lane's row of f] += sum_d tile[row0 + 32 n + .][d] f[d] for KK blocks of tile rows: KK independent chains of products
+  template <int KK>
+  static __device__ __forceinline__ void row_product(f32x16* acc, const char* tile, int row0, const frag* f, int l32, int h) {
     const int base = l32 * RB + ((h ^ attn_swz(l32)) << 4);
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const frag a = *(const frag*)(tile + row0 * RB + (base ^ (32 * (i & 3))) + 128 * (i >> 2));
+    for (int i = 0; i < NP; ++i)
 #pragma unroll
-      for (int n = 0; n < NB; ++n) acc[n] = mma(a, f[n][i], acc[n]);
-    }
+      for (int n = 0; n < KK; ++n)
+        acc[n] = mma(*(const frag*)(tile + (row0 + 32 * n) * RB + (base ^ (32 * (i & 3))) + 128 * (i >> 2)), f[i], acc[n]);
   }
   // the same with the second operand read from memory
   static __device__ __forceinline__ void row_product_mem(f32x16& acc, const char* tile, int row0, const T* row, int D, int l32, int h) {
@@ -184,11 +173,48 @@ struct attn_tile {
     }
   }
 
-  // acc[n][d][lane's column] += sum over the 32 tile rows from row0 of tile[.][d] p[n][.], p in accumulator layout.  For 16-bit types p is
-  // rounded to the inputs' type (round to nearest even, as every operand of the matrix unit is): an error of at most half a step per
-  // term, independent from term to term, while the sums stay in 32 bits.
+  // 32 tile rows of one column block as the second product's second operand.  For 16-bit types they are rounded to the inputs' type (round
+  // to nearest even, as every operand of the matrix unit is): an error of at most half a step per term, independent from term to term,
+  // while the sums stay in 32 bits.
+  struct operand {
+    typename std::conditional<F32, f32x16, bf16x8>::type x[F32 ? 1 : 2];
+  };
+  static __device__ __forceinline__ operand pack(const f32x16& p) {
+    operand r;
+    if constexpr (F32) {
+      r.x[0] = p;
+    } else {
+#pragma unroll
+      for (int kg = 0; kg < 2; ++kg) {
+        f32x8 y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = p[8 * kg + e];
+        r.x[kg] = __builtin_convertvector(y, bf16x8);
+      }
+    }
+    return r;
+  }
+  // l + the lane's terms as the product will see them: a row's weights then sum to one whatever their rounding did
+  static __device__ __forceinline__ float sum(const operand& p, float l) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) l += p.x[0][e];
+    } else {
+      const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+      for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const bf16x2 y = {p.x[kg][e], p.x[kg][e + 1]};
+          l = __builtin_amdgcn_fdot2_f32_bf16(y, one, l, false);
+        }
+    }
+    return l;
+  }
+
+  // acc[n][d][lane's column] += sum over the 32 tile rows from row0 of tile[.][d] p[n][.]
   template <int NB>
-  static __device__ __forceinline__ void col_product(f32x16 (*acc)[DP / 32], const char* tile, int row0, const f32x16* p, int lane) {
+  static __device__ __forceinline__ void col_product(f32x16 (*acc)[DP / 32], const char* tile, int row0, const operand* p, int lane) {
     const int h = lane >> 5;
     if constexpr (F32) {
       const int l32 = lane & 31;
@@ -200,22 +226,14 @@ struct attn_tile {
         for (int d = 0; d < DP / 32; ++d) {
           const float x = *(const float*)(a + 128 * d);
 #pragma unroll
-          for (int n = 0; n < NB; ++n) acc[n][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[n][e], acc[n][d], 0, 0, 0);
+          for (int n = 0; n < NB; ++n) acc[n][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[n].x[0][e], acc[n][d], 0, 0, 0);
         }
       }
     } else {
       const int i = lane & 15, blk = (lane >> 4) & 1, row = 4 * h + (i >> 2);
       const int base = row * RB + (((2 * blk + ((i & 3) >> 1)) ^ attn_swz(row)) << 4) + 8 * (i & 1);
 #pragma unroll
-      for (int kg = 0; kg < 2; ++kg) {
-        bf16x8 b[NB];
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          f32x8 x;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = p[n][8 * kg + e];
-          b[n] = __builtin_convertvector(x, bf16x8);
-        }
+      for (int kg = 0; kg < 2; ++kg)
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
           const char* a = tile + (row0 + 16 * kg) * RB + (base ^ (64 * (d & 1))) + 128 * (d >> 1);
@@ -223,9 +241,8 @@ struct attn_tile {
           const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(a + 8 * RB));
           const bf16x8 f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-          for (int n = 0; n < NB; ++n) acc[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, b[n], acc[n][d], 0, 0, 0);
+          for (int n = 0; n < NB; ++n) acc[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, p[n].x[kg], acc[n][d], 0, 0, 0);
         }
-      }
     }
   }
 
@@ -253,39 +270,144 @@ struct attn_tile {
   }
 };
 
-// row tiles of the dk / dv kernel: q, do, lse and delta of BQ rows of a problem
+// LDS-DMA of ROWS tile rows: instruction i of a wavefront fills 1 KiB; its lanes' offsets repeat every PER instructions (the swizzle has a
+// period of eight rows), the rest of the distance goes into the scalar offset.  Lanes behind D always point behind the resource's end.
+template <typename T, int DP, int ROWS, int WM>
+struct attn_loader {
+  typedef attn_tile<T, DP> tile_t;
+  static constexpr int N = ROWS * tile_t::NC / 64 / WM;              // instructions per wavefront
+  static constexpr int STEP = WM * 64 / tile_t::NC;                  // tile rows from one instruction to the next
+  static constexpr int PER = STEP >= 8 ? 1 : 8 / STEP;
+  uint32_t off[PER];
+  int row, cofs[PER];
+  __device__ __forceinline__ void init(int D, int wave, int lane) {
+    row = (wave * 64 + lane) / tile_t::NC;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int c = (lane % tile_t::NC) ^ attn_swz(row + j * STEP);
+      cofs[j] = c * tile_t::CE < D ? c * 16 : -1;
+    }
+  }
+  // rows stb bytes apart
+  __device__ __forceinline__ void strided(uint32_t stb) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) off[j] = cofs[j] < 0 ? ATTN_OOB : (row + j * STEP) * stb + cofs[j];
+  }
+  // rows whose bit in `live` is off become zeros
+  __device__ __forceinline__ void issue(char* lds, const void* base, uint32_t stb, uint64_t live, bool all, int wave) const {
+    const auto r = attn_rsrc(base);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      uint32_t o = off[i % PER];
+      if (!all) o = (live >> (row + i * STEP)) & 1 ? o : ATTN_OOB;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + (i * WM + wave) * 1024), 16, o,
+                                               (i / PER) * PER * STEP * stb, 0, 0);
+    }
+  }
+};
+
+// The key / value tiles of a problem, in stages of LDS: k tile, v tile, and for tiles with absent keys the scores' starting values (0, or
+// -infinity where no key exists: the scores' sums start from them, so masking costs no vector instruction).
+template <typename T, int DP, int BN, int WM>
+struct attn_stream {
+  typedef attn_tile<T, DP> tile_t;
+  static constexpr int TB = tile_t::bytes(BN), STAGE = 2 * TB + 256;
+  static constexpr uint64_t ALL = BN == 64 ? ~0ull : (1ull << (BN & 63)) - 1;
+  attn_loader<T, DP, BN, WM> lk, lv;
+  attn_keys keys;
+  const T *k, *v;
+  int64_t k_tile, v_tile;
+  uint32_t k_stb, v_stb;
+  int next, wave, lane;
+  bool ahead;                        // does this lane's key of the next tile exist (its mask byte was asked for a tile earlier)
+
+  __device__ __forceinline__ attn_stream(const attn_args& p, int b, int hk, int wave_, int lane_) : keys(p, b), next(0), wave(wave_), lane(lane_) {
+    k = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh;
+    v = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh;
+    k_tile = BN * p.k_st;
+    v_tile = BN * p.v_st;
+    k_stb = (uint32_t)(p.k_st * tile_t::ES);
+    v_stb = (uint32_t)(p.v_st * tile_t::ES);
+    lk.init(p.D, wave, lane);
+    lv = lk;
+    lk.strided(k_stb);
+    lv.strided(v_stb);
+  }
+  __device__ __forceinline__ int tiles() const { return (keys.n + BN - 1) / BN; }
+  __device__ __forceinline__ void seek(int t) {
+    next = t;
+    k += t * k_tile;
+    v += t * v_tile;
+  }
+  __device__ __forceinline__ void peek() { ahead = lane < BN && keys.alive(next * BN + lane); }
+  // starts the next tile's way into `stage` and returns which of its keys exist (none: nothing is loaded)
+  __device__ __forceinline__ uint64_t issue(char* stage) {
+    const uint64_t live = __ballot(ahead);
+    if (live) {
+      const bool all = live == ALL;
+      lk.issue(stage, k, k_stb, live, all, wave);
+      lv.issue(stage + TB, v, v_stb, live, all, wave);
+      if (!all && wave == 0) ((float*)(stage + 2 * TB))[lane] = ahead ? 0.f : -INFINITY;
+    }
+    k += k_tile;
+    v += v_tile;
+    ++next;
+    return live;
+  }
+  // starting values of the scores
+  static __device__ __forceinline__ void start(f32x16* s, const char* stage, uint64_t live, int h) {
+    if (live == ALL) {
+#pragma unroll
+      for (int n = 0; n < BN / 32; ++n) s[n] = f32x16_zero();
+    } else {
+#pragma unroll
+      for (int n = 0; n < BN / 32; ++n)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 x = *(const f32x4*)(stage + 2 * TB + 4 * (32 * n + 8 * g + 4 * h));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][4 * g + e] = x[e];
+        }
+    }
+  }
+};
+
+// The row tiles of the dk / dv kernel, in stages of LDS: q tile, do tile, lse and delta of the rows
+template <typename T, int DP, int BQ, int WM>
 struct attn_rows {
-  const char *q, *g;
+  typedef attn_tile<T, DP> tile_t;
+  static constexpr int TB = tile_t::bytes(BQ), STAGE = 2 * TB + 512;
+  attn_loader<T, DP, BQ, WM> lq, lg;
+  const T *q, *g;
   const float *lse, *delta;
-  __device__ __forceinline__ attn_rows(const attn_args& p, int b, int hk, int prob) {
-    q = (const char*)p.q;
-    g = (const char*)p.dout;
+  int next, wave, lane;
+  __device__ __forceinline__ attn_rows(const attn_args& p, int b, int hk, int prob, int first, int wave_, int lane_) : next(first), wave(wave_), lane(lane_) {
     lse = p.lse + (int64_t)prob * p.R;
     delta = p.delta + (int64_t)prob * p.R;
-    q_off = b * p.q_sb + (int64_t)hk * p.G * p.q_sh;
-    g_off = ((int64_t)b * p.Tq * p.H + (int64_t)hk * p.G) * p.D;
+    q = (const T*)p.q + b * p.q_sb + (int64_t)hk * p.G * p.q_sh;
+    g = (const T*)p.dout + ((int64_t)b * p.Tq * p.H + (int64_t)hk * p.G) * p.D;
+    lq.init(p.D, wave, lane);
+    lg = lq;
   }
-  int64_t q_off, g_off;
-  template <typename T, int DP, int BQ, int WM>
-  __device__ __forceinline__ void issue(const attn_args& p, char* lds, int tile_bytes, int t, int wave, int lane) const {
-    typedef attn_tile<T, DP> tile_t;
-    const int r0 = t * BQ, tb = r0 / p.G, left = p.R - r0;
-    const auto rq = attn_rsrc((const T*)q + q_off + (int64_t)tb * p.q_st);
-    const auto rg = attn_rsrc((const T*)g + g_off + (int64_t)tb * p.H * p.D);
+  __device__ __forceinline__ void issue(const attn_args& p, char* stage) {
+    const int r0 = next * BQ, tb = r0 / p.G, left = p.R - r0;
+    const auto rq = attn_rsrc(q + (int64_t)tb * p.q_st);
+    const auto rg = attn_rsrc(g + (int64_t)tb * p.H * p.D);
     const uint32_t qst = (uint32_t)(p.q_st * tile_t::ES), qsh = (uint32_t)(p.q_sh * tile_t::ES);
     const uint32_t gst = (uint32_t)(p.H * p.D * tile_t::ES), gsh = (uint32_t)(p.D * tile_t::ES);
 #pragma unroll
-    for (int i = 0; i < BQ * tile_t::NC / 64 / WM; ++i) {
-      const int lin = (i * WM + wave) * 64 + lane, row = lin / tile_t::NC, c = (lin % tile_t::NC) ^ attn_swz(row);
-      const int r = r0 + row, tt = r / p.G, gg = r - tt * p.G;
-      const bool ok = row < left && c * tile_t::CE < p.D;
-      attn_dma16(rq, lds + (i * WM + wave) * 1024, ok ? (tt - tb) * qst + gg * qsh + c * 16 : ATTN_OOB);
-      attn_dma16(rg, lds + tile_bytes + (i * WM + wave) * 1024, ok ? (tt - tb) * gst + gg * gsh + c * 16 : ATTN_OOB);
+    for (int i = 0; i < decltype(lq)::N; ++i) {
+      const int row = lq.row + i * decltype(lq)::STEP, c = lq.cofs[i % decltype(lq)::PER];
+      const bool ok = c >= 0 && row < left;
+      const int r = r0 + row - tb * p.G, tt = p.G == 1 ? r : r / p.G, gg = r - tt * p.G;
+      attn_dma16(rq, stage + (i * WM + wave) * 1024, ok ? tt * qst + gg * qsh + c : ATTN_OOB);
+      attn_dma16(rg, stage + TB + (i * WM + wave) * 1024, ok ? tt * gst + gg * gsh + c : ATTN_OOB);
     }
     if (wave == WM - 1) {
       const uint32_t off = lane < BQ && lane < left ? lane * 4 : ATTN_OOB;
-      attn_dma4(attn_rsrc(lse + r0), lds + 2 * tile_bytes, off);
-      attn_dma4(attn_rsrc(delta + r0), lds + 2 * tile_bytes + 256, off);
+      attn_dma4(attn_rsrc(lse + r0), stage + 2 * TB, off);
+      attn_dma4(attn_rsrc(delta + r0), stage + 2 * TB + 256, off);
     }
+    ++next;
   }
 };

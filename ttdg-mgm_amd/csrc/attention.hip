@@ -26,8 +26,8 @@ template <typename T, int DP, int BN, int WM>
 __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) void attn_fwd_kernel(attn_args p) {
   typedef attn_tile<T, DP> tile_t;
   typedef typename tile_t::frag frag;
+  typedef attn_stream<T, DP, BN, WM> stream_t;
   extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
-  constexpr int TB = tile_t::bytes(BN);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = lane >> 5, l32 = lane & 31;
   int prob, tile, split;
@@ -44,55 +44,39 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
   for (int d = 0; d < DP / 32; ++d) o[d] = f32x16_zero();
   float m = -INFINITY, l = 0.f;
 
-  const attn_keys keys(p, b);
-  const int nt = (keys.n + BN - 1) / BN;
-  const int t0 = (int)((int64_t)nt * split / p.splits), t1 = (int)((int64_t)nt * (split + 1) / p.splits);
-  const T* kb = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh;
-  const T* vb = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh;
-  uint64_t live_next = t0 < t1 ? keys.live<BN>(t0, lane) : 0;
-  if (live_next) {
-    tile_t::template issue<BN, WM>(attn_smem, kb + (int64_t)t0 * BN * p.k_st, p.k_st, p.D, live_next, wave, lane);
-    tile_t::template issue<BN, WM>(attn_smem + TB, vb + (int64_t)t0 * BN * p.v_st, p.v_st, p.D, live_next, wave, lane);
+  stream_t in(p, b, hk, wave, lane);
+  int t0, t1;
+  attn_part(in.tiles(), split, p.splits, t0, t1);
+  in.seek(t0);
+  uint64_t live_next = 0;
+  if (t0 < t1) {
+    in.peek();
+    live_next = in.issue(attn_smem);
+    in.peek();
   }
   for (int t = t0; t < t1; ++t) {
-    const char* kt = attn_smem + ((t - t0) & 1) * 2 * TB;
-    const char* vt = kt + TB;
+    char* stage = attn_smem + ((t - t0) & 1) * stream_t::STAGE;
     const uint64_t live = live_next;
     attn_wait_dma();                 // this wavefront's share of tile t has landed
-    __syncthreads();                 // ... everybody's has, and nobody still reads the other buffer
+    __syncthreads();                 // ... everybody's has, and nobody still reads the other stage
     if (t + 1 < t1) {
-      live_next = keys.live<BN>(t + 1, lane);
-      if (live_next) {
-        char* nx = attn_smem + ((t + 1 - t0) & 1) * 2 * TB;
-        tile_t::template issue<BN, WM>(nx, kb + (int64_t)(t + 1) * BN * p.k_st, p.k_st, p.D, live_next, wave, lane);
-        tile_t::template issue<BN, WM>(nx + TB, vb + (int64_t)(t + 1) * BN * p.v_st, p.v_st, p.D, live_next, wave, lane);
-      }
+      live_next = in.issue(attn_smem + ((t + 1 - t0) & 1) * stream_t::STAGE);
+      in.peek();
     }
     if (live == 0) continue;         // (the same for every wavefront of the workgroup)
     f32x16 s[BN / 32];
-#pragma unroll
-    for (int kk = 0; kk < BN / 32; ++kk) {
-      s[kk] = f32x16_zero();
-      tile_t::template row_product<1>(&s[kk], kt, 32 * kk, &qf, l32, h);
-    }
-    if (live != attn_all<BN>()) {
-#pragma unroll
-      for (int kk = 0; kk < BN / 32; ++kk) {
-        const uint32_t bits = (uint32_t)(live >> (32 * kk)) >> (4 * h);
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (!((bits >> attn_reg_row(e)) & 1)) s[kk][e] = -INFINITY;
-      }
-    }
+    stream_t::start(s, stage, live, h);
+    tile_t::template row_product<BN / 32>(s, stage, 0, qf, l32, h);
     float mx = s[0][0];
 #pragma unroll
     for (int kk = 0; kk < BN / 32; ++kk)
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kk][e]);
-    mx = attn_half_max(mx);
-    const float mn = fmaxf(m, mx * p.scale_log2);
-    if (__any(mn > m)) {             // the running maximum grew somewhere: rescale what has been summed
-      const float a = fast_exp2(m - mn);
+    mx = attn_half_max(mx) * p.scale_log2;
+    // The reference point m follows the running maximum only when that has grown by more than 2^8: terms up to 2^8 round no worse than
+    // terms up to 1 and their sums are far from any limit, and with m at every new maximum most tiles would rescale the sums.
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx), a = fast_exp2(m - mn);
       l *= a;
 #pragma unroll
       for (int d = 0; d < DP / 32; ++d) o[d] *= a;
@@ -101,12 +85,10 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
 #pragma unroll
     for (int kk = 0; kk < BN / 32; ++kk) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float x = fast_exp2(fmaf(s[kk][e], p.scale_log2, -m));
-        s[kk][e] = x;
-        l += x;
-      }
-      tile_t::template col_product<1>(&o, vt, 32 * kk, &s[kk], lane);
+      for (int e = 0; e < 16; ++e) s[kk][e] = fast_exp2(fmaf(s[kk][e], p.scale_log2, -m));
+      const typename tile_t::operand pr = tile_t::pack(s[kk]);
+      l = tile_t::sum(pr, l);
+      tile_t::template col_product<1>(&o, stage + stream_t::TB, 32 * kk, &pr, lane);
     }
   }
   l = attn_half_sum(l);
@@ -191,8 +173,8 @@ template <typename T, int DP, int BN, int WM>
 __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) void attn_bwd_dq_kernel(attn_args p) {
   typedef attn_tile<T, DP> tile_t;
   typedef typename tile_t::frag frag;
+  typedef attn_stream<T, DP, BN, WM> stream_t;
   extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
-  constexpr int TB = tile_t::bytes(BN);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = lane >> 5, l32 = lane & 31;
   int prob, tile, split;
@@ -215,43 +197,38 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) acc[d] = f32x16_zero();
 
-  const attn_keys keys(p, b);
-  const int nt = (keys.n + BN - 1) / BN;
-  const int t0 = (int)((int64_t)nt * split / p.splits), t1 = (int)((int64_t)nt * (split + 1) / p.splits);
-  const T* kb = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh;
-  const T* vb = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh;
-  uint64_t live_next = t0 < t1 ? keys.live<BN>(t0, lane) : 0;
-  if (live_next) {
-    tile_t::template issue<BN, WM>(attn_smem, kb + (int64_t)t0 * BN * p.k_st, p.k_st, p.D, live_next, wave, lane);
-    tile_t::template issue<BN, WM>(attn_smem + TB, vb + (int64_t)t0 * BN * p.v_st, p.v_st, p.D, live_next, wave, lane);
+  stream_t in(p, b, hk, wave, lane);
+  int t0, t1;
+  attn_part(in.tiles(), split, p.splits, t0, t1);
+  in.seek(t0);
+  uint64_t live_next = 0;
+  if (t0 < t1) {
+    in.peek();
+    live_next = in.issue(attn_smem);
+    in.peek();
   }
   for (int t = t0; t < t1; ++t) {
-    const char* kt = attn_smem + ((t - t0) & 1) * 2 * TB;
-    const char* vt = kt + TB;
+    char* stage = attn_smem + ((t - t0) & 1) * stream_t::STAGE;
     const uint64_t live = live_next;
     attn_wait_dma();
     __syncthreads();
     if (t + 1 < t1) {
-      live_next = keys.live<BN>(t + 1, lane);
-      if (live_next) {
-        char* nx = attn_smem + ((t + 1 - t0) & 1) * 2 * TB;
-        tile_t::template issue<BN, WM>(nx, kb + (int64_t)(t + 1) * BN * p.k_st, p.k_st, p.D, live_next, wave, lane);
-        tile_t::template issue<BN, WM>(nx + TB, vb + (int64_t)(t + 1) * BN * p.v_st, p.v_st, p.D, live_next, wave, lane);
-      }
+      live_next = in.issue(attn_smem + ((t + 1 - t0) & 1) * stream_t::STAGE);
+      in.peek();
     }
     if (live == 0) continue;
+    f32x16 s[BN / 32], dp[BN / 32];
+    stream_t::start(s, stage, live, h);
+    tile_t::template row_product<BN / 32>(s, stage, 0, qf, l32, h);
+#pragma unroll
+    for (int kk = 0; kk < BN / 32; ++kk) dp[kk] = f32x16_zero();
+    tile_t::template row_product<BN / 32>(dp, stage + stream_t::TB, 0, gf, l32, h);
 #pragma unroll
     for (int kk = 0; kk < BN / 32; ++kk) {
-      f32x16 s = f32x16_zero(), dp = f32x16_zero();
-      tile_t::template row_product<1>(&s, kt, 32 * kk, &qf, l32, h);
-      tile_t::template row_product<1>(&dp, vt, 32 * kk, &gf, l32, h);
-      const uint32_t bits = (uint32_t)(live >> (32 * kk)) >> (4 * h);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float pr = fast_exp2(fmaf(s[e], p.scale_log2, -lse));
-        s[e] = ((bits >> attn_reg_row(e)) & 1) ? pr * (dp[e] - delta) : 0.f;
-      }
-      tile_t::template col_product<1>(&acc, kt, 32 * kk, &s, lane);
+      for (int e = 0; e < 16; ++e) s[kk][e] = fast_exp2(fmaf(s[kk][e], p.scale_log2, -lse)) * (dp[kk][e] - delta);
+      const typename tile_t::operand ds = tile_t::pack(s[kk]);
+      tile_t::template col_product<1>(&acc, stage, 32 * kk, &ds, lane);
     }
   }
   if (row >= p.R) return;
@@ -259,103 +236,85 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
   else tile_t::store_row(acc, p.scale, (T*)p.dq + off, (T*)nullptr, p.D, h);
 }
 
-// dk and dv: a wavefront owns 32 NB keys, their k and v rows in registers (REGS) or re-read through the caches (the registers of float32
+// dk and dv: a wavefront owns 32 keys, their k and v rows in registers (REGS) or re-read through the caches (the registers of float32
 // with 256 channels are full of the two sums), and walks over the rows; q and do tiles in LDS serve both as rows (scores) and, transposed,
 // as the second products' first operand.
-template <typename T, int DP, int BQ, int WM, int NB, bool REGS>
+template <typename T, int DP, int BQ, int WM, bool REGS>
 __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) void attn_bwd_dkv_kernel(attn_args p) {
   typedef attn_tile<T, DP> tile_t;
   typedef typename tile_t::frag frag;
+  typedef attn_rows<T, DP, BQ, WM> rows_t;
   extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
-  constexpr int TB = tile_t::bytes(BQ);
-  constexpr int STAGE = 2 * TB + 1024;        // q tile, do tile, lse (64 floats), delta (64 floats), padding
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = lane >> 5, l32 = lane & 31;
   int prob, tile, split;
   attn_block(p, p.key_tiles, prob, tile, split);
   const int b = prob / p.Hk, hk = prob - b * p.Hk;
 
-  const int key0 = (tile * WM + wave) * 32 * NB + l32;      // block n of this lane: key0 + 32 n
+  const int key = (tile * WM + wave) * 32 + l32;
   const attn_keys keys(p, b);
-  const T* kb = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh;
-  const T* vb = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh;
-  const T *kp[NB], *vp[NB];
-  frag kf[NB][REGS ? tile_t::NP : 1], vf[NB][REGS ? tile_t::NP : 1];
-  f32x16 dk[NB][DP / 32], dv[NB][DP / 32];
-  bool mine[NB], any = false;
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const int key = key0 + 32 * n;
-    mine[n] = keys.alive(key);
-    any |= mine[n];
-    const int64_t kr = min(key, p.Tk - 1);
-    kp[n] = kb + kr * p.k_st;
-    vp[n] = vb + kr * p.v_st;
-    if constexpr (REGS) {
-      tile_t::load_row(kf[n], kp[n], p.D, h);
-      tile_t::load_row(vf[n], vp[n], p.D, h);
-    }
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d) { dk[n][d] = f32x16_zero(); dv[n][d] = f32x16_zero(); }
+  const bool mine = keys.alive(key);
+  const int64_t kr = min(key, p.Tk - 1);
+  const T* kp = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh + kr * p.k_st;
+  const T* vp = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh + kr * p.v_st;
+  frag kf[REGS ? tile_t::NP : 1], vf[REGS ? tile_t::NP : 1];
+  if constexpr (REGS) {
+    tile_t::load_row(kf, kp, p.D, h);
+    tile_t::load_row(vf, vp, p.D, h);
   }
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) { dk[d] = f32x16_zero(); dv[d] = f32x16_zero(); }
 
-  const int nt = __syncthreads_or(any) ? (p.R + BQ - 1) / BQ : 0;      // no key of this workgroup exists: zeros
-  const int t0 = (int)((int64_t)nt * split / p.splits), t1 = (int)((int64_t)nt * (split + 1) / p.splits);
-  const attn_rows rows(p, b, hk, prob);
-  if (t0 < t1) rows.template issue<T, DP, BQ, WM>(p, attn_smem, TB, t0, wave, lane);
+  int t0, t1;
+  attn_part(__syncthreads_or(mine) ? (p.R + BQ - 1) / BQ : 0, split, p.splits, t0, t1);      // no key of this workgroup exists: zeros
+  rows_t in(p, b, hk, prob, t0, wave, lane);
+  if (t0 < t1) in.issue(p, attn_smem);
   for (int t = t0; t < t1; ++t) {
-    const char* qt = attn_smem + ((t - t0) & 1) * STAGE;
-    const char* gt = qt + TB;
+    const char* qt = attn_smem + ((t - t0) & 1) * rows_t::STAGE;
+    const char* gt = qt + rows_t::TB;
     attn_wait_dma();
     __syncthreads();
-    if (t + 1 < t1) rows.template issue<T, DP, BQ, WM>(p, attn_smem + ((t + 1 - t0) & 1) * STAGE, TB, t + 1, wave, lane);
+    if (t + 1 < t1) in.issue(p, attn_smem + ((t + 1 - t0) & 1) * rows_t::STAGE);
 #pragma unroll 1
     for (int qq = 0; qq < BQ / 32; ++qq) {
-      f32x16 s[NB], dp[NB];
-#pragma unroll
-      for (int n = 0; n < NB; ++n) { s[n] = f32x16_zero(); dp[n] = f32x16_zero(); }
+      f32x16 s = f32x16_zero(), dp = f32x16_zero();
       if constexpr (REGS) {
-        tile_t::template row_product<NB>(s, qt, 32 * qq, kf, l32, h);
-        tile_t::template row_product<NB>(dp, gt, 32 * qq, vf, l32, h);
+        tile_t::template row_product<1>(&s, qt, 32 * qq, kf, l32, h);
+        tile_t::template row_product<1>(&dp, gt, 32 * qq, vf, l32, h);
       } else {
-        static_assert(REGS || NB == 1, "keys re-read from memory: one block");
-        tile_t::row_product_mem(s[0], qt, 32 * qq, kp[0], p.D, l32, h);
-        tile_t::row_product_mem(dp[0], gt, 32 * qq, vp[0], p.D, l32, h);
+        tile_t::row_product_mem(s, qt, 32 * qq, kp, p.D, l32, h);
+        tile_t::row_product_mem(dp, gt, 32 * qq, vp, p.D, l32, h);
       }
-      const float* st = (const float*)(qt + 2 * TB) + 32 * qq + 4 * h;
+      const float* st = (const float*)(qt + 2 * rows_t::TB) + 32 * qq + 4 * h;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 ls = *(const f32x4*)(st + 8 * g), de = *(const f32x4*)(st + 64 + 8 * g);
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float pr = fast_exp2(fmaf(s[n][4 * g + e], p.scale_log2, -ls[e]));
-            s[n][4 * g + e] = pr;
-            dp[n][4 * g + e] = pr * (dp[n][4 * g + e] - de[e]);
-          }
+        for (int e = 0; e < 4; ++e) {
+          const float pr = fast_exp2(fmaf(s[4 * g + e], p.scale_log2, -ls[e]));
+          s[4 * g + e] = pr;
+          dp[4 * g + e] = pr * (dp[4 * g + e] - de[e]);
+        }
       }
-      tile_t::template col_product<NB>(dv, gt, 32 * qq, s, lane);
-      tile_t::template col_product<NB>(dk, qt, 32 * qq, dp, lane);
+      const typename tile_t::operand pr = tile_t::pack(s), ds = tile_t::pack(dp);
+      tile_t::template col_product<1>(&dv, gt, 32 * qq, &pr, lane);
+      tile_t::template col_product<1>(&dk, qt, 32 * qq, &ds, lane);
     }
   }
+  if (key >= p.Tk) return;
+  const int64_t off = (((int64_t)b * p.Tk + key) * p.Hk + hk) * p.D;
+  if (!mine) {                        // (a select, not a factor: the sums of a key that does not exist may be anything)
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const int key = key0 + 32 * n;
-    if (key >= p.Tk) continue;
-    const int64_t off = (((int64_t)b * p.Tk + key) * p.Hk + hk) * p.D;
-    if (!mine[n]) {                        // (a select, not a factor: the sums of a key that does not exist may be anything)
-#pragma unroll
-      for (int d = 0; d < DP / 32; ++d) { dk[n][d] = f32x16_zero(); dv[n][d] = f32x16_zero(); }
-    }
-    if (p.splits > 1) {
-      const int64_t plane = (int64_t)p.B * p.Tk * p.Hk * p.D;
-      tile_t::store_row(dk[n], 1.f, p.part_o + 2 * split * plane + off, (float*)nullptr, p.D, h);
-      tile_t::store_row(dv[n], 1.f, p.part_o + (2 * split + 1) * plane + off, (float*)nullptr, p.D, h);
-    } else {
-      tile_t::store_row(dk[n], p.scale, (T*)p.dk + off, (T*)nullptr, p.D, h);
-      tile_t::store_row(dv[n], 1.f, (T*)p.dv + off, (T*)nullptr, p.D, h);
-    }
+    for (int d = 0; d < DP / 32; ++d) { dk[d] = f32x16_zero(); dv[d] = f32x16_zero(); }
+  }
+  if (p.splits > 1) {
+    const int64_t plane = (int64_t)p.B * p.Tk * p.Hk * p.D;
+    tile_t::store_row(dk, 1.f, p.part_o + 2 * split * plane + off, (float*)nullptr, p.D, h);
+    tile_t::store_row(dv, 1.f, p.part_o + (2 * split + 1) * plane + off, (float*)nullptr, p.D, h);
+  } else {
+    tile_t::store_row(dk, p.scale, (T*)p.dk + off, (T*)nullptr, p.D, h);
+    tile_t::store_row(dv, 1.f, (T*)p.dv + off, (T*)nullptr, p.D, h);
   }
 }
 
@@ -430,7 +389,7 @@ static int attn_splits(int64_t blocks, int units, int least) {
 }
 
 struct attn_plan {
-  int dp, wm, bn, row_tiles, fwd_splits, dq_splits, key_tiles, nb, bq, dkv_splits;
+  int dp, wm, bn, row_tiles, fwd_splits, dq_splits, key_tiles, bq, dkv_splits;
   size_t fwd_ws, bwd_ws;
 };
 
@@ -446,8 +405,7 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   const int kt = (a->Tk + q.bn - 1) / q.bn;
   q.fwd_splits = attn_splits(probs * q.row_tiles * q.wm / 4 + 1, kt, 2);
   q.dq_splits = attn_splits(probs * q.row_tiles * q.wm / 4 + 1, kt, 2);
-  q.nb = 1;
-  q.key_tiles = (a->Tk + 128 * q.nb - 1) / (128 * q.nb);
+  q.key_tiles = (a->Tk + 127) / 128;
   q.bq = q.bn;
   const int qt = (int)((R + q.bq - 1) / q.bq);
   q.dkv_splits = attn_splits(probs * q.key_tiles, qt, 2);
@@ -479,7 +437,7 @@ extern "C" size_t ttdg_attention_bwd_workspace_bytes(const ttdg_attention_t* a) 
 
 template <typename T, int DP, int BN>
 static int attn_fwd_launch(const attn_args& p, const attn_plan& q, ttdg_stream_t stream) {
-  constexpr int lds = 4 * attn_tile<T, DP>::bytes(BN);
+  constexpr int lds = 2 * attn_stream<T, DP, BN, 4>::STAGE;
   const int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;
   TTDG_LIMIT(grid < (1ll << 31), "attention_fwd: too many workgroups");
   if (q.wm == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 1>), grid, 64, lds, stream, p);
@@ -494,7 +452,7 @@ static int attn_fwd_launch(const attn_args& p, const attn_plan& q, ttdg_stream_t
 
 template <typename T, int DP, int BN>
 static int attn_bwd_launch(attn_args p, const attn_plan& q, ttdg_stream_t stream) {
-  constexpr int lds = 4 * attn_tile<T, DP>::bytes(BN);
+  constexpr int lds = 2 * attn_stream<T, DP, BN, 4>::STAGE;
   p.splits = q.dq_splits;
   int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;
   TTDG_LIMIT(grid < (1ll << 31), "attention_bwd: too many workgroups");
@@ -510,9 +468,8 @@ static int attn_bwd_launch(attn_args p, const attn_plan& q, ttdg_stream_t stream
   grid = (int64_t)p.B * p.Hk * p.key_tiles * p.splits;
   TTDG_LIMIT(grid < (1ll << 31), "attention_bwd: too many workgroups");
   constexpr bool regs = !(sizeof(T) == 4 && DP == 256);
-  constexpr int lds2 = 4 * attn_tile<T, DP>::bytes(BN) + 2048;
-  constexpr int nb = 1;
-  ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, 4, nb, regs>), grid, 256, lds2, stream, p);
+  constexpr int lds2 = 2 * attn_rows<T, DP, BN, 4>::STAGE;
+  ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, 4, regs>), grid, 256, lds2, stream, p);
   if (p.splits > 1) {
     for (int w = 0; w < 2; ++w) {
       hipLaunchKernelGGL(attn_reduce_kernel<T>, dim3((unsigned)((nk / 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p.part_o + w * nk, 2 * nk, p.splits,
