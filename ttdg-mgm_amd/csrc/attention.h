@@ -50,6 +50,12 @@ __device__ __forceinline__ float attn_half_sum(float x) {
 
 __device__ __forceinline__ void attn_wait_dma() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// Transposing LDS read: of the 4 x 16 block that 16 neighbouring lanes address (lane i: row i / 4, columns 4 (i % 4) ...) lane i gets column i.
+// (restrict: without alias information the compiler would wait here for every LDS-DMA in flight, that is for the next tile.)
+__device__ __forceinline__ bf16x4 attn_read_tr(const char* __restrict__ a) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)a);
+}
+
 #define ATTN_OOB 0x7ffffff0u          // behind the end of every buffer resource below: reads as zero
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t attn_rsrc(const void* base) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, 0x7fffff00, 0x00020000);
@@ -151,15 +157,44 @@ struct attn_tile {
     }
   }
 
-  // acc[n][tile row][lane's row of f] += sum_d tile[row0 + 32 n + .][d] f[d] for KK blocks of tile rows: KK independent chains of products
-  template <int KK>
-  static __device__ __forceinline__ void row_product(f32x16* acc, const char* tile, int row0, const frag* f, int l32, int h) {
+  // acc[k][n][tile row][lane's row of f[n]] += sum_d tile[row0 + 32 k + .][d] f[n][d]: KK blocks of tile rows times NB blocks of columns,
+  // KK NB independent chains of products.  PRE > 0: the chunks of PRE steps are read ahead of their products (the barriers keep the
+  // compiler from reading each one just before its use); 0: left to the compiler.
+  template <int KK, int NB, int PRE>
+  static __device__ __forceinline__ void row_product(f32x16 (*acc)[NB], const char* tile, int row0, const frag (*f)[NP], int l32, int h) {
     const int base = l32 * RB + ((h ^ attn_swz(l32)) << 4);
+    if constexpr (PRE == 0) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i)
+      for (int i = 0; i < NP; ++i)
 #pragma unroll
-      for (int n = 0; n < KK; ++n)
-        acc[n] = mma(*(const frag*)(tile + (row0 + 32 * n) * RB + (base ^ (32 * (i & 3))) + 128 * (i >> 2)), f[i], acc[n]);
+        for (int k = 0; k < KK; ++k) {
+          const frag a = *(const frag*)(tile + (row0 + 32 * k) * RB + (base ^ (32 * (i & 3))) + 128 * (i >> 2));
+#pragma unroll
+          for (int n = 0; n < NB; ++n) acc[k][n] = mma(a, f[n][i], acc[k][n]);
+        }
+    } else {
+      frag a[2][PRE][KK];
+#pragma unroll
+      for (int i = 0; i < NP + PRE; i += PRE) {
+        if (i < NP) {
+#pragma unroll
+          for (int j = 0; j < PRE; ++j)
+#pragma unroll
+            for (int k = 0; k < KK; ++k)
+              a[(i / PRE) & 1][j][k] = *(const frag*)(tile + (row0 + 32 * k) * RB + (base ^ (32 * ((i + j) & 3))) + 128 * ((i + j) >> 2));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (i > 0) {
+#pragma unroll
+          for (int j = 0; j < PRE; ++j)
+#pragma unroll
+            for (int k = 0; k < KK; ++k)
+#pragma unroll
+              for (int n = 0; n < NB; ++n) acc[k][n] = mma(a[(i / PRE + 1) & 1][j][k], f[n][i - PRE + j], acc[k][n]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
   }
   // the same with the second operand read from memory
   static __device__ __forceinline__ void row_product_mem(f32x16& acc, const char* tile, int row0, const T* row, int D, int l32, int h) {
@@ -237,8 +272,7 @@ struct attn_tile {
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
           const char* a = tile + (row0 + 16 * kg) * RB + (base ^ (64 * (d & 1))) + 128 * (d >> 1);
-          const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)a);
-          const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4*)(a + 8 * RB));
+          const bf16x4 lo = attn_read_tr(a), hi = attn_read_tr(a + 8 * RB);
           const bf16x8 f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
           for (int n = 0; n < NB; ++n) acc[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, p[n].x[kg], acc[n][d], 0, 0, 0);
@@ -319,7 +353,8 @@ struct attn_stream {
   int64_t k_tile, v_tile;
   uint32_t k_stb, v_stb;
   int next, wave, lane;
-  bool ahead;                        // does this lane's key of the next tile exist (its mask byte was asked for a tile earlier)
+  uint32_t ahead;                    // the mask byte of this lane's key of the next tile, asked for a tile earlier (kept as it comes: a
+                                     // comparison here would wait for it)
 
   __device__ __forceinline__ attn_stream(const attn_args& p, int b, int hk, int wave_, int lane_) : keys(p, b), next(0), wave(wave_), lane(lane_) {
     k = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh;
@@ -339,15 +374,20 @@ struct attn_stream {
     k += t * k_tile;
     v += t * v_tile;
   }
-  __device__ __forceinline__ void peek() { ahead = lane < BN && keys.alive(next * BN + lane); }
+  __device__ __forceinline__ void peek() {
+    const int key = next * BN + lane;
+    ahead = 1;
+    if (keys.mask && key < keys.n) ahead = keys.mask[key * keys.m_st];
+  }
   // starts the next tile's way into `stage` and returns which of its keys exist (none: nothing is loaded)
   __device__ __forceinline__ uint64_t issue(char* stage) {
-    const uint64_t live = __ballot(ahead);
+    const bool mine = lane < BN && next * BN + lane < keys.n && ahead;
+    const uint64_t live = __ballot(mine);
     if (live) {
       const bool all = live == ALL;
       lk.issue(stage, k, k_stb, live, all, wave);
       lv.issue(stage + TB, v, v_stb, live, all, wave);
-      if (!all && wave == 0) ((float*)(stage + 2 * TB))[lane] = ahead ? 0.f : -INFINITY;
+      if (!all && wave == 0) ((float*)(stage + 2 * TB))[lane] = mine ? 0.f : -INFINITY;
     }
     k += k_tile;
     v += v_tile;
@@ -355,20 +395,17 @@ struct attn_stream {
     return live;
   }
   // starting values of the scores
-  static __device__ __forceinline__ void start(f32x16* s, const char* stage, uint64_t live, int h) {
-    if (live == ALL) {
+  static __device__ __forceinline__ f32x16 start(const char* stage, int row0, uint64_t live, int h) {
+    f32x16 s = f32x16_zero();
+    if (live != ALL) {
 #pragma unroll
-      for (int n = 0; n < BN / 32; ++n) s[n] = f32x16_zero();
-    } else {
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 x = *(const f32x4*)(stage + 2 * TB + 4 * (row0 + 8 * g + 4 * h));
 #pragma unroll
-      for (int n = 0; n < BN / 32; ++n)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x4 x = *(const f32x4*)(stage + 2 * TB + 4 * (32 * n + 8 * g + 4 * h));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][4 * g + e] = x[e];
-        }
+        for (int e = 0; e < 4; ++e) s[4 * g + e] = x[e];
+      }
     }
+    return s;
   }
 };
 

@@ -21,9 +21,18 @@
 // and a cache may be longer than 4 GiB.
 #include "attention.h"
 
+// Wavefronts per SIMD that a kernel's LDS stages and registers allow; told to the compiler as minimum AND maximum, because left free it
+// saves registers for an occupancy that the LDS does not allow and then reads every operand just before its use.
+template <typename T, int DP, int SMALL>
+constexpr int attn_waves() {
+  return sizeof(T) == 2 ? (DP == 64 ? SMALL : DP == 128 ? 2 : 1) : (DP == 64 ? 2 : 1);
+}
+#define ATTN_WAVES(threads, n) __launch_bounds__(threads) __attribute__((amdgpu_waves_per_eu(n, n)))
+
 // ---------------------------------------------------------------------------------------------------------------- forward
-template <typename T, int DP, int BN, int WM>
-__global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) void attn_fwd_kernel(attn_args p) {
+// A wavefront owns 32 NB rows: every chunk that it reads from LDS serves NB products.
+template <typename T, int DP, int BN, int WM, int NB>
+__global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 4>())) void attn_fwd_kernel(attn_args p) {
   typedef attn_tile<T, DP> tile_t;
   typedef typename tile_t::frag frag;
   typedef attn_stream<T, DP, BN, WM> stream_t;
@@ -34,15 +43,19 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
   attn_block(p, p.row_tiles, prob, tile, split);
   const int b = prob / p.Hk, hk = prob - b * p.Hk;
 
-  const int row = (tile * WM + wave) * 32 + l32;
-  const attn_row rw(p, hk, row);
-  frag qf[tile_t::NP];
-  tile_t::load_row(qf, (const T*)p.q + b * p.q_sb + (int64_t)rw.t * p.q_st + (int64_t)rw.head * p.q_sh, p.D, h);
-
-  f32x16 o[DP / 32];
+  const int row0 = (tile * WM + wave) * 32 * NB + l32;      // block n of this lane: row0 + 32 n
+  frag qf[NB][tile_t::NP];
+  f32x16 o[NB][DP / 32];
+  float m[NB], l[NB];
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d) o[d] = f32x16_zero();
-  float m = -INFINITY, l = 0.f;
+  for (int n = 0; n < NB; ++n) {
+    const attn_row rw(p, hk, row0 + 32 * n);
+    tile_t::load_row(qf[n], (const T*)p.q + b * p.q_sb + (int64_t)rw.t * p.q_st + (int64_t)rw.head * p.q_sh, p.D, h);
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) o[n][d] = f32x16_zero();
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+  }
 
   stream_t in(p, b, hk, wave, lane);
   int t0, t1;
@@ -54,6 +67,7 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
     live_next = in.issue(attn_smem);
     in.peek();
   }
+  constexpr int KK = NB == 1 ? BN / 32 : 1;                 // blocks of 32 keys at a time: as many sums as the registers hold
   for (int t = t0; t < t1; ++t) {
     char* stage = attn_smem + ((t - t0) & 1) * stream_t::STAGE;
     const uint64_t live = live_next;
@@ -64,45 +78,71 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
       in.peek();
     }
     if (live == 0) continue;         // (the same for every wavefront of the workgroup)
-    f32x16 s[BN / 32];
-    stream_t::start(s, stage, live, h);
-    tile_t::template row_product<BN / 32>(s, stage, 0, qf, l32, h);
-    float mx = s[0][0];
+#pragma unroll 1
+    for (int k0 = 0; k0 < BN; k0 += 32 * KK) {
+      f32x16 s[KK][NB];
 #pragma unroll
-    for (int kk = 0; kk < BN / 32; ++kk)
+      for (int k = 0; k < KK; ++k)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kk][e]);
-    mx = attn_half_max(mx) * p.scale_log2;
-    // The reference point m follows the running maximum only when that has grown by more than 2^8: terms up to 2^8 round no worse than
-    // terms up to 1 and their sums are far from any limit, and with m at every new maximum most tiles would rescale the sums.
-    if (__any(mx > m + 8.f)) {
-      const float mn = fmaxf(m, mx), a = fast_exp2(m - mn);
-      l *= a;
+        for (int n = 0; n < NB; ++n) s[k][n] = stream_t::start(stage, k0 + 32 * k, live, h);
+      tile_t::template row_product<KK, NB, (NB == 1 && DP >= 128 ? 2 : 0)>(s, stage, k0, qf, l32, h);
+      float mx[NB];
+      bool grew = false;
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d) o[d] *= a;
-      m = mn;
-    }
+      for (int n = 0; n < NB; ++n) {
+        mx[n] = s[0][n][0];
 #pragma unroll
-    for (int kk = 0; kk < BN / 32; ++kk) {
+        for (int k = 0; k < KK; ++k)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[kk][e] = fast_exp2(fmaf(s[kk][e], p.scale_log2, -m));
-      const typename tile_t::operand pr = tile_t::pack(s[kk]);
-      l = tile_t::sum(pr, l);
-      tile_t::template col_product<1>(&o, stage + stream_t::TB, 32 * kk, &pr, lane);
+          for (int e = 0; e < 16; ++e) mx[n] = fmaxf(mx[n], s[k][n][e]);
+        mx[n] = attn_half_max(mx[n]) * p.scale_log2;
+        grew |= mx[n] > m[n] + 8.f;
+      }
+      // The reference point m follows the running maximum only when that has grown by more than 2^8: terms up to 2^8 round no worse than
+      // terms up to 1 and their sums are far from any limit, and with m at every new maximum most tiles would rescale the sums.
+      if (__any(grew)) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const float mn = fmaxf(m[n], mx[n]), a = mn > -INFINITY ? fast_exp2(m[n] - mn) : 1.f;
+          l[n] *= a;
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) o[n][d] *= a;
+          m[n] = mn;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < KK; ++k) {
+        typename tile_t::operand pr[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          const float ref = m[n] > -INFINITY ? m[n] : 0.f;      // (no key yet in this row: every term is 2^-infinity = 0)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[k][n][e] = fast_exp2(fmaf(s[k][n][e], p.scale_log2, -ref));
+          pr[n] = tile_t::pack(s[k][n]);
+          l[n] = tile_t::sum(pr[n], l[n]);
+        }
+        tile_t::template col_product<NB>(o, stage + stream_t::TB, k0 + 32 * k, pr, lane);
+      }
     }
   }
-  l = attn_half_sum(l);
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;      // no key at all: zeros
-  const float lse = l > 0.f || l != l ? m + fast_log2(l) : -INFINITY;
-  if (row >= p.R) return;
-  if (p.splits > 1) {
-    const int64_t pr = ((int64_t)prob * p.R + row) * p.splits + split;
-    if (h == 0) p.part_lse[pr] = lse;
-    tile_t::store_row(o, inv, p.part_o + pr * p.D, (float*)nullptr, p.D, h);
-  } else {
-    if (h == 0 && p.lse) p.lse[(int64_t)prob * p.R + row] = lse;
-    const int64_t off = (((int64_t)b * p.Tq + rw.t) * p.H + rw.head) * p.D;
-    tile_t::store_row(o, inv, (T*)p.out + off, p.out_lo ? (T*)p.out_lo + off : (T*)nullptr, p.D, h);
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const float sum = attn_half_sum(l[n]);
+    const bool any = sum > 0.f || sum != sum;
+    const float inv = any ? 1.f / sum : 0.f;                // no key at all: zeros
+    const float lse = any ? m[n] + fast_log2(sum) : -INFINITY;
+    const int row = row0 + 32 * n;
+    if (row >= p.R) continue;
+    if (p.splits > 1) {
+      const int64_t pr = ((int64_t)prob * p.R + row) * p.splits + split;
+      if (h == 0) p.part_lse[pr] = lse;
+      tile_t::store_row(o[n], inv, p.part_o + pr * p.D, (float*)nullptr, p.D, h);
+    } else {
+      const attn_row rw(p, hk, row);
+      if (h == 0 && p.lse) p.lse[(int64_t)prob * p.R + row] = lse;
+      const int64_t off = (((int64_t)b * p.Tq + rw.t) * p.H + rw.head) * p.D;
+      tile_t::store_row(o[n], inv, (T*)p.out + off, p.out_lo ? (T*)p.out_lo + off : (T*)nullptr, p.D, h);
+    }
   }
 }
 
@@ -170,7 +210,7 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(attn_args p) {
 // dq, and delta_i = do_i . o_i on the way (the dk / dv kernel reads it).  o is taken as out + out_lo: with the output rounded to bfloat16
 // alone the error of delta (2^-9 |o| |do|, the same for every key of a row) would reach dq times the mean key.
 template <typename T, int DP, int BN, int WM>
-__global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) void attn_bwd_dq_kernel(attn_args p) {
+__global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dq_kernel(attn_args p) {
   typedef attn_tile<T, DP> tile_t;
   typedef typename tile_t::frag frag;
   typedef attn_stream<T, DP, BN, WM> stream_t;
@@ -217,18 +257,20 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
       in.peek();
     }
     if (live == 0) continue;
-    f32x16 s[BN / 32], dp[BN / 32];
-    stream_t::start(s, stage, live, h);
-    tile_t::template row_product<BN / 32>(s, stage, 0, qf, l32, h);
+    f32x16 s[BN / 32][1], dp[BN / 32][1];
 #pragma unroll
-    for (int kk = 0; kk < BN / 32; ++kk) dp[kk] = f32x16_zero();
-    tile_t::template row_product<BN / 32>(dp, stage + stream_t::TB, 0, gf, l32, h);
+    for (int k = 0; k < BN / 32; ++k) {
+      s[k][0] = stream_t::start(stage, 32 * k, live, h);
+      dp[k][0] = f32x16_zero();
+    }
+    tile_t::template row_product<BN / 32, 1, (DP >= 128 ? 2 : 0)>(s, stage, 0, &qf, l32, h);
+    tile_t::template row_product<BN / 32, 1, (DP >= 128 ? 2 : 0)>(dp, stage + stream_t::TB, 0, &gf, l32, h);
 #pragma unroll
-    for (int kk = 0; kk < BN / 32; ++kk) {
+    for (int k = 0; k < BN / 32; ++k) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[kk][e] = fast_exp2(fmaf(s[kk][e], p.scale_log2, -lse)) * (dp[kk][e] - delta);
-      const typename tile_t::operand ds = tile_t::pack(s[kk]);
-      tile_t::template col_product<1>(&acc, stage, 32 * kk, &ds, lane);
+      for (int e = 0; e < 16; ++e) s[k][0][e] = fast_exp2(fmaf(s[k][0][e], p.scale_log2, -lse)) * (dp[k][0][e] - delta);
+      const typename tile_t::operand ds = tile_t::pack(s[k][0]);
+      tile_t::template col_product<1>(&acc, stage, 32 * k, &ds, lane);
     }
   }
   if (row >= p.R) return;
@@ -240,7 +282,7 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
 // with 256 channels are full of the two sums), and walks over the rows; q and do tiles in LDS serve both as rows (scores) and, transposed,
 // as the second products' first operand.
 template <typename T, int DP, int BQ, int WM, bool REGS>
-__global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) void attn_bwd_dkv_kernel(attn_args p) {
+__global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kernel(attn_args p) {
   typedef attn_tile<T, DP> tile_t;
   typedef typename tile_t::frag frag;
   typedef attn_rows<T, DP, BQ, WM> rows_t;
@@ -280,8 +322,8 @@ __global__ __launch_bounds__(64 * WM, (DP <= 128 && sizeof(T) == 2) ? 2 : 1) voi
     for (int qq = 0; qq < BQ / 32; ++qq) {
       f32x16 s = f32x16_zero(), dp = f32x16_zero();
       if constexpr (REGS) {
-        tile_t::template row_product<1>(&s, qt, 32 * qq, kf, l32, h);
-        tile_t::template row_product<1>(&dp, gt, 32 * qq, vf, l32, h);
+        tile_t::template row_product<1, 1, 0>((f32x16(*)[1])&s, qt, 32 * qq, &kf, l32, h);
+        tile_t::template row_product<1, 1, 0>((f32x16(*)[1])&dp, gt, 32 * qq, &vf, l32, h);
       } else {
         tile_t::row_product_mem(s, qt, 32 * qq, kp, p.D, l32, h);
         tile_t::row_product_mem(dp, gt, 32 * qq, vp, p.D, l32, h);
@@ -389,7 +431,7 @@ static int attn_splits(int64_t blocks, int units, int least) {
 }
 
 struct attn_plan {
-  int dp, wm, bn, row_tiles, fwd_splits, dq_splits, key_tiles, bq, dkv_splits;
+  int dp, wm, nb, bn, fwd_tiles, row_tiles, fwd_splits, dq_splits, key_tiles, bq, dkv_splits;
   size_t fwd_ws, bwd_ws;
 };
 
@@ -403,7 +445,9 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   q.wm = R <= 32 ? 1 : 4;
   q.row_tiles = (int)((R + 32 * q.wm - 1) / (32 * q.wm));
   const int kt = (a->Tk + q.bn - 1) / q.bn;
-  q.fwd_splits = attn_splits(probs * q.row_tiles * q.wm / 4 + 1, kt, 2);
+  q.nb = !f32 && q.dp <= 128 && q.wm == 4 && probs * ((R + 255) / 256) >= 1024 ? 2 : 1;
+  q.fwd_tiles = (int)((R + 32 * q.wm * q.nb - 1) / (32 * q.wm * q.nb));
+  q.fwd_splits = attn_splits(probs * q.fwd_tiles * q.wm / 4 + 1, kt, 2);
   q.dq_splits = attn_splits(probs * q.row_tiles * q.wm / 4 + 1, kt, 2);
   q.key_tiles = (a->Tk + 127) / 128;
   q.bq = q.bn;
@@ -438,10 +482,11 @@ extern "C" size_t ttdg_attention_bwd_workspace_bytes(const ttdg_attention_t* a) 
 template <typename T, int DP, int BN>
 static int attn_fwd_launch(const attn_args& p, const attn_plan& q, ttdg_stream_t stream) {
   constexpr int lds = 2 * attn_stream<T, DP, BN, 4>::STAGE;
-  const int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;
+  const int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;         // (of the forward: 32 nb wm rows per tile)
   TTDG_LIMIT(grid < (1ll << 31), "attention_fwd: too many workgroups");
-  if (q.wm == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 1>), grid, 64, lds, stream, p);
-  else ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 4>), grid, 256, lds, stream, p);
+  if (q.wm == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 1, 1>), grid, 64, lds, stream, p);
+  else if (q.nb == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 4, 1>), grid, 256, lds, stream, p);
+  else if constexpr (sizeof(T) == 2 && DP <= 128) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 4, 2>), grid, 256, lds, stream, p);
   if (p.splits > 1) {
     const int64_t rows = (int64_t)p.B * p.Hk * p.R;
     if (p.splits > 32) ATTN_LAUNCH((attn_combine_kernel<T, 4>), rows, 256, 0, stream, p);
@@ -500,7 +545,7 @@ extern "C" int ttdg_attention_fwd(const ttdg_attention_t* a, ttdg_stream_t strea
   const attn_plan q = attn_planned(a);
   TTDG_REQUIRE(q.fwd_ws == 0 || (a->ws && (uintptr_t)a->ws % 16 == 0 && a->ws_bytes >= q.fwd_ws), "attention_fwd: workspace too small or misaligned");
   attn_args p = attn_make(a);
-  p.row_tiles = q.row_tiles;
+  p.row_tiles = q.fwd_tiles;
   p.splits = q.fwd_splits;
   p.part_o = (float*)a->ws;
   p.part_lse = (float*)a->ws + (size_t)q.fwd_splits * p.B * p.Hk * p.R * p.D;
