@@ -673,6 +673,11 @@ def test_c_entry_points_refuse_without_a_launch():
     assert lib.ttdg_attention_bwd(C.byref(a), None) == -1 and b"workspace" in lib.ttdg_last_error()
     a = att(dout=fake, dq=fake, dk=fake, lse=fake)
     assert lib.ttdg_attention_bwd(C.byref(a), None) == -1 and b"both or none" in lib.ttdg_last_error()
+    for Tq, Tk, B, H, D in ((0, 0, 1, 2, 64), (4, 0, 1, 2, 8), (0, 5, 3, 2, 256), (1, 1, 1, 2, 64), (5, 60000, 2, 16, 128), (5000, 7, 1, 2, 40), (1, 1 << 20, 64, 8, 128)):
+        for dtype in (_lib.F32, _lib.BF16):            # the plan of every size is made (and its workspace is finite) without a device
+            a = att(Tq=Tq, Tk=Tk, B=B, H=H, D=D, dtype=dtype, q_st=H * D, q_sh=D, k_st=D, v_st=D)
+            f, g = lib.ttdg_attention_fwd_workspace_bytes(C.byref(a)), lib.ttdg_attention_bwd_workspace_bytes(C.byref(a))
+            assert f <= 257 * B * Tq * H * (D + 1) * 4 and (g >= B * Tq * H * 4)
     assert lib.ttdg_attention_fwd(None, None) == -1 and lib.ttdg_attention_bwd(None, None) == -1
     a = att(B=0)
     assert lib.ttdg_attention_fwd(C.byref(a), None) == 0 and lib.ttdg_attention_bwd(C.byref(a), None) == 0          # nothing to do

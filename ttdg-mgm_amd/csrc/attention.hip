@@ -30,15 +30,19 @@ constexpr int attn_waves() {
 #define ATTN_WAVES(threads, n) __launch_bounds__(threads) __attribute__((amdgpu_waves_per_eu(n, n)))
 
 // ---------------------------------------------------------------------------------------------------------------- forward
-// A wavefront owns 32 NB rows: every chunk that it reads from LDS serves NB products.
-template <typename T, int DP, int BN, int WM, int NB>
-__global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 4>())) void attn_fwd_kernel(attn_args p) {
+// A wavefront owns 32 NB rows: every chunk that it reads from LDS serves NB products.  WM wavefronts share the key tiles; KW wavefronts
+// (few rows: WM = 1) have key tiles of their own, walk over parts of the keys without a barrier and join their rows at the end.
+template <typename T, int DP, int BN, int WM, int NB, int KW>
+__global__ ATTN_WAVES(64 * WM * KW, (KW > 1 ? 1 : attn_waves<T, DP, 4>())) void attn_fwd_kernel(attn_args p) {
   typedef attn_tile<T, DP> tile_t;
   typedef typename tile_t::frag frag;
   typedef attn_stream<T, DP, BN, WM> stream_t;
+  static_assert(WM == 1 || KW == 1, "wavefronts along rows or along keys");
   extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, w_ = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = KW > 1 ? 0 : w_, kw = KW > 1 ? w_ : 0;
   const int h = lane >> 5, l32 = lane & 31;
+  char* const smem = attn_smem + kw * 2 * stream_t::STAGE;
   int prob, tile, split;
   attn_block(p, p.row_tiles, prob, tile, split);
   const int b = prob / p.Hk, hk = prob - b * p.Hk;
@@ -59,22 +63,22 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 4>())) void attn_fwd_kernel(at
 
   stream_t in(p, b, hk, wave, lane);
   int t0, t1;
-  attn_part(in.tiles(), split, p.splits, t0, t1);
+  attn_part(in.tiles(), split * KW + kw, p.splits * KW, t0, t1);
   in.seek(t0);
   uint64_t live_next = 0;
   if (t0 < t1) {
     in.peek();
-    live_next = in.issue(attn_smem);
+    live_next = in.issue(smem);
     in.peek();
   }
-  constexpr int KK = NB == 1 ? BN / 32 : 1;                 // blocks of 32 keys at a time: as many sums as the registers hold
+  constexpr int KK = NB == 1 ? BN / 32 : 1;                // blocks of 32 keys at a time: as many sums as the registers hold
   for (int t = t0; t < t1; ++t) {
-    char* stage = attn_smem + ((t - t0) & 1) * stream_t::STAGE;
+    char* stage = smem + ((t - t0) & 1) * stream_t::STAGE;
     const uint64_t live = live_next;
     attn_wait_dma();                 // this wavefront's share of tile t has landed
-    __syncthreads();                 // ... everybody's has, and nobody still reads the other stage
+    if (WM > 1) __syncthreads();     // ... everybody's has, and nobody still reads the other stage
     if (t + 1 < t1) {
-      live_next = in.issue(attn_smem + ((t + 1 - t0) & 1) * stream_t::STAGE);
+      live_next = in.issue(smem + ((t + 1 - t0) & 1) * stream_t::STAGE);
       in.peek();
     }
     if (live == 0) continue;         // (the same for every wavefront of the workgroup)
@@ -85,7 +89,7 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 4>())) void attn_fwd_kernel(at
       for (int k = 0; k < KK; ++k)
 #pragma unroll
         for (int n = 0; n < NB; ++n) s[k][n] = stream_t::start(stage, k0 + 32 * k, live, h);
-      tile_t::template row_product<KK, NB, (NB == 1 && DP >= 128 ? 2 : 0)>(s, stage, k0, qf, l32, h);
+      tile_t::template row_product<KK, NB, (NB == 1 && DP == 128 ? 2 : 0)>(s, stage, k0, qf, l32, h);
       float mx[NB];
       bool grew = false;
 #pragma unroll
@@ -124,6 +128,46 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 4>())) void attn_fwd_kernel(at
         tile_t::template col_product<NB>(o, stage + stream_t::TB, k0 + 32 * k, pr, lane);
       }
     }
+  }
+  if constexpr (KW > 1) {              // the wavefronts' rows meet in LDS, wavefront 0 goes on with them
+    static_assert(NB == 1 && KW * 32 * (DP + 2) * 4 <= KW * 2 * stream_t::STAGE, "the rows fit where the tiles were");
+    l[0] = attn_half_sum(l[0]);
+    __syncthreads();
+    float* mine = (float*)attn_smem + kw * 32 * (DP + 2);
+    if (kw > 0) {
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mine[(32 * d + attn_reg_row(e) + 4 * h) * 32 + l32] = o[0][d][e];
+      if (h == 0) {
+        mine[DP * 32 + l32] = m[0];
+        mine[DP * 32 + 32 + l32] = l[0];
+      }
+    }
+    __syncthreads();
+    if (kw > 0) return;
+    float mx = m[0], f[KW];
+#pragma unroll
+    for (int w = 1; w < KW; ++w) mx = fmaxf(mx, mine[w * 32 * (DP + 2) + DP * 32 + l32]);
+    const float ref = mx > -INFINITY ? mx : 0.f;
+    f[0] = fast_exp2(m[0] - ref);
+    l[0] *= f[0];
+#pragma unroll
+    for (int w = 1; w < KW; ++w) {
+      f[w] = fast_exp2(mine[w * 32 * (DP + 2) + DP * 32 + l32] - ref);
+      l[0] = fmaf(f[w], mine[w * 32 * (DP + 2) + DP * 32 + 32 + l32], l[0]);
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float x = o[0][d][e] * f[0];
+#pragma unroll
+        for (int w = 1; w < KW; ++w) x = fmaf(f[w], mine[w * 32 * (DP + 2) + (32 * d + attn_reg_row(e) + 4 * h) * 32 + l32], x);
+        o[0][d][e] = x;
+      }
+    m[0] = mx;
+    l[0] *= 0.5f;                      // (both halves hold the whole sum; they are added below)
   }
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
@@ -263,8 +307,8 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dq_kernel
       s[k][0] = stream_t::start(stage, 32 * k, live, h);
       dp[k][0] = f32x16_zero();
     }
-    tile_t::template row_product<BN / 32, 1, (DP >= 128 ? 2 : 0)>(s, stage, 0, &qf, l32, h);
-    tile_t::template row_product<BN / 32, 1, (DP >= 128 ? 2 : 0)>(dp, stage + stream_t::TB, 0, &gf, l32, h);
+    tile_t::template row_product<BN / 32, 1, (DP == 128 ? 2 : 0)>(s, stage, 0, &qf, l32, h);
+    tile_t::template row_product<BN / 32, 1, (DP == 128 ? 2 : 0)>(dp, stage + stream_t::TB, 0, &gf, l32, h);
 #pragma unroll
     for (int k = 0; k < BN / 32; ++k) {
 #pragma unroll
@@ -360,18 +404,25 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
   }
 }
 
-// adds the planes of a split in their order: out[i] = factor * sum_s part[s * stride + i], four values per thread (n % 4 == 0: D is)
+// adds the planes of a split in their order: out[i] = factor * sum_s part[s * stride + i], four values per thread (n % 4 == 0: D is);
+// blockIdx.y = 1: the second tensor, whose planes follow the first one's
 template <typename T>
-__global__ __launch_bounds__(256) void attn_reduce_kernel(const float* __restrict__ part, int64_t stride, int splits, float factor,
-                                                          T* __restrict__ out, int64_t n) {
+__global__ __launch_bounds__(256) void attn_reduce_kernel(const float* __restrict__ part, int64_t stride, int splits, float factor, T* __restrict__ out,
+                                                          T* __restrict__ out2, int64_t n) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= n) return;
-  f32x4 a = *(const f32x4*)(part + i);
-  for (int s = 1; s < splits; ++s) a += *(const f32x4*)(part + s * stride + i);
-  attn_store4(out + i, a * factor);
+  const float* at = part + i + (blockIdx.y ? n : 0);
+  f32x4 a = *(const f32x4*)at;
+#pragma unroll 4
+  for (int s = 1; s < splits; ++s) a += *(const f32x4*)(at + s * stride);
+  if (blockIdx.y) attn_store4(out2 + i, a);
+  else attn_store4(out + i, a * factor);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
+// wavefronts along the keys in the forward's form for few rows: two stages of 32 keys each, in 128 KiB of LDS
+static constexpr int attn_kw(int dp, bool f32) { return dp * (f32 ? 4 : 2) <= 256 ? 4 : dp * (f32 ? 4 : 2) <= 512 ? 2 : 1; }
+
 static int attn_check(const ttdg_attention_t* a, const char* what) {
   static thread_local char msg[160];
 #define ATTN_REQUIRE(cond, text)                                        \
@@ -420,20 +471,32 @@ static attn_args attn_make(const ttdg_attention_t* a) {
   return p;
 }
 
-// How many workgroups share one (problem, tile): the long axis (`units` tiles of it) is split until the launch fills the chip - 512
-// workgroups, two per CU - but a part keeps at least `least` tiles, below which the join costs more than the part saves.
-static int attn_splits(int64_t blocks, int units, int least) {
-  if (blocks >= 384 || units < 2 * least) return 1;
-  int64_t s = (512 + blocks - 1) / blocks;
-  if (s > units / least) s = units / least;
-  if (s > 256) s = 256;
-  return s < 1 ? 1 : (int)s;
+// How many workgroups share one (problem, tile): the long axis (`units` tiles of it) is split into s parts when that shortens the estimated
+// time in microseconds: `tile_us` per tile with all of the chip's `slots` taken (where several workgroups fit on a CU, one alone there runs up to
+// twice as fast, so the rounds are not counted in full), 6 us per workgroup (first loads, last stores), and for the join a launch and the parts written and read once (`part_bytes` each)
+// at 5 TB/s.  Measured both ways: dk / dv of 4 x 2047 x 16 heads over 2500 keys (320 workgroups for 512 slots) 408 us unsplit, 293 in two
+// parts, 362 in three; of 8 x 1000 x 12 heads x 64 over 1500 keys (1152 for 768) 98 us unsplit, 137 in two.
+static int attn_splits(int64_t blocks, int units, int slots, double tile_us, double part_bytes) {
+  int best = 1;
+  double least = 0;
+  if (units < 2 || blocks < 1) return 1;
+  for (int s = 1; s <= 256 && (s == 1 || 2 * s <= units) && (s == 1 || blocks * s <= 8 * (int64_t)slots); ++s) {
+    const int per = (units + s - 1) / s;
+    const double full = (double)blocks * s / slots, rounds = (double)((blocks * s + slots - 1) / slots);
+    const double taken = slots <= 256 ? rounds : full < 1 ? 0.5 + 0.5 * full : full + 0.1 * (rounds - full);
+    const double us = taken * (per * tile_us + 6) + (s > 1 ? 3 + 2 * s * part_bytes / 5e6 : 0);
+    if (s == 1 || us < 0.97 * least) { least = us; best = (units + per - 1) / per; }
+  }
+  return best;
 }
 
 struct attn_plan {
-  int dp, wm, nb, bn, fwd_tiles, row_tiles, fwd_splits, dq_splits, key_tiles, bq, dkv_splits;
+  int dp, wm, nb, fwd_tiles, row_tiles, fwd_splits, dq_splits, key_tiles, dkv_splits;
   size_t fwd_ws, bwd_ws;
 };
+
+// keys per tile of the kernels that share tiles between wavefronts; 32 where wavefronts have their own
+static int attn_bn(int dp, bool f32) { return dp == 64 || (dp == 128 && !f32) ? 64 : 32; }
 
 static attn_plan attn_planned(const ttdg_attention_t* a) {
   attn_plan q;
@@ -441,18 +504,23 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   const int64_t probs = (int64_t)a->B * a->Hkv;
   const int64_t R = (int64_t)a->Tq * (a->H / a->Hkv);
   q.dp = a->D <= 64 ? 64 : a->D <= 128 ? 128 : 256;
-  q.bn = q.dp == 64 || (q.dp == 128 && !f32) ? 64 : 32;
+  const int bn = attn_bn(q.dp, f32);
+  // 256 CUs; workgroups per CU by the registers and LDS of the kernels
+  const int shared = q.dp == 256 || (q.dp == 128 && f32) ? 256 : q.dp == 128 || f32 ? 512 : 768;
   q.wm = R <= 32 ? 1 : 4;
   q.row_tiles = (int)((R + 32 * q.wm - 1) / (32 * q.wm));
-  const int kt = (a->Tk + q.bn - 1) / q.bn;
   q.nb = !f32 && q.dp <= 128 && q.wm == 4 && probs * ((R + 255) / 256) >= 1024 ? 2 : 1;
   q.fwd_tiles = (int)((R + 32 * q.wm * q.nb - 1) / (32 * q.wm * q.nb));
-  q.fwd_splits = attn_splits(probs * q.fwd_tiles * q.wm / 4 + 1, kt, 2);
-  q.dq_splits = attn_splits(probs * q.row_tiles * q.wm / 4 + 1, kt, 2);
+  const int kt = (a->Tk + bn - 1) / bn, kt32 = (a->Tk + 31) / 32, kw = attn_kw(q.dp, f32);
+  // a tile's time at 800 (bf16) / 110 TFLOP/s (fp32) for the products of a full chip; few rows: its bytes at 20 GB/s per CU
+  const double es = f32 ? 4 : 2, prod_us = 2.0 * 128 * bn * q.dp * shared / (f32 ? 110e6 : 800e6);
+  const double q_bytes = (double)probs * R * a->D * 4, kv_bytes = 2.0 * a->B * a->Tk * a->Hkv * a->D * 4;
+  q.fwd_splits = q.wm == 1 ? attn_splits(probs, (kt32 + kw - 1) / kw, 1024 / kw, kw * 2 * 32 * a->D * es / 20e3, q_bytes)
+                           : attn_splits(probs * q.fwd_tiles, kt, shared, 2 * q.nb * prod_us, q_bytes);
+  q.dq_splits = attn_splits(probs * q.row_tiles, kt, shared, 3 * prod_us, q_bytes);
   q.key_tiles = (a->Tk + 127) / 128;
-  q.bq = q.bn;
-  const int qt = (int)((R + q.bq - 1) / q.bq);
-  q.dkv_splits = attn_splits(probs * q.key_tiles, qt, 2);
+  const int qt = (int)((R + bn - 1) / bn);
+  q.dkv_splits = attn_splits(probs * q.key_tiles, qt, shared, 4 * prod_us, kv_bytes);
   const size_t rows = (size_t)probs * R;
   q.fwd_ws = q.fwd_splits > 1 ? (size_t)q.fwd_splits * rows * (a->D + 1) * 4 : 0;
   const size_t kv = (size_t)a->B * a->Tk * a->Hkv * a->D * 4;
@@ -484,9 +552,10 @@ static int attn_fwd_launch(const attn_args& p, const attn_plan& q, ttdg_stream_t
   constexpr int lds = 2 * attn_stream<T, DP, BN, 4>::STAGE;
   const int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;         // (of the forward: 32 nb wm rows per tile)
   TTDG_LIMIT(grid < (1ll << 31), "attention_fwd: too many workgroups");
-  if (q.wm == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 1, 1>), grid, 64, lds, stream, p);
-  else if (q.nb == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 4, 1>), grid, 256, lds, stream, p);
-  else if constexpr (sizeof(T) == 2 && DP <= 128) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 4, 2>), grid, 256, lds, stream, p);
+  constexpr int KW = attn_kw(DP, sizeof(T) == 4), ldsk = 2 * KW * attn_stream<T, DP, 32, 1>::STAGE;
+  if (q.wm == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, 32, 1, 1, KW>), grid, 64 * KW, ldsk, stream, p);
+  else if (q.nb == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 4, 1, 1>), grid, 256, lds, stream, p);
+  else if constexpr (sizeof(T) == 2 && DP <= 128) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 4, 2, 1>), grid, 256, lds, stream, p);
   if (p.splits > 1) {
     const int64_t rows = (int64_t)p.B * p.Hk * p.R;
     if (p.splits > 32) ATTN_LAUNCH((attn_combine_kernel<T, 4>), rows, 256, 0, stream, p);
@@ -505,7 +574,8 @@ static int attn_bwd_launch(attn_args p, const attn_plan& q, ttdg_stream_t stream
   else ATTN_LAUNCH((attn_bwd_dq_kernel<T, DP, BN, 4>), grid, 256, lds, stream, p);
   const int64_t nq = (int64_t)p.B * p.Tq * p.H * p.D, nk = (int64_t)p.B * p.Tk * p.Hk * p.D;
   if (p.splits > 1) {
-    hipLaunchKernelGGL(attn_reduce_kernel<T>, dim3((unsigned)((nq / 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p.part_o, nq, p.splits, p.scale, (T*)p.dq, nq);
+    hipLaunchKernelGGL(attn_reduce_kernel<T>, dim3((unsigned)((nq / 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p.part_o, nq, p.splits, p.scale,
+                       (T*)p.dq, (T*)nullptr, nq);
     if (int e = ttdg_launch_status("attn_reduce")) return e;
   }
   if (p.Tk == 0 || !p.dk) return 0;
@@ -516,11 +586,9 @@ static int attn_bwd_launch(attn_args p, const attn_plan& q, ttdg_stream_t stream
   constexpr int lds2 = 2 * attn_rows<T, DP, BN, 4>::STAGE;
   ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, 4, regs>), grid, 256, lds2, stream, p);
   if (p.splits > 1) {
-    for (int w = 0; w < 2; ++w) {
-      hipLaunchKernelGGL(attn_reduce_kernel<T>, dim3((unsigned)((nk / 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p.part_o + w * nk, 2 * nk, p.splits,
-                         w == 0 ? p.scale : 1.f, (T*)(w == 0 ? p.dk : p.dv), nk);
-      if (int e = ttdg_launch_status("attn_reduce")) return e;
-    }
+    hipLaunchKernelGGL(attn_reduce_kernel<T>, dim3((unsigned)((nk / 4 + 255) / 256), 2), dim3(256), 0, (hipStream_t)stream, p.part_o, 2 * nk, p.splits,
+                       p.scale, (T*)p.dk, (T*)p.dv, nk);
+    if (int e = ttdg_launch_status("attn_reduce")) return e;
   }
   return 0;
 }

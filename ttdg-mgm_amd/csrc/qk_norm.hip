@@ -121,9 +121,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_fwd_kernel(qkn_args p) {
   const int groups = 256 / p.lanes, j = threadIdx.x & (p.lanes - 1);
   const int64_t u = (int64_t)blk * groups + threadIdx.x / p.lanes;
   if (u >= (int64_t)p.B * s.T * s.chunks) return;               // whole groups of lanes leave together
-  const int chunk = (int)(u % s.chunks);
-  const int64_t tok = u / s.chunks;
-  const int b = (int)(tok / s.T), t = (int)(tok - (int64_t)b * s.T);
+  const uint32_t tk = (uint32_t)u / (uint32_t)s.chunks;         // (the host keeps units below 2^31)
+  const int chunk = (int)((uint32_t)u - tk * s.chunks), b = (int)(tk / (uint32_t)s.T), t = (int)(tk - (uint32_t)b * s.T);
+  const int64_t tok = tk;
   const qkn_lane<V> ln(p, j);
   F w0 = {}, w1 = {};
   float cs[V], sn[V];
@@ -175,9 +175,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(qkn_args p) {
     w1 = qkn_vec<float, V>::load(s.w + ln.c1);
   }
   for (int64_t u = (int64_t)blk * groups + grp; u < units; u += (int64_t)s.blocks * groups) {
-    const int chunk = (int)(u % s.chunks);
-    const int64_t tok = u / s.chunks;
-    const int b = (int)(tok / s.T), t = (int)(tok - (int64_t)b * s.T);
+    const uint32_t tk = (uint32_t)u / (uint32_t)s.chunks;
+    const int chunk = (int)((uint32_t)u - tk * s.chunks), b = (int)(tk / (uint32_t)s.T), t = (int)(tk - (uint32_t)b * s.T);
+    const int64_t tok = tk;
     float cs[V], sn[V];
     qkn_angles<V>(p, s, ln, b, t, cs, sn);
     const T* x = (const T*)s.x + b * s.sb + t * s.st;
@@ -267,7 +267,7 @@ static int qkn_check(const ttdg_qk_norm_rope_t* a) {
     TTDG_REQUIRE(s.x && s.w && (a->R == 0 || s.pos), "qk_norm_rope: null pointer");
     TTDG_REQUIRE(s.sb >= 0 && s.st >= 0 && s.sh >= 0 && s.sb % ce == 0 && s.st % ce == 0 && s.sh % ce == 0, "qk_norm_rope: strides must be multiples of 16 bytes");
     TTDG_REQUIRE(((uintptr_t)s.x | (uintptr_t)s.w) % 16 == 0, "qk_norm_rope: tensors must be 16-byte aligned");
-    TTDG_REQUIRE((int64_t)a->B * s.T * s.H < (1ll << 33), "qk_norm_rope: too many rows");
+    TTDG_REQUIRE((int64_t)a->B * s.T < (1ll << 30) && (int64_t)a->B * s.T * s.H < (1ll << 31), "qk_norm_rope: more than 2^31 rows");
   }
   return 0;
 }
