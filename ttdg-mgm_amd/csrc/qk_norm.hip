@@ -28,6 +28,30 @@ struct qkn_vec {
   static __device__ __forceinline__ f32 load(const T* p) { return __builtin_convertvector(*(const mem*)p, f32); }
   static __device__ __forceinline__ void store(T* p, f32 x) { *(mem*)p = __builtin_convertvector(x, mem); }
 };
+// the two chunks of a lane: one access of 2 V values when they are neighbours (PAIRS), two of V otherwise
+template <typename T, int V, bool PAIRS>
+__device__ __forceinline__ void qkn_load(const T* p, int c0, int c1, typename qkn_vec<T, V>::f32& a, typename qkn_vec<T, V>::f32& b) {
+  if constexpr (PAIRS) {
+    const typename qkn_vec<T, 2 * V>::f32 x = qkn_vec<T, 2 * V>::load(p + c0);
+#pragma unroll
+    for (int e = 0; e < V; ++e) { a[e] = x[e]; b[e] = x[V + e]; }
+  } else {
+    a = qkn_vec<T, V>::load(p + c0);
+    b = qkn_vec<T, V>::load(p + c1);
+  }
+}
+template <typename T, int V, bool PAIRS>
+__device__ __forceinline__ void qkn_store(T* p, int c0, int c1, typename qkn_vec<T, V>::f32 a, typename qkn_vec<T, V>::f32 b) {
+  if constexpr (PAIRS) {
+    typename qkn_vec<T, 2 * V>::f32 x;
+#pragma unroll
+    for (int e = 0; e < V; ++e) { x[e] = a[e]; x[V + e] = b[e]; }
+    qkn_vec<T, 2 * V>::store(p + c0, x);
+  } else {
+    qkn_vec<T, V>::store(p + c0, a);
+    qkn_vec<T, V>::store(p + c1, b);
+  }
+}
 
 #define QKN_MAX_BLOCKS 1024           // persistent workgroups of the backward, per side
 
@@ -47,7 +71,7 @@ struct qkn_args {
 };
 
 // the lane's two chunks and whether they rotate; pair e of the lane is (chunk 0, e)-(chunk 1, e), or neighbours when interleaved
-template <int V>
+template <int V, bool PAIRS>
 struct qkn_lane {
   int c0, c1, pair;
   bool on, rot;
@@ -56,13 +80,13 @@ struct qkn_lane {
     rot = j < p.R / (2 * V);
     pair = V * j;
     if (!rot) { c0 = 2 * V * j; c1 = c0 + V; }
-    else if (p.interleaved) { c0 = 2 * V * j; c1 = c0 + V; }
+    else if (PAIRS) { c0 = 2 * V * j; c1 = c0 + V; }
     else { c0 = V * j; c1 = p.R / 2 + V * j; }
   }
 };
 
-template <int V>
-__device__ __forceinline__ void qkn_angles(const qkn_args& p, const qkn_side& s, const qkn_lane<V>& ln, int b, int t, float* cs, float* sn) {
+template <int V, bool PAIRS>
+__device__ __forceinline__ void qkn_angles(const qkn_args& p, const qkn_side& s, const qkn_lane<V, PAIRS>& ln, int b, int t, float* cs, float* sn) {
 #pragma unroll
   for (int e = 0; e < V; ++e) { cs[e] = 1.f; sn[e] = 0.f; }
   if (!ln.rot) return;
@@ -84,9 +108,9 @@ __device__ __forceinline__ void qkn_angles(const qkn_args& p, const qkn_side& s,
   }
 }
 
-template <typename F, int V>
-__device__ __forceinline__ void qkn_turn(F& a, F& b, const float* cs, const float* sn, bool interleaved, float sign) {
-  if (!interleaved) {
+template <typename F, int V, bool PAIRS>
+__device__ __forceinline__ void qkn_turn(F& a, F& b, const float* cs, const float* sn, float sign) {
+  if constexpr (!PAIRS) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const float x = a[e], y = b[e], s = sign * sn[e];
@@ -111,10 +135,9 @@ __device__ __forceinline__ float qkn_row_sum(float v, int lanes) {
   return v;
 }
 
-template <typename T, int V>
+template <typename T, int V, bool PAIRS>
 __global__ __launch_bounds__(256) void qk_norm_rope_fwd_kernel(qkn_args p) {
-  typedef qkn_vec<T, V> vec;
-  typedef typename vec::f32 F;
+  typedef typename qkn_vec<T, V>::f32 F;
   const int side = blockIdx.x >= p.s[0].blocks;
   const qkn_side s = p.s[side];
   const int blk = blockIdx.x - (side ? p.s[0].blocks : 0);
@@ -124,22 +147,20 @@ __global__ __launch_bounds__(256) void qk_norm_rope_fwd_kernel(qkn_args p) {
   const uint32_t tk = (uint32_t)u / (uint32_t)s.chunks;         // (the host keeps units below 2^31)
   const int chunk = (int)((uint32_t)u - tk * s.chunks), b = (int)(tk / (uint32_t)s.T), t = (int)(tk - (uint32_t)b * s.T);
   const int64_t tok = tk;
-  const qkn_lane<V> ln(p, j);
+  const qkn_lane<V, PAIRS> ln(p, j);
   F w0 = {}, w1 = {};
   float cs[V], sn[V];
   if (ln.on) {
-    w0 = qkn_vec<float, V>::load(s.w + ln.c0);
-    w1 = qkn_vec<float, V>::load(s.w + ln.c1);
+    qkn_load<float, V, PAIRS>(s.w, ln.c0, ln.c1, w0, w1);
   }
-  qkn_angles<V>(p, s, ln, b, t, cs, sn);
+  qkn_angles<V, PAIRS>(p, s, ln, b, t, cs, sn);
   const T* x = (const T*)s.x + b * s.sb + t * s.st;
   T* y = (T*)s.y + tok * s.H * p.D;
   const int h1 = min(s.H, (chunk + 1) * p.hc);
   for (int hd = chunk * p.hc; hd < h1; ++hd) {
     F a = {}, c = {};
     if (ln.on) {
-      a = vec::load(x + hd * s.sh + ln.c0);
-      c = vec::load(x + hd * s.sh + ln.c1);
+      qkn_load<T, V, PAIRS>(x + hd * s.sh, ln.c0, ln.c1, a, c);
     }
     float q = 0.f;
 #pragma unroll
@@ -148,38 +169,35 @@ __global__ __launch_bounds__(256) void qk_norm_rope_fwd_kernel(qkn_args p) {
     const float r = rsqrtf(q / (float)p.D + p.eps);
     a = a * r * w0;
     c = c * r * w1;
-    if (ln.rot) qkn_turn<F, V>(a, c, cs, sn, p.interleaved, 1.f);
+    if (ln.rot) qkn_turn<F, V, PAIRS>(a, c, cs, sn, 1.f);
     if (ln.on) {
-      vec::store(y + (int64_t)hd * p.D + ln.c0, a);
-      vec::store(y + (int64_t)hd * p.D + ln.c1, c);
+      qkn_store<T, V, PAIRS>(y + (int64_t)hd * p.D, ln.c0, ln.c1, a, c);
     }
   }
 }
 
 // persistent workgroups (each walks over units a grid apart), so that the weight gradient is summed in registers and leaves one partial
 // row per workgroup
-template <typename T, int V>
+template <typename T, int V, bool PAIRS>
 __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(qkn_args p) {
-  typedef qkn_vec<T, V> vec;
-  typedef typename vec::f32 F;
+  typedef typename qkn_vec<T, V>::f32 F;
   __shared__ float red[256 * 2 * V];
   const int side = blockIdx.x >= p.s[0].blocks;
   const qkn_side s = p.s[side];
   const int blk = blockIdx.x - (side ? p.s[0].blocks : 0);
   const int groups = 256 / p.lanes, j = threadIdx.x & (p.lanes - 1), grp = threadIdx.x / p.lanes;
   const int64_t units = (int64_t)p.B * s.T * s.chunks;
-  const qkn_lane<V> ln(p, j);
+  const qkn_lane<V, PAIRS> ln(p, j);
   F w0 = {}, w1 = {}, d0 = {}, d1 = {};
   if (ln.on) {
-    w0 = qkn_vec<float, V>::load(s.w + ln.c0);
-    w1 = qkn_vec<float, V>::load(s.w + ln.c1);
+    qkn_load<float, V, PAIRS>(s.w, ln.c0, ln.c1, w0, w1);
   }
   for (int64_t u = (int64_t)blk * groups + grp; u < units; u += (int64_t)s.blocks * groups) {
     const uint32_t tk = (uint32_t)u / (uint32_t)s.chunks;
     const int chunk = (int)((uint32_t)u - tk * s.chunks), b = (int)(tk / (uint32_t)s.T), t = (int)(tk - (uint32_t)b * s.T);
     const int64_t tok = tk;
     float cs[V], sn[V];
-    qkn_angles<V>(p, s, ln, b, t, cs, sn);
+    qkn_angles<V, PAIRS>(p, s, ln, b, t, cs, sn);
     const T* x = (const T*)s.x + b * s.sb + t * s.st;
     const T* dy = (const T*)s.dy + tok * s.H * p.D;
     T* dx = (T*)s.dx + tok * s.H * p.D;
@@ -187,12 +205,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(qkn_args p) {
     for (int hd = chunk * p.hc; hd < h1; ++hd) {
       F a = {}, c = {}, ga = {}, gc = {};
       if (ln.on) {
-        a = vec::load(x + hd * s.sh + ln.c0);
-        c = vec::load(x + hd * s.sh + ln.c1);
-        ga = vec::load(dy + (int64_t)hd * p.D + ln.c0);
-        gc = vec::load(dy + (int64_t)hd * p.D + ln.c1);
+        qkn_load<T, V, PAIRS>(x + hd * s.sh, ln.c0, ln.c1, a, c);
+        qkn_load<T, V, PAIRS>(dy + (int64_t)hd * p.D, ln.c0, ln.c1, ga, gc);
       }
-      if (ln.rot) qkn_turn<F, V>(ga, gc, cs, sn, p.interleaved, -1.f);
+      if (ln.rot) qkn_turn<F, V, PAIRS>(ga, gc, cs, sn, -1.f);
       float q = 0.f, d = 0.f;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
@@ -208,28 +224,33 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(qkn_args p) {
       d0 += ga * a;
       d1 += gc * c;
       if (ln.on) {
-        vec::store(dx + (int64_t)hd * p.D + ln.c0, (ga * w0) * r - a * m);
-        vec::store(dx + (int64_t)hd * p.D + ln.c1, (gc * w1) * r - c * m);
+        qkn_store<T, V, PAIRS>(dx + (int64_t)hd * p.D, ln.c0, ln.c1, (ga * w0) * r - a * m, (gc * w1) * r - c * m);
       }
     }
   }
+  // the groups of a wavefront by shuffles, the four wavefronts in LDS, always in the same order
+  for (int o = p.lanes; o < 64; o <<= 1) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      d0[e] += __shfl_xor(d0[e], o, 64);
+      d1[e] += __shfl_xor(d1[e], o, 64);
+    }
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    red[(e * 2) * 256 + threadIdx.x] = d0[e];
-    red[(e * 2 + 1) * 256 + threadIdx.x] = d1[e];
+    red[(wave * 2 * V + e) * 64 + lane] = d0[e];
+    red[(wave * 2 * V + V + e) * 64 + lane] = d1[e];
   }
   __syncthreads();
-  if (grp == 0 && ln.on) {
+  if (threadIdx.x < p.lanes && ln.on) {
     float* out = p.part + (int64_t)blockIdx.x * p.D;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      float a = 0.f, c = 0.f;
-      for (int g = 0; g < groups; ++g) {
-        a += red[(e * 2) * 256 + g * p.lanes + j];
-        c += red[(e * 2 + 1) * 256 + g * p.lanes + j];
-      }
-      out[ln.c0 + e] = a;
-      out[ln.c1 + e] = c;
+      const float* r0 = red + e * 64 + j;
+      const float* r1 = r0 + V * 64;
+      out[ln.c0 + e] = (r0[0] + r0[2 * V * 64]) + (r0[4 * V * 64] + r0[6 * V * 64]);
+      out[ln.c1 + e] = (r1[0] + r1[2 * V * 64]) + (r1[4 * V * 64] + r1[6 * V * 64]);
     }
   }
 }
@@ -272,8 +293,24 @@ static int qkn_check(const ttdg_qk_norm_rope_t* a) {
   return 0;
 }
 
-// V = channels per chunk: 16 bytes; four (8 bytes of bf16) when D or R is an odd multiple of 8
-static int qkn_v(const ttdg_qk_norm_rope_t* a) { return a->dtype == TTDG_BF16 && a->D % 16 == 0 && a->R % 16 == 0 ? 8 : 4; }
+// V = channels per chunk.  Neighbouring pairs (and no rotation): a lane's two chunks are one access, 16 bytes in all.  Halves: 16 bytes per
+// chunk forward; 8 bytes for bf16 when D or R is an odd multiple of 8.
+static bool qkn_pairs(const ttdg_qk_norm_rope_t* a) { return a->interleaved || a->R == 0; }
+static int qkn_v(const ttdg_qk_norm_rope_t* a) {
+  if (qkn_pairs(a)) return a->dtype == TTDG_BF16 ? 4 : 2;
+  return a->dtype == TTDG_BF16 && a->D % 16 == 0 && a->R % 16 == 0 ? 8 : 4;
+}
+#define QKN_LAUNCH(kernel, a, v, grid, stream, p)                                                                                       \
+  do {                                                                                                                                  \
+    const dim3 g_(grid), b_(256);                                                                                                       \
+    if (qkn_pairs(a)) {                                                                                                                 \
+      if ((a)->dtype == TTDG_F32) hipLaunchKernelGGL((kernel<float, 2, true>), g_, b_, 0, (hipStream_t)stream, p);                      \
+      else hipLaunchKernelGGL((kernel<__bf16, 4, true>), g_, b_, 0, (hipStream_t)stream, p);                                            \
+    } else if ((a)->dtype == TTDG_F32) hipLaunchKernelGGL((kernel<float, 4, false>), g_, b_, 0, (hipStream_t)stream, p);                \
+    else if ((v) == 8) hipLaunchKernelGGL((kernel<__bf16, 8, false>), g_, b_, 0, (hipStream_t)stream, p);                               \
+    else hipLaunchKernelGGL((kernel<__bf16, 4, false>), g_, b_, 0, (hipStream_t)stream, p);                                             \
+    if (int e_ = ttdg_launch_status(#kernel)) return e_;                                                                                \
+  } while (0)
 
 static qkn_args qkn_make(const ttdg_qk_norm_rope_t* a, int v, bool bwd) {
   qkn_args p = {};
@@ -285,7 +322,7 @@ static qkn_args qkn_make(const ttdg_qk_norm_rope_t* a, int v, bool bwd) {
   p.hc = 8;
   while (p.hc > 1) {
     const int64_t units = (int64_t)a->B * ((int64_t)a->q.T * ((a->q.H + p.hc - 1) / p.hc) + (int64_t)a->k.T * ((a->k.H + p.hc - 1) / p.hc));
-    if (units * p.lanes >= 262144) break;
+    if (units * p.lanes >= (bwd ? 524288 : 262144)) break;
     p.hc /= 2;
   }
   for (int i = 0; i < 2; ++i) {
@@ -320,10 +357,8 @@ extern "C" int ttdg_qk_norm_rope_fwd(const ttdg_qk_norm_rope_t* a, ttdg_stream_t
   }
   const int grid = p.s[0].blocks + p.s[1].blocks;
   if (grid == 0) return 0;
-  if (a->dtype == TTDG_F32) hipLaunchKernelGGL((qk_norm_rope_fwd_kernel<float, 4>), dim3(grid), dim3(256), 0, (hipStream_t)stream, p);
-  else if (v == 8) hipLaunchKernelGGL((qk_norm_rope_fwd_kernel<__bf16, 8>), dim3(grid), dim3(256), 0, (hipStream_t)stream, p);
-  else hipLaunchKernelGGL((qk_norm_rope_fwd_kernel<__bf16, 4>), dim3(grid), dim3(256), 0, (hipStream_t)stream, p);
-  return ttdg_launch_status("qk_norm_rope_fwd");
+  QKN_LAUNCH(qk_norm_rope_fwd_kernel, a, v, grid, stream, p);
+  return 0;
 }
 
 extern "C" int ttdg_qk_norm_rope_bwd(const ttdg_qk_norm_rope_t* a, ttdg_stream_t stream) {
@@ -339,12 +374,7 @@ extern "C" int ttdg_qk_norm_rope_bwd(const ttdg_qk_norm_rope_t* a, ttdg_stream_t
   TTDG_REQUIRE((a->q.H == 0 || a->q.dw) && (a->k.H == 0 || a->k.dw), "qk_norm_rope_bwd: null pointer");
   TTDG_REQUIRE(grid == 0 || (a->ws && a->ws_bytes >= (size_t)grid * a->D * 4), "qk_norm_rope_bwd: workspace too small");
   p.part = (float*)a->ws;
-  if (grid) {
-    if (a->dtype == TTDG_F32) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<float, 4>), dim3(grid), dim3(256), 0, (hipStream_t)stream, p);
-    else if (v == 8) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<__bf16, 8>), dim3(grid), dim3(256), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<__bf16, 4>), dim3(grid), dim3(256), 0, (hipStream_t)stream, p);
-    if (int e = ttdg_launch_status("qk_norm_rope_bwd")) return e;
-  }
+  if (grid) QKN_LAUNCH(qk_norm_rope_bwd_kernel, a, v, grid, stream, p);
   const int sides = a->k.H ? 2 : 1;
   hipLaunchKernelGGL(qk_norm_rope_dw_kernel, dim3(a->D / 4, sides), dim3(256), 0, (hipStream_t)stream, p.part, p.s[0].blocks, p.s[1].blocks, a->D,
                      a->q.dw, a->k.dw);
