@@ -33,7 +33,7 @@ constexpr int attn_waves() {
 // A wavefront owns 32 NB rows: every chunk that it reads from LDS serves NB products.  WM wavefronts share the key tiles; KW wavefronts
 // (few rows: WM = 1) have key tiles of their own, walk over parts of the keys without a barrier and join their rows at the end.
 template <typename T, int DP, int BN, int WM, int NB, int KW>
-__global__ ATTN_WAVES(64 * WM * KW, (KW > 1 ? 1 : attn_waves<T, DP, 4>())) void attn_fwd_kernel(attn_args p) {
+__global__ ATTN_WAVES(64 * WM * KW, (KW > 1 ? 1 : DP == 256 && sizeof(T) == 2 ? 2 : attn_waves<T, DP, 4>())) void attn_fwd_kernel(attn_args p) {
   typedef attn_tile<T, DP> tile_t;
   typedef typename tile_t::frag frag;
   typedef attn_stream<T, DP, BN, WM> stream_t;
@@ -89,7 +89,7 @@ __global__ ATTN_WAVES(64 * WM * KW, (KW > 1 ? 1 : attn_waves<T, DP, 4>())) void 
       for (int k = 0; k < KK; ++k)
 #pragma unroll
         for (int n = 0; n < NB; ++n) s[k][n] = stream_t::start(stage, k0 + 32 * k, live, h);
-      tile_t::template row_product<KK, NB, (NB == 1 && DP == 128 ? 2 : 0)>(s, stage, k0, qf, l32, h);
+      tile_t::template row_product<KK, NB, 0>(s, stage, k0, qf, l32, h);
       float mx[NB];
       bool grew = false;
 #pragma unroll
@@ -301,14 +301,15 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dq_kernel
       in.peek();
     }
     if (live == 0) continue;
+    constexpr int PRE = attn_waves<T, DP, 3>() == 1 && sizeof(T) == 2 ? 2 : 0;      // one wavefront per SIMD: nobody else hides the LDS
     f32x16 s[BN / 32][1], dp[BN / 32][1];
 #pragma unroll
     for (int k = 0; k < BN / 32; ++k) {
       s[k][0] = stream_t::start(stage, 32 * k, live, h);
       dp[k][0] = f32x16_zero();
     }
-    tile_t::template row_product<BN / 32, 1, (DP == 128 ? 2 : 0)>(s, stage, 0, &qf, l32, h);
-    tile_t::template row_product<BN / 32, 1, (DP == 128 ? 2 : 0)>(dp, stage + stream_t::TB, 0, &gf, l32, h);
+    tile_t::template row_product<BN / 32, 1, PRE>(s, stage, 0, &qf, l32, h);
+    tile_t::template row_product<BN / 32, 1, PRE>(dp, stage + stream_t::TB, 0, &gf, l32, h);
 #pragma unroll
     for (int k = 0; k < BN / 32; ++k) {
 #pragma unroll
@@ -364,10 +365,11 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
     if (t + 1 < t1) in.issue(p, attn_smem + ((t + 1 - t0) & 1) * rows_t::STAGE);
 #pragma unroll 1
     for (int qq = 0; qq < BQ / 32; ++qq) {
+      constexpr int PRE = attn_waves<T, DP, 3>() == 1 && sizeof(T) == 2 ? 4 : 0;
       f32x16 s = f32x16_zero(), dp = f32x16_zero();
       if constexpr (REGS) {
-        tile_t::template row_product<1, 1, 0>((f32x16(*)[1])&s, qt, 32 * qq, &kf, l32, h);
-        tile_t::template row_product<1, 1, 0>((f32x16(*)[1])&dp, gt, 32 * qq, &vf, l32, h);
+        tile_t::template row_product<1, 1, PRE>((f32x16(*)[1])&s, qt, 32 * qq, &kf, l32, h);
+        tile_t::template row_product<1, 1, PRE>((f32x16(*)[1])&dp, gt, 32 * qq, &vf, l32, h);
       } else {
         tile_t::row_product_mem(s, qt, 32 * qq, kp, p.D, l32, h);
         tile_t::row_product_mem(dp, gt, 32 * qq, vp, p.D, l32, h);
@@ -509,7 +511,7 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   const int shared = q.dp == 256 || (q.dp == 128 && f32) ? 256 : q.dp == 128 || f32 ? 512 : 768;
   q.wm = R <= 32 ? 1 : 4;
   q.row_tiles = (int)((R + 32 * q.wm - 1) / (32 * q.wm));
-  q.nb = !f32 && q.dp <= 128 && q.wm == 4 && probs * ((R + 255) / 256) >= 1024 ? 2 : 1;
+  q.nb = !f32 && q.dp == 128 && q.wm == 4 && probs * ((R + 255) / 256) >= 1024 ? 2 : 1;
   q.fwd_tiles = (int)((R + 32 * q.wm * q.nb - 1) / (32 * q.wm * q.nb));
   const int kt = (a->Tk + bn - 1) / bn, kt32 = (a->Tk + 31) / 32, kw = attn_kw(q.dp, f32);
   // a tile's time at 800 (bf16) / 110 TFLOP/s (fp32) for the products of a full chip; few rows: its bytes at 20 GB/s per CU
@@ -555,7 +557,7 @@ static int attn_fwd_launch(const attn_args& p, const attn_plan& q, ttdg_stream_t
   constexpr int KW = attn_kw(DP, sizeof(T) == 4), ldsk = 2 * KW * attn_stream<T, DP, 32, 1>::STAGE;
   if (q.wm == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, 32, 1, 1, KW>), grid, 64 * KW, ldsk, stream, p);
   else if (q.nb == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 4, 1, 1>), grid, 256, lds, stream, p);
-  else if constexpr (sizeof(T) == 2 && DP <= 128) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 4, 2, 1>), grid, 256, lds, stream, p);
+  else if constexpr (sizeof(T) == 2 && DP == 128) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 4, 2, 1>), grid, 256, lds, stream, p);
   if (p.splits > 1) {
     const int64_t rows = (int64_t)p.B * p.Hk * p.R;
     if (p.splits > 32) ATTN_LAUNCH((attn_combine_kernel<T, 4>), rows, 256, 0, stream, p);
