@@ -112,12 +112,13 @@ struct attn_keys {
 // consecutive rows read the same c), and the four rows of a transposing read's 16-lane group land in four different 32-byte windows.
 __device__ __forceinline__ int attn_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
 
-template <typename T, int DP>
+// DP channels of tiles whose rows have RD (a wavefront may work on a part of the channels)
+template <typename T, int DP, int RD = DP>
 struct attn_tile {
   static constexpr bool F32 = sizeof(T) == 4;
   static constexpr int ES = sizeof(T), CE = 16 / ES;      // element size, elements per chunk
-  static constexpr int RB = DP * ES;                      // bytes of a tile row
-  static constexpr int NC = RB / 16, NP = NC / 2;         // chunks per row; chunk pairs: the wavefront's halves take one chunk each
+  static constexpr int RB = RD * ES;                      // bytes of a tile row
+  static constexpr int NC = DP * ES / 16, NP = NC / 2;    // chunks per row; chunk pairs: the wavefront's halves take one chunk each
   static constexpr int bytes(int rows) { return rows * RB; }
   typedef __attribute__((ext_vector_type(16 / sizeof(T)))) T frag;
 
@@ -194,17 +195,6 @@ struct attn_tile {
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-    }
-  }
-  // the same with the second operand read from memory
-  static __device__ __forceinline__ void row_product_mem(f32x16& acc, const char* tile, int row0, const T* row, int D, int l32, int h) {
-    const int base = l32 * RB + ((h ^ attn_swz(l32)) << 4);
-#pragma unroll 4
-    for (int i = 0; i < NP; ++i) {
-      const int c = (2 * i + h) * CE;
-      frag f = {};
-      if (c < D) f = *(const frag*)(row + c);
-      acc = mma(*(const frag*)(tile + row0 * RB + (base ^ (32 * (i & 3))) + 128 * (i >> 2)), f, acc);
     }
   }
 
@@ -303,6 +293,17 @@ struct attn_tile {
       }
   }
 };
+
+// Two wavefronts that hold sums over half the channels each add them: `own` and `other` are their 4 KiB of LDS.  Every wavefront of the
+// workgroup takes part in the barriers.
+__device__ __forceinline__ void attn_exchange(f32x16& x, float* own, const float* other, int lane) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) own[e * 64 + lane] = x[e];
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] += other[e * 64 + lane];
+  __syncthreads();
+}
 
 // LDS-DMA of ROWS tile rows: instruction i of a wavefront fills 1 KiB; its lanes' offsets repeat every PER instructions (the swizzle has a
 // period of eight rows), the rest of the distance goes into the scalar offset.  Lanes behind D always point behind the resource's end.

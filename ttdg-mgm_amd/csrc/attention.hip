@@ -21,6 +21,14 @@
 // and a cache may be longer than 4 GiB.
 #include "attention.h"
 
+// float32 with 256 channels: the operands and sums of 32 rows times 256 channels overflow a wavefront's registers and take 14 us per tile of
+// 32 keys, so two wavefronts share 32 rows, each with half the channels: half of every score's sum (exchanged through LDS) and half of
+// the output.  dk / dv 85 -> 112 TFLOP/s, 8 x 256 rows over 794 keys forward + backward 198 -> 150 us; the exchange costs the forward of
+// large calls 14 %.  bfloat16 fits without (with the exchange: 640 -> 560 TFLOP/s).
+constexpr int attn_cs(int dp, bool f32) { return dp == 256 && f32 ? 2 : 1; }
+constexpr int attn_rows_wg(int dp, bool f32) { return 128 / attn_cs(dp, f32); }      // rows, or keys, of a workgroup of four wavefronts
+constexpr int attn_exchange_bytes(int dp, bool f32) { return attn_cs(dp, f32) > 1 ? 4 * 4096 : 0; }
+
 // Wavefronts per SIMD that a kernel's LDS stages and registers allow; told to the compiler as minimum AND maximum, because left free it
 // saves registers for an occupancy that the LDS does not allow and then reads every operand just before its use.
 template <typename T, int DP, int SMALL>
@@ -33,30 +41,34 @@ constexpr int attn_waves() {
 // A wavefront owns 32 NB rows: every chunk that it reads from LDS serves NB products.  WM wavefronts share the key tiles; KW wavefronts
 // (few rows: WM = 1) have key tiles of their own, walk over parts of the keys without a barrier and join their rows at the end.
 template <typename T, int DP, int BN, int WM, int NB, int KW>
-__global__ ATTN_WAVES(64 * WM * KW, (KW > 1 ? 1 : DP == 256 && sizeof(T) == 2 ? 2 : attn_waves<T, DP, 4>())) void attn_fwd_kernel(attn_args p) {
-  typedef attn_tile<T, DP> tile_t;
+__global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ? 2 : attn_waves<T, DP, 4>())) void attn_fwd_kernel(attn_args p) {
+  constexpr int CS = WM > 1 ? attn_cs(DP, sizeof(T) == 4) : 1, DC = DP / CS;
+  typedef attn_tile<T, DC, DP> tile_t;
   typedef typename tile_t::frag frag;
   typedef attn_stream<T, DP, BN, WM> stream_t;
   static_assert(WM == 1 || KW == 1, "wavefronts along rows or along keys");
+  static_assert(CS == 1 || (NB == 1 && BN == 32), "one sum at a time to exchange");
   extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
   const int lane = threadIdx.x & 63, w_ = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave = KW > 1 ? 0 : w_, kw = KW > 1 ? w_ : 0;
   const int h = lane >> 5, l32 = lane & 31;
+  const int cs = CS > 1 ? w_ % CS : 0;                        // which part of the channels
   char* const smem = attn_smem + kw * 2 * stream_t::STAGE;
+  float* const ex = (float*)(attn_smem + 2 * stream_t::STAGE);
   int prob, tile, split;
   attn_block(p, p.row_tiles, prob, tile, split);
   const int b = prob / p.Hk, hk = prob - b * p.Hk;
 
-  const int row0 = (tile * WM + wave) * 32 * NB + l32;      // block n of this lane: row0 + 32 n
+  const int row0 = (tile * (WM / CS) + wave / CS) * 32 * NB + l32;      // block n of this lane: row0 + 32 n
   frag qf[NB][tile_t::NP];
-  f32x16 o[NB][DP / 32];
+  f32x16 o[NB][DC / 32];
   float m[NB], l[NB];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     const attn_row rw(p, hk, row0 + 32 * n);
-    tile_t::load_row(qf[n], (const T*)p.q + b * p.q_sb + (int64_t)rw.t * p.q_st + (int64_t)rw.head * p.q_sh, p.D, h);
+    tile_t::load_row(qf[n], (const T*)p.q + b * p.q_sb + (int64_t)rw.t * p.q_st + (int64_t)rw.head * p.q_sh + cs * DC, p.D - cs * DC, h);
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) o[n][d] = f32x16_zero();
+    for (int d = 0; d < DC / 32; ++d) o[n][d] = f32x16_zero();
     m[n] = -INFINITY;
     l[n] = 0.f;
   }
@@ -89,7 +101,8 @@ __global__ ATTN_WAVES(64 * WM * KW, (KW > 1 ? 1 : DP == 256 && sizeof(T) == 2 ? 
       for (int k = 0; k < KK; ++k)
 #pragma unroll
         for (int n = 0; n < NB; ++n) s[k][n] = stream_t::start(stage, k0 + 32 * k, live, h);
-      tile_t::template row_product<KK, NB, 0>(s, stage, k0, qf, l32, h);
+      tile_t::template row_product<KK, NB, 0>(s, stage + cs * DC * tile_t::ES, k0, qf, l32, h);
+      if constexpr (CS > 1) attn_exchange(s[0][0], ex + w_ * 1024, ex + (w_ ^ 1) * 1024, lane);
       float mx[NB];
       bool grew = false;
 #pragma unroll
@@ -110,7 +123,7 @@ __global__ ATTN_WAVES(64 * WM * KW, (KW > 1 ? 1 : DP == 256 && sizeof(T) == 2 ? 
           const float mn = fmaxf(m[n], mx[n]), a = mn > -INFINITY ? fast_exp2(m[n] - mn) : 1.f;
           l[n] *= a;
 #pragma unroll
-          for (int d = 0; d < DP / 32; ++d) o[n][d] *= a;
+          for (int d = 0; d < DC / 32; ++d) o[n][d] *= a;
           m[n] = mn;
         }
       }
@@ -125,7 +138,7 @@ __global__ ATTN_WAVES(64 * WM * KW, (KW > 1 ? 1 : DP == 256 && sizeof(T) == 2 ? 
           pr[n] = tile_t::pack(s[k][n]);
           l[n] = tile_t::sum(pr[n], l[n]);
         }
-        tile_t::template col_product<NB>(o, stage + stream_t::TB, k0 + 32 * k, pr, lane);
+        tile_t::template col_product<NB>(o, stage + stream_t::TB + cs * DC * tile_t::ES, k0 + 32 * k, pr, lane);
       }
     }
   }
@@ -136,7 +149,7 @@ __global__ ATTN_WAVES(64 * WM * KW, (KW > 1 ? 1 : DP == 256 && sizeof(T) == 2 ? 
     float* mine = (float*)attn_smem + kw * 32 * (DP + 2);
     if (kw > 0) {
 #pragma unroll
-      for (int d = 0; d < DP / 32; ++d)
+      for (int d = 0; d < DC / 32; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) mine[(32 * d + attn_reg_row(e) + 4 * h) * 32 + l32] = o[0][d][e];
       if (h == 0) {
@@ -158,7 +171,7 @@ __global__ ATTN_WAVES(64 * WM * KW, (KW > 1 ? 1 : DP == 256 && sizeof(T) == 2 ? 
       l[0] = fmaf(f[w], mine[w * 32 * (DP + 2) + DP * 32 + 32 + l32], l[0]);
     }
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
+    for (int d = 0; d < DC / 32; ++d)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         float x = o[0][d][e] * f[0];
@@ -179,13 +192,13 @@ __global__ ATTN_WAVES(64 * WM * KW, (KW > 1 ? 1 : DP == 256 && sizeof(T) == 2 ? 
     if (row >= p.R) continue;
     if (p.splits > 1) {
       const int64_t pr = ((int64_t)prob * p.R + row) * p.splits + split;
-      if (h == 0) p.part_lse[pr] = lse;
-      tile_t::store_row(o[n], inv, p.part_o + pr * p.D, (float*)nullptr, p.D, h);
+      if (h == 0 && cs == 0) p.part_lse[pr] = lse;
+      tile_t::store_row(o[n], inv, p.part_o + pr * p.D + cs * DC, (float*)nullptr, p.D - cs * DC, h);
     } else {
       const attn_row rw(p, hk, row);
-      if (h == 0 && p.lse) p.lse[(int64_t)prob * p.R + row] = lse;
-      const int64_t off = (((int64_t)b * p.Tq + rw.t) * p.H + rw.head) * p.D;
-      tile_t::store_row(o[n], inv, (T*)p.out + off, p.out_lo ? (T*)p.out_lo + off : (T*)nullptr, p.D, h);
+      if (h == 0 && cs == 0 && p.lse) p.lse[(int64_t)prob * p.R + row] = lse;
+      const int64_t off = (((int64_t)b * p.Tq + rw.t) * p.H + rw.head) * p.D + cs * DC;
+      tile_t::store_row(o[n], inv, (T*)p.out + off, p.out_lo ? (T*)p.out_lo + off : (T*)nullptr, p.D - cs * DC, h);
     }
   }
 }
@@ -254,8 +267,9 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(attn_args p) {
 // dq, and delta_i = do_i . o_i on the way (the dk / dv kernel reads it).  o is taken as out + out_lo: with the output rounded to bfloat16
 // alone the error of delta (2^-9 |o| |do|, the same for every key of a row) would reach dq times the mean key.
 template <typename T, int DP, int BN, int WM>
-__global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dq_kernel(attn_args p) {
-  typedef attn_tile<T, DP> tile_t;
+__global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn_bwd_dq_kernel(attn_args p) {
+  constexpr int CS = WM > 1 ? attn_cs(DP, sizeof(T) == 4) : 1, DC = DP / CS;
+  typedef attn_tile<T, DC, DP> tile_t;
   typedef typename tile_t::frag frag;
   typedef attn_stream<T, DP, BN, WM> stream_t;
   extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
@@ -265,21 +279,29 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dq_kernel
   attn_block(p, p.row_tiles, prob, tile, split);
   const int b = prob / p.Hk, hk = prob - b * p.Hk;
 
-  const int row = (tile * WM + wave) * 32 + l32;
+  const int cs = CS > 1 ? wave % CS : 0;                      // which part of the channels
+  float* const ex = (float*)(attn_smem + 2 * stream_t::STAGE);
+  const int row = (tile * (WM / CS) + wave / CS) * 32 + l32;
   const attn_row rw(p, hk, row);
   frag qf[tile_t::NP], gf[tile_t::NP];
-  tile_t::load_row(qf, (const T*)p.q + b * p.q_sb + (int64_t)rw.t * p.q_st + (int64_t)rw.head * p.q_sh, p.D, h);
-  const int64_t off = (((int64_t)b * p.Tq + rw.t) * p.H + rw.head) * p.D;
-  tile_t::load_row(gf, (const T*)p.dout + off, p.D, h);
-  float delta = tile_t::row_dot(gf, (const T*)p.out + off, p.out_lo ? (const T*)p.out_lo + off : (const T*)nullptr, p.D, h);
+  tile_t::load_row(qf, (const T*)p.q + b * p.q_sb + (int64_t)rw.t * p.q_st + (int64_t)rw.head * p.q_sh + cs * DC, p.D - cs * DC, h);
+  const int64_t off = (((int64_t)b * p.Tq + rw.t) * p.H + rw.head) * p.D + cs * DC;
+  tile_t::load_row(gf, (const T*)p.dout + off, p.D - cs * DC, h);
+  float delta = tile_t::row_dot(gf, (const T*)p.out + off, p.out_lo ? (const T*)p.out_lo + off : (const T*)nullptr, p.D - cs * DC, h);
   delta = attn_half_sum(delta);
+  if constexpr (CS > 1) {
+    ex[wave * 64 + lane] = delta;
+    __syncthreads();
+    delta += ex[(wave ^ 1) * 64 + lane];
+    __syncthreads();
+  }
   float lse = p.lse[(int64_t)prob * p.R + rw.row];
-  if (split == 0 && h == 0 && row < p.R) p.delta[(int64_t)prob * p.R + row] = delta;
+  if (split == 0 && h == 0 && cs == 0 && row < p.R) p.delta[(int64_t)prob * p.R + row] = delta;
   if (lse == -INFINITY) lse = INFINITY;       // a row without any key: p = 0
 
-  f32x16 acc[DP / 32];
+  f32x16 acc[DC / 32];
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d) acc[d] = f32x16_zero();
+  for (int d = 0; d < DC / 32; ++d) acc[d] = f32x16_zero();
 
   stream_t in(p, b, hk, wave, lane);
   int t0, t1;
@@ -301,34 +323,38 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dq_kernel
       in.peek();
     }
     if (live == 0) continue;
-    constexpr int PRE = attn_waves<T, DP, 3>() == 1 && sizeof(T) == 2 ? 2 : 0;      // one wavefront per SIMD: nobody else hides the LDS
+    constexpr int PRE = DP == 256 && sizeof(T) == 2 ? 2 : 0;      // one wavefront per SIMD: nobody else hides the LDS
     f32x16 s[BN / 32][1], dp[BN / 32][1];
 #pragma unroll
     for (int k = 0; k < BN / 32; ++k) {
       s[k][0] = stream_t::start(stage, 32 * k, live, h);
       dp[k][0] = f32x16_zero();
     }
-    tile_t::template row_product<BN / 32, 1, PRE>(s, stage, 0, &qf, l32, h);
-    tile_t::template row_product<BN / 32, 1, PRE>(dp, stage + stream_t::TB, 0, &gf, l32, h);
+    tile_t::template row_product<BN / 32, 1, PRE>(s, stage + cs * DC * tile_t::ES, 0, &qf, l32, h);
+    tile_t::template row_product<BN / 32, 1, PRE>(dp, stage + stream_t::TB + cs * DC * tile_t::ES, 0, &gf, l32, h);
+    if constexpr (CS > 1) {
+      attn_exchange(s[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
+      attn_exchange(dp[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
+    }
 #pragma unroll
     for (int k = 0; k < BN / 32; ++k) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[k][0][e] = fast_exp2(fmaf(s[k][0][e], p.scale_log2, -lse)) * (dp[k][0][e] - delta);
       const typename tile_t::operand ds = tile_t::pack(s[k][0]);
-      tile_t::template col_product<1>(&acc, stage, 32 * k, &ds, lane);
+      tile_t::template col_product<1>(&acc, stage + cs * DC * tile_t::ES, 32 * k, &ds, lane);
     }
   }
   if (row >= p.R) return;
-  if (p.splits > 1) tile_t::store_row(acc, 1.f, p.part_o + (int64_t)split * p.B * p.Tq * p.H * p.D + off, (float*)nullptr, p.D, h);
-  else tile_t::store_row(acc, p.scale, (T*)p.dq + off, (T*)nullptr, p.D, h);
+  if (p.splits > 1) tile_t::store_row(acc, 1.f, p.part_o + (int64_t)split * p.B * p.Tq * p.H * p.D + off, (float*)nullptr, p.D - cs * DC, h);
+  else tile_t::store_row(acc, p.scale, (T*)p.dq + off, (T*)nullptr, p.D - cs * DC, h);
 }
 
-// dk and dv: a wavefront owns 32 keys, their k and v rows in registers (REGS) or re-read through the caches (the registers of float32
-// with 256 channels are full of the two sums), and walks over the rows; q and do tiles in LDS serve both as rows (scores) and, transposed,
-// as the second products' first operand.
-template <typename T, int DP, int BQ, int WM, bool REGS>
+// dk and dv: a wavefront owns 32 keys, their k and v rows in registers, and walks over the rows; q and do tiles in LDS serve both as rows
+// (scores) and, transposed, as the second products' first operand.
+template <typename T, int DP, int BQ, int WM>
 __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kernel(attn_args p) {
-  typedef attn_tile<T, DP> tile_t;
+  constexpr int CS = attn_cs(DP, sizeof(T) == 4), DC = DP / CS;
+  typedef attn_tile<T, DC, DP> tile_t;
   typedef typename tile_t::frag frag;
   typedef attn_rows<T, DP, BQ, WM> rows_t;
   extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
@@ -338,20 +364,20 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
   attn_block(p, p.key_tiles, prob, tile, split);
   const int b = prob / p.Hk, hk = prob - b * p.Hk;
 
-  const int key = (tile * WM + wave) * 32 + l32;
+  const int cs = CS > 1 ? wave % CS : 0;                      // which part of the channels
+  float* const ex = (float*)(attn_smem + 2 * rows_t::STAGE);
+  const int key = (tile * (WM / CS) + wave / CS) * 32 + l32;
   const attn_keys keys(p, b);
   const bool mine = keys.alive(key);
   const int64_t kr = min(key, p.Tk - 1);
-  const T* kp = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh + kr * p.k_st;
-  const T* vp = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh + kr * p.v_st;
-  frag kf[REGS ? tile_t::NP : 1], vf[REGS ? tile_t::NP : 1];
-  if constexpr (REGS) {
-    tile_t::load_row(kf, kp, p.D, h);
-    tile_t::load_row(vf, vp, p.D, h);
-  }
-  f32x16 dk[DP / 32], dv[DP / 32];
+  const T* kp = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh + kr * p.k_st + cs * DC;
+  const T* vp = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh + kr * p.v_st + cs * DC;
+  frag kf[tile_t::NP], vf[tile_t::NP];
+  tile_t::load_row(kf, kp, p.D - cs * DC, h);
+  tile_t::load_row(vf, vp, p.D - cs * DC, h);
+  f32x16 dk[DC / 32], dv[DC / 32];
 #pragma unroll
-  for (int d = 0; d < DP / 32; ++d) { dk[d] = f32x16_zero(); dv[d] = f32x16_zero(); }
+  for (int d = 0; d < DC / 32; ++d) { dk[d] = f32x16_zero(); dv[d] = f32x16_zero(); }
 
   int t0, t1;
   attn_part(__syncthreads_or(mine) ? (p.R + BQ - 1) / BQ : 0, split, p.splits, t0, t1);      // no key of this workgroup exists: zeros
@@ -365,14 +391,13 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
     if (t + 1 < t1) in.issue(p, attn_smem + ((t + 1 - t0) & 1) * rows_t::STAGE);
 #pragma unroll 1
     for (int qq = 0; qq < BQ / 32; ++qq) {
-      constexpr int PRE = attn_waves<T, DP, 3>() == 1 && sizeof(T) == 2 ? 4 : 0;
-      f32x16 s = f32x16_zero(), dp = f32x16_zero();
-      if constexpr (REGS) {
-        tile_t::template row_product<1, 1, PRE>((f32x16(*)[1])&s, qt, 32 * qq, &kf, l32, h);
-        tile_t::template row_product<1, 1, PRE>((f32x16(*)[1])&dp, gt, 32 * qq, &vf, l32, h);
-      } else {
-        tile_t::row_product_mem(s, qt, 32 * qq, kp, p.D, l32, h);
-        tile_t::row_product_mem(dp, gt, 32 * qq, vp, p.D, l32, h);
+      constexpr int PRE = DP == 256 && sizeof(T) == 2 ? 4 : 0;
+      f32x16 s[1][1] = {{f32x16_zero()}}, dp[1][1] = {{f32x16_zero()}};
+      tile_t::template row_product<1, 1, PRE>(s, qt + cs * DC * tile_t::ES, 32 * qq, &kf, l32, h);
+      tile_t::template row_product<1, 1, PRE>(dp, gt + cs * DC * tile_t::ES, 32 * qq, &vf, l32, h);
+      if constexpr (CS > 1) {
+        attn_exchange(s[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
+        attn_exchange(dp[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
       }
       const float* st = (const float*)(qt + 2 * rows_t::TB) + 32 * qq + 4 * h;
 #pragma unroll
@@ -380,29 +405,29 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
         const f32x4 ls = *(const f32x4*)(st + 8 * g), de = *(const f32x4*)(st + 64 + 8 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float pr = fast_exp2(fmaf(s[4 * g + e], p.scale_log2, -ls[e]));
-          s[4 * g + e] = pr;
-          dp[4 * g + e] = pr * (dp[4 * g + e] - de[e]);
+          const float pr = fast_exp2(fmaf(s[0][0][4 * g + e], p.scale_log2, -ls[e]));
+          s[0][0][4 * g + e] = pr;
+          dp[0][0][4 * g + e] = pr * (dp[0][0][4 * g + e] - de[e]);
         }
       }
-      const typename tile_t::operand pr = tile_t::pack(s), ds = tile_t::pack(dp);
-      tile_t::template col_product<1>(&dv, gt, 32 * qq, &pr, lane);
-      tile_t::template col_product<1>(&dk, qt, 32 * qq, &ds, lane);
+      const typename tile_t::operand pr = tile_t::pack(s[0][0]), ds = tile_t::pack(dp[0][0]);
+      tile_t::template col_product<1>(&dv, gt + cs * DC * tile_t::ES, 32 * qq, &pr, lane);
+      tile_t::template col_product<1>(&dk, qt + cs * DC * tile_t::ES, 32 * qq, &ds, lane);
     }
   }
   if (key >= p.Tk) return;
-  const int64_t off = (((int64_t)b * p.Tk + key) * p.Hk + hk) * p.D;
+  const int64_t off = (((int64_t)b * p.Tk + key) * p.Hk + hk) * p.D + cs * DC;
   if (!mine) {                        // (a select, not a factor: the sums of a key that does not exist may be anything)
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) { dk[d] = f32x16_zero(); dv[d] = f32x16_zero(); }
+    for (int d = 0; d < DC / 32; ++d) { dk[d] = f32x16_zero(); dv[d] = f32x16_zero(); }
   }
   if (p.splits > 1) {
     const int64_t plane = (int64_t)p.B * p.Tk * p.Hk * p.D;
-    tile_t::store_row(dk, 1.f, p.part_o + 2 * split * plane + off, (float*)nullptr, p.D, h);
-    tile_t::store_row(dv, 1.f, p.part_o + (2 * split + 1) * plane + off, (float*)nullptr, p.D, h);
+    tile_t::store_row(dk, 1.f, p.part_o + 2 * split * plane + off, (float*)nullptr, p.D - cs * DC, h);
+    tile_t::store_row(dv, 1.f, p.part_o + (2 * split + 1) * plane + off, (float*)nullptr, p.D - cs * DC, h);
   } else {
-    tile_t::store_row(dk, p.scale, (T*)p.dk + off, (T*)nullptr, p.D, h);
-    tile_t::store_row(dv, 1.f, (T*)p.dv + off, (T*)nullptr, p.D, h);
+    tile_t::store_row(dk, p.scale, (T*)p.dk + off, (T*)nullptr, p.D - cs * DC, h);
+    tile_t::store_row(dv, 1.f, (T*)p.dv + off, (T*)nullptr, p.D - cs * DC, h);
   }
 }
 
@@ -422,8 +447,9 @@ __global__ __launch_bounds__(256) void attn_reduce_kernel(const float* __restric
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
-// wavefronts along the keys in the forward's form for few rows: two stages of 32 keys each, in 128 KiB of LDS
-static constexpr int attn_kw(int dp, bool f32) { return dp * (f32 ? 4 : 2) <= 256 ? 4 : dp * (f32 ? 4 : 2) <= 512 ? 2 : 1; }
+// wavefronts along the keys in the forward's form for few rows: two stages of 32 keys each, in 128 KiB of LDS (float32 with 256 channels
+// would have room for one only, and takes the form for many rows)
+static constexpr int attn_kw(int dp, bool f32) { return dp * (f32 ? 4 : 2) <= 256 ? 4 : 2; }
 
 static int attn_check(const ttdg_attention_t* a, const char* what) {
   static thread_local char msg[160];
@@ -493,7 +519,7 @@ static int attn_splits(int64_t blocks, int units, int slots, double tile_us, dou
 }
 
 struct attn_plan {
-  int dp, wm, nb, fwd_tiles, row_tiles, fwd_splits, dq_splits, key_tiles, dkv_splits;
+  int dp, few, nb, fwd_tiles, row_tiles, fwd_splits, dq_splits, key_tiles, dkv_splits;
   size_t fwd_ws, bwd_ws;
 };
 
@@ -509,18 +535,19 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   const int bn = attn_bn(q.dp, f32);
   // 256 CUs; workgroups per CU by the registers and LDS of the kernels
   const int shared = q.dp == 256 || (q.dp == 128 && f32) ? 256 : q.dp == 128 || f32 ? 512 : 768;
-  q.wm = R <= 32 ? 1 : 4;
-  q.row_tiles = (int)((R + 32 * q.wm - 1) / (32 * q.wm));
-  q.nb = !f32 && q.dp == 128 && q.wm == 4 && probs * ((R + 255) / 256) >= 1024 ? 2 : 1;
-  q.fwd_tiles = (int)((R + 32 * q.wm * q.nb - 1) / (32 * q.wm * q.nb));
+  const int wg = attn_rows_wg(q.dp, f32);
+  q.few = R <= 32 && !(f32 && q.dp == 256);
+  q.row_tiles = q.few ? 1 : (int)((R + wg - 1) / wg);
+  q.nb = !f32 && q.dp == 128 && !q.few && probs * ((R + 255) / 256) >= 1024 ? 2 : 1;
+  q.fwd_tiles = q.few ? 1 : (int)((R + wg * q.nb - 1) / (wg * q.nb));
   const int kt = (a->Tk + bn - 1) / bn, kt32 = (a->Tk + 31) / 32, kw = attn_kw(q.dp, f32);
   // a tile's time at 800 (bf16) / 110 TFLOP/s (fp32) for the products of a full chip; few rows: its bytes at 20 GB/s per CU
-  const double es = f32 ? 4 : 2, prod_us = 2.0 * 128 * bn * q.dp * shared / (f32 ? 110e6 : 800e6);
+  const double es = f32 ? 4 : 2, prod_us = 2.0 * wg * bn * q.dp * shared / (f32 ? 110e6 : 800e6);
   const double q_bytes = (double)probs * R * a->D * 4, kv_bytes = 2.0 * a->B * a->Tk * a->Hkv * a->D * 4;
-  q.fwd_splits = q.wm == 1 ? attn_splits(probs, (kt32 + kw - 1) / kw, 1024 / kw, kw * 2 * 32 * a->D * es / 20e3, q_bytes)
+  q.fwd_splits = q.few ? attn_splits(probs, (kt32 + kw - 1) / kw, 1024 / kw, kw * 2 * 32 * a->D * es / 20e3, q_bytes)
                            : attn_splits(probs * q.fwd_tiles, kt, shared, 2 * q.nb * prod_us, q_bytes);
   q.dq_splits = attn_splits(probs * q.row_tiles, kt, shared, 3 * prod_us, q_bytes);
-  q.key_tiles = (a->Tk + 127) / 128;
+  q.key_tiles = (a->Tk + wg - 1) / wg;
   const int qt = (int)((R + bn - 1) / bn);
   q.dkv_splits = attn_splits(probs * q.key_tiles, qt, shared, 4 * prod_us, kv_bytes);
   const size_t rows = (size_t)probs * R;
@@ -551,13 +578,17 @@ extern "C" size_t ttdg_attention_bwd_workspace_bytes(const ttdg_attention_t* a) 
 
 template <typename T, int DP, int BN>
 static int attn_fwd_launch(const attn_args& p, const attn_plan& q, ttdg_stream_t stream) {
-  constexpr int lds = 2 * attn_stream<T, DP, BN, 4>::STAGE;
-  const int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;         // (of the forward: 32 nb wm rows per tile)
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int WM = 4, lds = 2 * attn_stream<T, DP, BN, WM>::STAGE + attn_exchange_bytes(DP, F32);
+  const int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;         // (of the forward)
   TTDG_LIMIT(grid < (1ll << 31), "attention_fwd: too many workgroups");
-  constexpr int KW = attn_kw(DP, sizeof(T) == 4), ldsk = 2 * KW * attn_stream<T, DP, 32, 1>::STAGE;
-  if (q.wm == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, 32, 1, 1, KW>), grid, 64 * KW, ldsk, stream, p);
-  else if (q.nb == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 4, 1, 1>), grid, 256, lds, stream, p);
-  else if constexpr (sizeof(T) == 2 && DP == 128) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, 4, 2, 1>), grid, 256, lds, stream, p);
+  if constexpr (!(F32 && DP == 256)) {
+    constexpr int KW = attn_kw(DP, F32), ldsk = 2 * KW * attn_stream<T, DP, 32, 1>::STAGE;
+    if (q.few) ATTN_LAUNCH((attn_fwd_kernel<T, DP, 32, 1, 1, KW>), grid, 64 * KW, ldsk, stream, p);
+  }
+  if (q.few) {
+  } else if (q.nb == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 1, 1>), grid, 64 * WM, lds, stream, p);
+  else if constexpr (sizeof(T) == 2 && DP == 128) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 2, 1>), grid, 64 * WM, lds, stream, p);
   if (p.splits > 1) {
     const int64_t rows = (int64_t)p.B * p.Hk * p.R;
     if (p.splits > 32) ATTN_LAUNCH((attn_combine_kernel<T, 4>), rows, 256, 0, stream, p);
@@ -568,12 +599,15 @@ static int attn_fwd_launch(const attn_args& p, const attn_plan& q, ttdg_stream_t
 
 template <typename T, int DP, int BN>
 static int attn_bwd_launch(attn_args p, const attn_plan& q, ttdg_stream_t stream) {
-  constexpr int lds = 2 * attn_stream<T, DP, BN, 4>::STAGE;
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int WM = 4, lds = 2 * attn_stream<T, DP, BN, WM>::STAGE + attn_exchange_bytes(DP, F32);
   p.splits = q.dq_splits;
   int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;
   TTDG_LIMIT(grid < (1ll << 31), "attention_bwd: too many workgroups");
-  if (q.wm == 1) ATTN_LAUNCH((attn_bwd_dq_kernel<T, DP, BN, 1>), grid, 64, lds, stream, p);
-  else ATTN_LAUNCH((attn_bwd_dq_kernel<T, DP, BN, 4>), grid, 256, lds, stream, p);
+  if constexpr (!(F32 && DP == 256)) {
+    if (q.few) ATTN_LAUNCH((attn_bwd_dq_kernel<T, DP, BN, 1>), grid, 64, lds, stream, p);
+  }
+  if (!q.few) ATTN_LAUNCH((attn_bwd_dq_kernel<T, DP, BN, WM>), grid, 64 * WM, lds, stream, p);
   const int64_t nq = (int64_t)p.B * p.Tq * p.H * p.D, nk = (int64_t)p.B * p.Tk * p.Hk * p.D;
   if (p.splits > 1) {
     hipLaunchKernelGGL(attn_reduce_kernel<T>, dim3((unsigned)((nq / 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p.part_o, nq, p.splits, p.scale,
@@ -584,9 +618,8 @@ static int attn_bwd_launch(attn_args p, const attn_plan& q, ttdg_stream_t stream
   p.splits = q.dkv_splits;
   grid = (int64_t)p.B * p.Hk * p.key_tiles * p.splits;
   TTDG_LIMIT(grid < (1ll << 31), "attention_bwd: too many workgroups");
-  constexpr bool regs = !(sizeof(T) == 4 && DP == 256);
-  constexpr int lds2 = 2 * attn_rows<T, DP, BN, 4>::STAGE;
-  ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, 4, regs>), grid, 256, lds2, stream, p);
+  constexpr int lds2 = 2 * attn_rows<T, DP, BN, WM>::STAGE + attn_exchange_bytes(DP, F32);
+  ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, WM>), grid, 64 * WM, lds2, stream, p);
   if (p.splits > 1) {
     hipLaunchKernelGGL(attn_reduce_kernel<T>, dim3((unsigned)((nk / 4 + 255) / 256), 2), dim3(256), 0, (hipStream_t)stream, p.part_o, 2 * nk, p.splits,
                        p.scale, (T*)p.dk, (T*)p.dv, nk);
