@@ -198,48 +198,54 @@ struct attn_tile {
     }
   }
 
-  // 32 tile rows of one column block as the second product's second operand.  For 16-bit types they are rounded to the inputs' type (round
+  // 32 tile rows of one column block as the second product's second operand.  For 16-bit types a value is rounded to the inputs' type (round
   // to nearest even, as every operand of the matrix unit is): an error of at most half a step per term, independent from term to term,
-  // while the sums stay in 32 bits.
+  // while the sums stay in 32 bits.  PARTS = 2 adds what that rounding dropped as a second operand (16 bits of significand in all).
+  template <int PARTS>
   struct operand {
-    typename std::conditional<F32, f32x16, bf16x8>::type x[F32 ? 1 : 2];
+    typename std::conditional<F32, f32x16, bf16x8>::type x[F32 ? 1 : PARTS][F32 ? 1 : 2];
   };
-  static __device__ __forceinline__ operand pack(const f32x16& p) {
-    operand r;
+  template <int PARTS>
+  static __device__ __forceinline__ operand<PARTS> pack(const f32x16& p) {
+    operand<PARTS> r;
     if constexpr (F32) {
-      r.x[0] = p;
+      r.x[0][0] = p;
     } else {
 #pragma unroll
       for (int kg = 0; kg < 2; ++kg) {
         f32x8 y;
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = p[8 * kg + e];
-        r.x[kg] = __builtin_convertvector(y, bf16x8);
+        r.x[0][kg] = __builtin_convertvector(y, bf16x8);
+        if constexpr (PARTS == 2) r.x[1][kg] = __builtin_convertvector(y - __builtin_convertvector(r.x[0][kg], f32x8), bf16x8);
       }
     }
     return r;
   }
-  // l + the lane's terms as the product will see them: a row's weights then sum to one whatever their rounding did
-  static __device__ __forceinline__ float sum(const operand& p, float l) {
+  // l + the lane's terms.  With one part the terms as the product will see them: a row's weights then sum to one whatever their rounding did
+  template <int PARTS>
+  static __device__ __forceinline__ float sum(const operand<PARTS>& p, float l) {
     if constexpr (F32) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) l += p.x[0][e];
+      for (int e = 0; e < 16; ++e) l += p.x[0][0][e];
     } else {
       const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
 #pragma unroll
-      for (int kg = 0; kg < 2; ++kg)
+      for (int q = 0; q < PARTS; ++q)
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const bf16x2 y = {p.x[kg][e], p.x[kg][e + 1]};
-          l = __builtin_amdgcn_fdot2_f32_bf16(y, one, l, false);
-        }
+        for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const bf16x2 y = {p.x[q][kg][e], p.x[q][kg][e + 1]};
+            l = __builtin_amdgcn_fdot2_f32_bf16(y, one, l, false);
+          }
     }
     return l;
   }
 
   // acc[n][d][lane's column] += sum over the 32 tile rows from row0 of tile[.][d] p[n][.]
-  template <int NB>
-  static __device__ __forceinline__ void col_product(f32x16 (*acc)[DP / 32], const char* tile, int row0, const operand* p, int lane) {
+  template <int NB, int PARTS>
+  static __device__ __forceinline__ void col_product(f32x16 (*acc)[DP / 32], const char* tile, int row0, const operand<PARTS>* p, int lane) {
     const int h = lane >> 5;
     if constexpr (F32) {
       const int l32 = lane & 31;
@@ -251,7 +257,7 @@ struct attn_tile {
         for (int d = 0; d < DP / 32; ++d) {
           const float x = *(const float*)(a + 128 * d);
 #pragma unroll
-          for (int n = 0; n < NB; ++n) acc[n][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[n].x[0][e], acc[n][d], 0, 0, 0);
+          for (int n = 0; n < NB; ++n) acc[n][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[n].x[0][0][e], acc[n][d], 0, 0, 0);
         }
       }
     } else {
@@ -265,7 +271,9 @@ struct attn_tile {
           const bf16x4 lo = attn_read_tr(a), hi = attn_read_tr(a + 8 * RB);
           const bf16x8 f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-          for (int n = 0; n < NB; ++n) acc[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, p[n].x[kg], acc[n][d], 0, 0, 0);
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) acc[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f, p[n].x[q][kg], acc[n][d], 0, 0, 0);
         }
     }
   }

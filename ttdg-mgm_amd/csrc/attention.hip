@@ -37,10 +37,19 @@ constexpr int attn_waves() {
 }
 #define ATTN_WAVES(threads, n) __launch_bounds__(threads) __attribute__((amdgpu_waves_per_eu(n, n)))
 
+// How many bfloat16 operands carry a probability or a score gradient into the second product (PARTS of the kernels, attn_tile::pack).  With
+// one, the rounding of p (or ds) adds an error of the size of the result's own rounding.  ds takes two everywhere: half of its terms
+// cancel in dq and dk, which then had 1.5 times the error of their own rounding (1.04 with two; backward of 4 x 2047 x 2500 x 16 heads x
+// 128: 415 -> 500 us).  p takes two where a launch leaves the chip room - few rows, or workgroups for half of the slots at most: few values are
+// averaged there, and the extra products hide behind the loads (one token over 53294 keys: 21.0 and 21.6 us) - and one in large calls
+// (8 x 1000 x 12 heads x 64 over 1500 keys, forward: 64 and 93 us), where out and dv have 1.2 to 1.45 times their own rounding's error.
+template <typename T>
+constexpr int attn_parts(bool two) { return sizeof(T) == 2 && two ? 2 : 1; }
+
 // ---------------------------------------------------------------------------------------------------------------- forward
 // A wavefront owns 32 NB rows: every chunk that it reads from LDS serves NB products.  WM wavefronts share the key tiles; KW wavefronts
 // (few rows: WM = 1) have key tiles of their own, walk over parts of the keys without a barrier and join their rows at the end.
-template <typename T, int DP, int BN, int WM, int NB, int KW>
+template <typename T, int DP, int BN, int WM, int NB, int KW, int PARTS>
 __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ? 2 : attn_waves<T, DP, 4>())) void attn_fwd_kernel(attn_args p) {
   constexpr int CS = WM > 1 ? attn_cs(DP, sizeof(T) == 4) : 1, DC = DP / CS;
   typedef attn_tile<T, DC, DP> tile_t;
@@ -129,16 +138,16 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
       }
 #pragma unroll
       for (int k = 0; k < KK; ++k) {
-        typename tile_t::operand pr[NB];
+        typename tile_t::template operand<PARTS> pr[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
           const float ref = m[n] > -INFINITY ? m[n] : 0.f;      // (no key yet in this row: every term is 2^-infinity = 0)
 #pragma unroll
           for (int e = 0; e < 16; ++e) s[k][n][e] = fast_exp2(fmaf(s[k][n][e], p.scale_log2, -ref));
-          pr[n] = tile_t::pack(s[k][n]);
+          pr[n] = tile_t::template pack<PARTS>(s[k][n]);
           l[n] = tile_t::sum(pr[n], l[n]);
         }
-        tile_t::template col_product<NB>(o, stage + stream_t::TB + cs * DC * tile_t::ES, k0 + 32 * k, pr, lane);
+        tile_t::template col_product<NB, PARTS>(o, stage + stream_t::TB + cs * DC * tile_t::ES, k0 + 32 * k, pr, lane);
       }
     }
   }
@@ -340,8 +349,8 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
     for (int k = 0; k < BN / 32; ++k) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[k][0][e] = fast_exp2(fmaf(s[k][0][e], p.scale_log2, -lse)) * (dp[k][0][e] - delta);
-      const typename tile_t::operand ds = tile_t::pack(s[k][0]);
-      tile_t::template col_product<1>(&acc, stage + cs * DC * tile_t::ES, 32 * k, &ds, lane);
+      const auto ds = tile_t::template pack<attn_parts<T>(true)>(s[k][0]);
+      tile_t::template col_product<1, attn_parts<T>(true)>(&acc, stage + cs * DC * tile_t::ES, 32 * k, &ds, lane);
     }
   }
   if (row >= p.R) return;
@@ -351,7 +360,7 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
 
 // dk and dv: a wavefront owns 32 keys, their k and v rows in registers, and walks over the rows; q and do tiles in LDS serve both as rows
 // (scores) and, transposed, as the second products' first operand.
-template <typename T, int DP, int BQ, int WM>
+template <typename T, int DP, int BQ, int WM, int PARTS>
 __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kernel(attn_args p) {
   constexpr int CS = attn_cs(DP, sizeof(T) == 4), DC = DP / CS;
   typedef attn_tile<T, DC, DP> tile_t;
@@ -410,9 +419,10 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
           dp[0][0][4 * g + e] = pr * (dp[0][0][4 * g + e] - de[e]);
         }
       }
-      const typename tile_t::operand pr = tile_t::pack(s[0][0]), ds = tile_t::pack(dp[0][0]);
-      tile_t::template col_product<1>(&dv, gt + cs * DC * tile_t::ES, 32 * qq, &pr, lane);
-      tile_t::template col_product<1>(&dk, qt + cs * DC * tile_t::ES, 32 * qq, &ds, lane);
+      const auto pr = tile_t::template pack<PARTS>(s[0][0]);
+      const auto ds = tile_t::template pack<attn_parts<T>(true)>(dp[0][0]);
+      tile_t::template col_product<1, PARTS>(&dv, gt + cs * DC * tile_t::ES, 32 * qq, &pr, lane);
+      tile_t::template col_product<1, attn_parts<T>(true)>(&dk, qt + cs * DC * tile_t::ES, 32 * qq, &ds, lane);
     }
   }
   if (key >= p.Tk) return;
@@ -519,7 +529,7 @@ static int attn_splits(int64_t blocks, int units, int slots, double tile_us, dou
 }
 
 struct attn_plan {
-  int dp, few, nb, fwd_tiles, row_tiles, fwd_splits, dq_splits, key_tiles, dkv_splits;
+  int dp, slots, few, nb, fwd_tiles, row_tiles, fwd_splits, dq_splits, key_tiles, dkv_splits;
   size_t fwd_ws, bwd_ws;
 };
 
@@ -535,6 +545,7 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   const int bn = attn_bn(q.dp, f32);
   // 256 CUs; workgroups per CU by the registers and LDS of the kernels
   const int shared = q.dp == 256 || (q.dp == 128 && f32) ? 256 : q.dp == 128 || f32 ? 512 : 768;
+  q.slots = shared;
   const int wg = attn_rows_wg(q.dp, f32);
   q.few = R <= 32 && !(f32 && q.dp == 256);
   q.row_tiles = q.few ? 1 : (int)((R + wg - 1) / wg);
@@ -584,11 +595,12 @@ static int attn_fwd_launch(const attn_args& p, const attn_plan& q, ttdg_stream_t
   TTDG_LIMIT(grid < (1ll << 31), "attention_fwd: too many workgroups");
   if constexpr (!(F32 && DP == 256)) {
     constexpr int KW = attn_kw(DP, F32), ldsk = 2 * KW * attn_stream<T, DP, 32, 1>::STAGE;
-    if (q.few) ATTN_LAUNCH((attn_fwd_kernel<T, DP, 32, 1, 1, KW>), grid, 64 * KW, ldsk, stream, p);
+    if (q.few) ATTN_LAUNCH((attn_fwd_kernel<T, DP, 32, 1, 1, KW, attn_parts<T>(true)>), grid, 64 * KW, ldsk, stream, p);
   }
   if (q.few) {
-  } else if (q.nb == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 1, 1>), grid, 64 * WM, lds, stream, p);
-  else if constexpr (sizeof(T) == 2 && DP == 128) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 2, 1>), grid, 64 * WM, lds, stream, p);
+  } else if (q.nb == 1 && 2 * grid <= q.slots) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 1, 1, attn_parts<T>(true)>), grid, 64 * WM, lds, stream, p);
+  else if (q.nb == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 1, 1, 1>), grid, 64 * WM, lds, stream, p);
+  else if constexpr (sizeof(T) == 2 && DP == 128) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 2, 1, 1>), grid, 64 * WM, lds, stream, p);
   if (p.splits > 1) {
     const int64_t rows = (int64_t)p.B * p.Hk * p.R;
     if (p.splits > 32) ATTN_LAUNCH((attn_combine_kernel<T, 4>), rows, 256, 0, stream, p);
@@ -619,7 +631,8 @@ static int attn_bwd_launch(attn_args p, const attn_plan& q, ttdg_stream_t stream
   grid = (int64_t)p.B * p.Hk * p.key_tiles * p.splits;
   TTDG_LIMIT(grid < (1ll << 31), "attention_bwd: too many workgroups");
   constexpr int lds2 = 2 * attn_rows<T, DP, BN, WM>::STAGE + attn_exchange_bytes(DP, F32);
-  ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, WM>), grid, 64 * WM, lds2, stream, p);
+  if (2 * grid <= q.slots) ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, WM, attn_parts<T>(true)>), grid, 64 * WM, lds2, stream, p);
+  else ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, WM, 1>), grid, 64 * WM, lds2, stream, p);
   if (p.splits > 1) {
     hipLaunchKernelGGL(attn_reduce_kernel<T>, dim3((unsigned)((nk / 4 + 255) / 256), 2), dim3(256), 0, (hipStream_t)stream, p.part_o, 2 * nk, p.splits,
                        p.scale, (T*)p.dk, (T*)p.dv, nk);
