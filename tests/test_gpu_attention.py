@@ -576,6 +576,56 @@ def test_norm_rotation_and_attention_together(dev, dtype):
             assert e <= norm, (t, e)
 
 
+@gpu
+@pytest.mark.parametrize("num_heads,shared", [(4, False), (1, False), (8, True)])
+def test_multi_head_layer_over_another_set(dev, num_heads, shared):
+    """MultiHeadAttention.attend: projections, heads, attention over ragged states, output projection, residual, LayerNorm, with gradients of
+    every parameter, against the same layer in float64."""
+    from ttdg_mgm_amd.GModule.utils.attentions import MultiHeadAttention
+    torch.manual_seed(5)
+    m = MultiHeadAttention(256, num_heads).to(dev)
+    g = gen(31, dev)
+    x, st = normal(g, 3, 33, 256), normal(g, *((77, 256) if shared else (3, 77, 256)))
+    dout = normal(g, 3, 33, 256)
+    lens = torch.tensor([77, 20, 0], device=dev)
+    leaves = [x.clone().requires_grad_(), st.clone().requires_grad_()] + list(m.parameters())
+    out = m.attend(leaves[0], leaves[1], state_lens=lens)
+    grads = torch.autograd.grad(out, leaves, dout)
+
+    import copy
+    m64 = copy.deepcopy(m).double()
+    r = [x.double().requires_grad_(), st.double().requires_grad_()] + list(m64.parameters())
+    D = 256 // num_heads
+    q = m64.linear_q(r[0]).unflatten(-1, (num_heads, D)).transpose(1, 2)
+    k, v = (l(r[1]).unflatten(-1, (num_heads, D)).transpose(-3, -2) for l in (m64.linear_k, m64.linear_v))
+    hide = (torch.arange(77, device=dev)[None] >= lens[:, None])[:, None, None]
+    p = torch.softmax((q @ k.transpose(-1, -2) * D ** -0.5).masked_fill(hide, float("-inf")), -1).masked_fill(hide, 0.0)
+    ref = m64.layer_norm(r[0] + m64.linear_final((p @ v).transpose(1, 2).flatten(2)))
+    rg = torch.autograd.grad(ref, r, dout.double())
+    # float32 products of 256 terms feed products of 256 terms: 2 x 5 (2 sqrt(256) + sqrt(77) + sqrt(99) + 8 + 3 x 8) u of the sizes involved;
+    # linear_k's bias moves no softmax, its gradient is zero in exact arithmetic: the bound is taken on the size of the other bias gradients
+    tol = 10 * (2 * 16 + math.sqrt(77) + math.sqrt(99) + 32) * U
+    size = float(max(b.abs().max() for n, b in zip([n for n, _ in m.named_parameters()], rg[2:]) if n.endswith("bias")))
+    assert float((out.detach().double() - ref.detach()).abs().max()) <= tol * float(ref.detach().abs().max())
+    for n, a, b in zip(["x", "states"] + [n for n, _ in m.named_parameters()], grads, rg):
+        assert float((a.double() - b).abs().max()) <= tol * max(float(b.abs().max()), size if n.endswith("bias") else 0.0), n
+    with torch.no_grad():                      # the same without a tape, and a sample alone
+        assert torch.equal(m.attend(x, st, state_lens=lens), out.detach())
+        one = m.attend(x[1:2], st if shared else st[1:2, :20], state_lens=lens[1:2] if shared else None)
+        assert float((one - out.detach()[1:2]).abs().max()) <= tol * float(ref.detach().abs().max())
+
+
+def test_multi_head_layer_refuses():
+    from ttdg_mgm_amd.GModule.utils.attentions import MultiHeadAttention
+    m = MultiHeadAttention(256, 4)
+    x = torch.zeros(2, 3, 256)
+    for q, s in ((x[0], x), (x, x[:1]), (x[..., :128], x), (x, x[..., :128]), (x, x[0, 0])):
+        with pytest.raises(ValueError):
+            m.attend(q, s)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        m.attend(x, x)
+
+
 # ------------------------------------------------------------------------------------------- refusals (no GPU needed: nothing is launched)
 def _qkv(**kw):
     s = dict(B=2, Tq=3, Tk=5, H=4, Hk=2, D=64, dtype=F32)

@@ -4,7 +4,8 @@ Parameter names (linear_k/v/q/final, layer_norm) are the checkpoint contract.  T
 the attention map (multi_graph_matching.py:498), which comes from csrc/mha.hip without autograd; ``forward`` returns the
 (output, attention) pair and is differentiable when gradients are enabled (the source-training loss U_sup.forward
 back-propagates through ``output``, multi_graph_matching.py:100-106): the four projections run on the MFMA GEMM
-(ops.LinearFn), softmax / LayerNorm are torch glue."""
+(ops.LinearFn), softmax / LayerNorm are torch glue.  ``attend`` is the layer's output alone, for any number of heads and for batches whose
+queries and states are different sets (the reference's forward(key_value_query) with key = value != query)."""
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -42,6 +43,28 @@ class MultiHeadAttention(nn.Module):
             scale = (k.shape[-1] // self.num_heads) ** -0.5            # attentions.py:80
             a = ops.mha_adjacency(q, k, ops.graphs([n]), [n], scale, p, sd, zero_diag=False).view(n, n)
             return a
+
+    def attend(self, query, states, state_lens=None, state_mask=None):
+        """layer_norm(query + dropout(linear_final(heads of softmax(q k^T / sqrt(dim_per_head)) v))) without the attention map
+        (csrc/attention.hip keeps no map): query (B, n, model_dim), states (B, m, model_dim) or (m, model_dim) for all samples; the states
+        j < state_lens[b] with state_mask[b, j] exist (ops.cross_attention).  Dropout acts on the output only, not on the map."""
+        if query.dim() != 3 or states.dim() not in (2, 3) or query.shape[2] != self.linear_q.in_features or states.shape[-1] != query.shape[2]:
+            raise ValueError("attend: query (B, n, %d) and states (B, m, %d) or (m, %d), got %s and %s" %
+                             (self.linear_q.in_features, self.linear_k.in_features, self.linear_k.in_features, tuple(query.shape), tuple(states.shape)))
+        B, H, D = query.shape[0], self.num_heads, self.dim_per_head
+        if states.dim() == 3 and states.shape[0] != B:
+            raise ValueError("attend: %d samples of queries, %d of states" % (B, states.shape[0]))
+
+        def lin(x, layer):
+            y = ops.LinearFn.apply(x.float().reshape(-1, x.shape[-1]).contiguous(), layer.weight, layer.bias)
+            return y.view(*x.shape[:-1], layer.out_features)
+
+        def heads(x):
+            return x.unflatten(-1, (H, D)) if x.dim() == 3 else x.unflatten(-1, (H, D)).unsqueeze(0).expand(B, -1, -1, -1)
+
+        out = ops.cross_attention(heads(lin(query, self.linear_q)), heads(lin(states, self.linear_k)), heads(lin(states, self.linear_v)),
+                                  k_lens=state_lens, key_mask=state_mask)
+        return self.layer_norm(query + self.dropout(lin(out.flatten(2), self.linear_final)))
 
     def forward(self, key_value_query, attn_mask=None):
         key, value, query = key_value_query
