@@ -62,38 +62,29 @@ class DiskDataset(torch.utils.data.Dataset):
 
 
 class _Ring:
-    """A ring of batch slots in SHARED memory, page-locked for the GPU: worker processes write a decoded batch straight into
-    its slot, the main process starts the DMA from there - no per-batch shared-memory segment, no staging memcpy (measured on
-    the GPU box: 2.4 ms memcpy + 2.1 ms upload call per 3 MB tensor through a staging buffer; ~10 ms per batch of host time).
+    """A ring of batch slots in SHARED memory: worker processes write a decoded batch straight into its slot - no per-batch
+    shared-memory segment.  For the GPU every slot has a page-locked twin of the main process (allocated as such: registering the
+    shared memory itself is refused on some hosts): ``expand`` copies an arrived slot there once and the DMA starts from it.
     Allocated before the workers are forked, so they inherit the mapping.  Slot s is handed to a worker again only after the
-    copy that read it has completed (``wait``)."""
+    upload that read its twin has completed (``wait``)."""
 
     def __init__(self, slots, batch, image_shape, masks_per_image, mask_shape, register):
         self.slots, self.batch, self.mpi = slots, batch, masks_per_image
         self.images = torch.empty((slots, batch) + tuple(image_shape), dtype=torch.uint8).share_memory_()
         self.masks = torch.empty((slots, batch * max(1, masks_per_image)) + tuple(mask_shape), dtype=torch.bool).share_memory_()
         self.events = [None] * slots
-        self.pinned = False
-        if register and torch.cuda.is_available():
-            rt = torch.cuda.cudart()
-            done = []
-            for t in (self.images, self.masks):
-                if int(rt.cudaHostRegister(t.data_ptr(), t.numel() * t.element_size(), 0)) != 0:
-                    for u in done:               # all or nothing: a half-registered ring would leak the first registration
-                        rt.cudaHostUnregister(u.data_ptr())
-                    done = None
-                    break
-                done.append(t)
-            self.pinned = done is not None
+        self.pinned = bool(register and torch.cuda.is_available())
+        if self.pinned:
+            self.pin_images = torch.empty(self.images.shape, dtype=self.images.dtype, pin_memory=True)
+            self.pin_masks = torch.empty(self.masks.shape, dtype=self.masks.dtype, pin_memory=True)
 
-    def __del__(self):
-        if getattr(self, "pinned", False):
-            try:
-                rt = torch.cuda.cudart()
-                for t in (self.images, self.masks):
-                    rt.cudaHostUnregister(t.data_ptr())
-            except Exception:          # interpreter shutdown: the driver releases the registration with the process
-                pass
+    def batch_views(self, slot, nb):
+        """Images and masks (None without any) of the ``nb`` items that have arrived in a slot."""
+        images, masks = self.images[slot, :nb], self.masks[slot, :nb * self.mpi] if self.mpi else None
+        if self.pinned:
+            images = self.pin_images[slot, :nb].copy_(images)
+            masks = None if masks is None else self.pin_masks[slot, :nb * self.mpi].copy_(masks)
+        return images, masks
 
     def wait(self, slot):
         if self.events[slot] is not None:
@@ -167,8 +158,7 @@ def expand(batch, ring=None):
         return batch["items"]
     if batch.get("slot") is not None and batch["images"] is None:
         nb = len(batch["meta"])
-        batch["images"] = ring.images[batch["slot"], :nb]
-        batch["masks"] = ring.masks[batch["slot"], :nb * ring.mpi] if ring.mpi else None
+        batch["images"], batch["masks"] = ring.batch_views(batch["slot"], nb)
     out, k = [], 0
     for i, m in enumerate(batch["meta"]):
         anns = []
@@ -188,7 +178,7 @@ def expand(batch, ring=None):
 class DiskStream:
     """Persistent worker processes over a DiskDataset; ``epoch(lo, hi)`` iterates collated batches (``_collate``): pass them to
     ``expand(batch, stream.ring)`` for the list of dataset dicts; ``images`` / ``masks`` are then the stacked tensors (None for
-    ragged batches).  ``ring=True``: batches of the dataset's common shape travel through a shared page-locked ring."""
+    ragged batches).  ``ring=True``: batches of the dataset's common shape travel through a shared ring."""
 
     def __init__(self, root, n, batch, workers=4, prefetch=2, ring=False, register=True):
         self.ring = None
