@@ -7,6 +7,7 @@ a non-zero status raises.
 """
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -105,6 +106,12 @@ class QkNormRope(C.Structure):
                [("eps", C.c_float), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
 
 
+# The same two structs for struct.pack: these descriptors are made on every call, a third of the time of filling ctypes fields (and of half
+# of a small call's host time when autograd's thread does it).  Pointers are integers, 0 = NULL.
+ATTENTION = struct.Struct("@3Q 9q 2Q 2q 7if 7Q 2Q")
+QK_NORM_ROPE = struct.Struct("@" + 2 * "Q 3q 2i 2Q 3q 4Q " + "Q 7if 2Q")
+assert ATTENTION.size == C.sizeof(Attention) and QK_NORM_ROPE.size == C.sizeof(QkNormRope)
+
 F32, BF16 = 0, 1          # TTDG_F32, TTDG_BF16
 GEMM_GROUP_MAX = 8
 ROW_SCALE_MAX = 64
@@ -132,13 +139,13 @@ SIGNATURES = {
     "ttdg_sinkhorn_batched_fwd": (C.c_int, [_P, _L, _L, _L, _I, _I, _I, _P, _P, _I, _F, _I, _P, _P, _S]),
     "ttdg_sinkhorn_batched_bwd": (C.c_int, [_P, _L, _L, _L, _I, _I, _I, _P, _P, _I, _F, _I, _P, _P, _P, _S]),
     "ttdg_mha_adjacency": (C.c_int, [_P, _P, _I, Graphs, _F, _F, C.c_uint64, _I, _P, _S]),
-    "ttdg_attention_fwd_workspace_bytes": (C.c_size_t, [C.POINTER(Attention)]),
-    "ttdg_attention_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(Attention)]),
-    "ttdg_attention_fwd": (C.c_int, [C.POINTER(Attention), _S]),
-    "ttdg_attention_bwd": (C.c_int, [C.POINTER(Attention), _S]),
-    "ttdg_qk_norm_rope_fwd": (C.c_int, [C.POINTER(QkNormRope), _S]),
-    "ttdg_qk_norm_rope_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(QkNormRope)]),
-    "ttdg_qk_norm_rope_bwd": (C.c_int, [C.POINTER(QkNormRope), _S]),
+    "ttdg_attention_fwd_workspace_bytes": (C.c_size_t, [_P]),      # (Attention / QkNormRope by reference, or their packed bytes)
+    "ttdg_attention_bwd_workspace_bytes": (C.c_size_t, [_P]),
+    "ttdg_attention_fwd": (C.c_int, [_P, _S]),
+    "ttdg_attention_bwd": (C.c_int, [_P, _S]),
+    "ttdg_qk_norm_rope_fwd": (C.c_int, [_P, _S]),
+    "ttdg_qk_norm_rope_bwd_workspace_bytes": (C.c_size_t, [_P]),
+    "ttdg_qk_norm_rope_bwd": (C.c_int, [_P, _S]),
     "ttdg_gagm_workspace_bytes": (C.c_size_t, [_I]),
     "ttdg_gagm_solve": (C.c_int, [_P, _P, _P, Graphs, GagmCfg, _P, _P, _P, _S]),
     "ttdg_lap_batched": (C.c_int, [_P, _I, _I, _I, _P, _S]),

@@ -430,13 +430,25 @@ def _on_device_of(t):
     return _NO_DEVICE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
-def _timed_call(name, arg, timer, meta):
-    """call(name, byref(arg), stream()), stamped when bench.py asks for it (the usual case stays free of the context manager)."""
+def _packed_call(name, packer, fields, ws_query, device, meta):
+    """call(name, descriptor, stream()) with a workspace of the size ``ws_query`` asks for; stamped when bench.py asks for it (the usual case
+    stays free of the context manager).  The workspace may go back to the allocator once the call is enqueued, as any temporary."""
+    desc = packer.pack(*fields, 0, 0)
+    ws = None
+    if ws_query is not None:
+        n = ws_query(desc)
+        if n:
+            ws = torch.empty(n, device=device, dtype=torch.uint8)
+            desc = packer.pack(*fields, ws.data_ptr(), n)
     if KERNEL_TIMERS is None:
-        call(name, C.byref(arg), stream())
+        call(name, desc, stream())
     else:
-        with _timed(timer, meta):
-            call(name, C.byref(arg), stream())
+        with _timed(name[5:], meta):
+            call(name, desc, stream())
+
+
+def _at(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _like(t):
@@ -482,26 +494,17 @@ def _attn_check(q, k, v, k_lens, key_mask):
         ptr(q)                          # raises: no CPU fallback
 
 
-def _attn_desc(q, k, v, scale, k_lens, key_mask, out=None, out_lo=None, lse=None, dout=None, dq=None, dk=None, dv=None):
-    """ttdg_attention_t without a workspace (positional: the field order of the struct)."""
+def _attn_fields(q, k, v, scale, k_lens, key_mask, out, out_lo, lse, dout=None, dq=None, dk=None, dv=None):
+    """the fields of ttdg_attention_t before the workspace, in their order"""
     B, Tq, H, D = q.shape
     qb, qt, qh, _ = q.stride()
     kb, kt, kh, _ = k.stride()
     vb, vt, vh, _ = v.stride()
-    mask, mb, mt = None, 0, 0
+    mask, mb, mt = 0, 0, 0
     if key_mask is not None:
         mask, mb, mt = key_mask.data_ptr(), (0 if key_mask.shape[0] == 1 else key_mask.stride(0)), key_mask.stride(1)
-    return _lib.Attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), qb, qt, qh, kb, kt, kh, vb, vt, vh, None if k_lens is None else k_lens.data_ptr(),
-                          mask, mb, mt, B, Tq, k.shape[1], H, k.shape[2], D, _ATTN_DTYPES[q.dtype], scale, ptr(out), ptr(out_lo), ptr(lse), ptr(dout),
-                          ptr(dq), ptr(dk), ptr(dv))
-
-
-def _attn_workspace(a, nbytes, device):
-    if nbytes == 0:
-        return None
-    ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
-    a.ws, a.ws_bytes = ws.data_ptr(), nbytes
-    return ws
+    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), qb, qt, qh, kb, kt, kh, vb, vt, vh, _at(k_lens), mask, mb, mt, B, Tq, k.shape[1], H, k.shape[2], D,
+            _ATTN_DTYPES[q.dtype], scale, out.data_ptr(), _at(out_lo), _at(lse), _at(dout), _at(dq), _at(dk), _at(dv))
 
 
 def _attn_forward(q, k, v, scale, k_lens, key_mask, keep):
@@ -513,9 +516,8 @@ def _attn_forward(q, k, v, scale, k_lens, key_mask, keep):
     if keep:
         lse = torch.empty(q.shape[0] * q.shape[1] * q.shape[2], device=q.device, dtype=torch.float32)
         lo = None if q.dtype == torch.float32 else _like(q)
-    a = _attn_desc(q, k, v, scale, k_lens, key_mask, out, lo, lse)
-    ws = _attn_workspace(a, _lib.load().ttdg_attention_fwd_workspace_bytes(C.byref(a)), q.device)    # noqa: F841 (alive until enqueued)
-    _timed_call("ttdg_attention_fwd", a, "attention_fwd", q.shape + k.shape[1:3])
+    _packed_call("ttdg_attention_fwd", _lib.ATTENTION, _attn_fields(q, k, v, scale, k_lens, key_mask, out, lo, lse),
+                 _lib.load().ttdg_attention_fwd_workspace_bytes, q.device, q.shape + k.shape[1:3])
     return out, lo, lse
 
 
@@ -546,9 +548,8 @@ class CrossAttentionFn(torch.autograd.Function):
             dq = _like(q)
             dk, dv = (_like(k), _like(k)) if kv else (None, None)
             dout = _dense_grad(dout)
-            a = _attn_desc(q, k, v, ctx.scale, k_lens, key_mask, out, lo, lse, dout, dq, dk, dv)
-            ws = _attn_workspace(a, _lib.load().ttdg_attention_bwd_workspace_bytes(C.byref(a)), q.device)    # noqa: F841
-            _timed_call("ttdg_attention_bwd", a, "attention_bwd", q.shape + k.shape[1:3])
+            _packed_call("ttdg_attention_bwd", _lib.ATTENTION, _attn_fields(q, k, v, ctx.scale, k_lens, key_mask, out, lo, lse, dout, dq, dk, dv),
+                         _lib.load().ttdg_attention_bwd_workspace_bytes, q.device, q.shape + k.shape[1:3])
         return dq, dk, dv, None, None, None
 
 
@@ -585,68 +586,77 @@ def rope_frequencies(rot_dim, base=10000.0, axes=1, device=None):
     return f.repeat(axes)
 
 
+def _qkn_check_side(name, x, w, pos, q, R, dims):
+    if x.dim() != 4:
+        raise ValueError("qk_norm_rope: %s must be (batch, positions, heads, channels), got %s" % (name, tuple(x.shape)))
+    B, T, _, D = x.shape
+    dev = q.device
+    if x is not q:
+        if x.dtype != q.dtype:
+            raise TypeError("qk_norm_rope: float32 or bfloat16 tensors of one type, got %s and %s" % (q.dtype, x.dtype))
+        if x.device != dev or B != q.shape[0] or D != q.shape[3]:
+            raise ValueError("qk_norm_rope: q %s and k %s do not belong together" % (tuple(q.shape), tuple(x.shape)))
+    if w is None or w.dtype != torch.float32 or w.dim() != 1 or w.shape[0] != D or w.device != dev:
+        raise TypeError("qk_norm_rope: the weight of %s must be float32 (%d,) on %s" % (name, D, dev))
+    if dims:
+        if pos is None or pos.dtype not in (torch.int64, torch.int32):
+            raise TypeError("qk_norm_rope: positions must be int32 or int64, the same for queries and keys")
+        ps = pos.shape
+        if len(ps) != dims or ps[1] != T or ps[0] not in (1, B) or (dims == 3 and ps[2] != 2) or pos.device != dev:
+            raise ValueError("qk_norm_rope: positions of %s must be (%d or 1, %d) or (.., .., 2) on %s, got %s" % (name, B, T, dev, tuple(ps)))
+
+
 def _qkn_check(q, k, q_weight, k_weight, freq, q_pos, k_pos):
-    R = 0 if freq is None else 2 * freq.numel()
-    axes = 1
+    """-> number of position axes"""
+    if q.dtype not in _ATTN_DTYPES:
+        raise TypeError("qk_norm_rope: float32 or bfloat16 tensors of one type, got %s" % q.dtype)
+    R = dims = 0
     if freq is not None:
         if freq.dtype != torch.float64 or freq.dim() != 1 or freq.device != q.device:
             raise TypeError("qk_norm_rope: frequencies must be a float64 vector on %s" % q.device)
         if q_pos is None:
             raise ValueError("qk_norm_rope: a rotation needs positions")
-        axes = 1 if q_pos.dim() == 2 else 2
-    for name, x, w, pos in (("q", q, q_weight, q_pos), ("k", k, k_weight, k_pos)):
-        if x is None:
-            if w is not None or (pos is not None and name == "k" and pos is not q_pos):
-                raise ValueError("qk_norm_rope: a weight or positions for keys, but no keys")
-            continue
-        if x.dim() != 4:
-            raise ValueError("qk_norm_rope: %s must be (batch, positions, heads, channels), got %s" % (name, tuple(x.shape)))
-        if x.dtype != q.dtype or q.dtype not in _ATTN_DTYPES:
-            raise TypeError("qk_norm_rope: float32 or bfloat16 tensors of one type, got %s and %s" % (q.dtype, x.dtype))
-        if x.device != q.device or x.shape[0] != q.shape[0] or x.shape[3] != q.shape[3]:
-            raise ValueError("qk_norm_rope: q %s and k %s do not belong together" % (tuple(q.shape), tuple(x.shape)))
-        D = x.shape[3]
-        if D % 8 or not 8 <= D <= 256 or R > D or R % 8:
-            raise ValueError("qk_norm_rope: %d channels per head, %d of them rotated; multiples of 8 up to 256 are supported" % (D, R))
-        if w is None or w.dtype != torch.float32 or tuple(w.shape) != (D,) or w.device != q.device:
-            raise TypeError("qk_norm_rope: the weight of %s must be float32 (%d,) on %s" % (name, D, q.device))
-        if freq is None:
-            continue
-        if pos is None or pos.dtype not in (torch.int32, torch.int64) or pos.dtype != q_pos.dtype:
+        R, dims = 2 * freq.shape[0], 3 if q_pos.dim() == 3 else 2
+    _qkn_check_side("q", q, q_weight, q_pos, q, R, dims)
+    D = q.shape[3]
+    if D % 8 or not 8 <= D <= 256 or R > D or R % 8:
+        raise ValueError("qk_norm_rope: %d channels per head, %d of them rotated; multiples of 8 up to 256 are supported" % (D, R))
+    if k is not None:
+        _qkn_check_side("k", k, k_weight, k_pos, q, R, dims)
+        if dims and k_pos.dtype != q_pos.dtype:
             raise TypeError("qk_norm_rope: positions must be int32 or int64, the same for queries and keys")
-        if pos.dim() != q_pos.dim() or pos.dim() not in (2, 3) or pos.shape[0] not in (1, x.shape[0]) or pos.shape[1] != x.shape[1] or \
-                (pos.dim() == 3 and pos.shape[2] != 2) or pos.device != q.device:
-            raise ValueError("qk_norm_rope: positions of %s must be (%d or 1, %d) or (.., .., 2) on %s, got %s" %
-                             (name, x.shape[0], x.shape[1], q.device, tuple(pos.shape)))
-    ptr(q)                              # (refuses CPU tensors)
-    return axes
+    elif k_weight is not None or k_pos is not None:
+        raise ValueError("qk_norm_rope: a weight or positions for keys, but no keys")
+    if not q.is_cuda:
+        ptr(q)                          # raises: no CPU fallback
+    return 1 if dims < 3 else 2
 
 
 def _qkn_side(x, w, pos, y, dy, dx, dw):
-    """ttdg_norm_rope_side_t (positional)"""
+    """the fields of ttdg_norm_rope_side_t"""
     if x is None:
-        return _lib.NormRopeSide()
+        return (0,) * 15
     _, T, H, _ = x.shape
     sb, st, sh, _ = x.stride()
-    at, pb, pt, pa = None, 0, 0, 0
+    at = pb = pt = pa = 0
     if pos is not None:
         at, pb, pt = pos.data_ptr(), (0 if pos.shape[0] == 1 else pos.stride(0)), pos.stride(1)
         pa = pos.stride(2) if pos.dim() == 3 else 0
-    return _lib.NormRopeSide(x.data_ptr(), sb, st, sh, T, H, w.data_ptr(), at, pb, pt, pa, ptr(y), ptr(dy), ptr(dx), ptr(dw))
+    return (x.data_ptr(), sb, st, sh, T, H, w.data_ptr(), at, pb, pt, pa, _at(y), _at(dy), _at(dx), _at(dw))
 
 
-def _qkn_desc(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, eps, interleaved, outs=(None, None), grads=(None,) * 6):
-    """ttdg_qk_norm_rope_t without a workspace; grads: dy, dx, dw of the queries, then of the keys"""
-    R, at, wide = (0, None, 0) if freq is None else (2 * freq.numel(), freq.data_ptr(), int(q_pos.dtype == torch.int64))
-    return _lib.QkNormRope(_qkn_side(q, q_weight, q_pos, outs[0], *grads[:3]), _qkn_side(k, k_weight, k_pos, outs[1], *grads[3:]), at, q.shape[0],
-                           q.shape[3], R, axes, interleaved, wide, _ATTN_DTYPES[q.dtype], eps)
+def _qkn_fields(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, eps, interleaved, outs=(None, None), grads=(None,) * 6):
+    """the fields of ttdg_qk_norm_rope_t before the workspace; grads: dy, dx, dw of the queries, then of the keys"""
+    R, at, wide = (0, 0, 0) if freq is None else (2 * freq.numel(), freq.data_ptr(), int(q_pos.dtype == torch.int64))
+    return _qkn_side(q, q_weight, q_pos, outs[0], *grads[:3]) + _qkn_side(k, k_weight, k_pos, outs[1], *grads[3:]) + \
+        (at, q.shape[0], q.shape[3], R, axes, interleaved, wide, _ATTN_DTYPES[q.dtype], eps)
 
 
 def _qkn_forward(q, k, *args):
     yq = _like(q)
     yk = None if k is None else _like(k)
-    a = _qkn_desc(q, k, *args, outs=(yq, yk))
-    _timed_call("ttdg_qk_norm_rope_fwd", a, "qk_norm_rope_fwd", 2 * (yq.numel() + (0 if yk is None else yk.numel())) * yq.element_size())   # algorithmic bytes
+    _packed_call("ttdg_qk_norm_rope_fwd", _lib.QK_NORM_ROPE, _qkn_fields(q, k, *args, outs=(yq, yk)), None, q.device,
+                 2 * (yq.numel() + (0 if yk is None else yk.numel())) * yq.element_size())          # algorithmic bytes
     return yq, yk
 
 
@@ -672,9 +682,8 @@ class QkNormRopeFn(torch.autograd.Function):
             if k is not None:
                 gk = _dense_grad(gk) if gk is not None else torch.zeros(k.shape, device=k.device, dtype=k.dtype)
                 dk, dwk = _like(k), _like(k_weight)
-            a = _qkn_desc(q, k, q_weight, k_weight, freq, q_pos, k_pos, *ctx.args, grads=(gq, dq, dwq, gk, dk, dwk))
-            ws = _attn_workspace(a, _lib.load().ttdg_qk_norm_rope_bwd_workspace_bytes(C.byref(a)), q.device)      # noqa: F841
-            _timed_call("ttdg_qk_norm_rope_bwd", a, "qk_norm_rope_bwd", 3 * (q.numel() + (0 if k is None else k.numel())) * q.element_size())
+            _packed_call("ttdg_qk_norm_rope_bwd", _lib.QK_NORM_ROPE, _qkn_fields(q, k, q_weight, k_weight, freq, q_pos, k_pos, *ctx.args, grads=(gq, dq, dwq, gk, dk, dwk)),
+                         _lib.load().ttdg_qk_norm_rope_bwd_workspace_bytes, q.device, 3 * (q.numel() + (0 if k is None else k.numel())) * q.element_size())
         return dq, dk, dwq, dwk, None, None, None, None, None, None
 
 
