@@ -306,6 +306,21 @@ def test_attention_gradients_of_some_inputs_only(dev):
 
 
 @gpu
+def test_second_derivatives_are_refused(dev):
+    """A recorded backward (create_graph) gives the same first derivatives; differentiating it raises instead of taking them for constants."""
+    from ttdg_mgm_amd import ops
+    g = gen(41, dev)
+    q, k, v = (normal(g, 1, 5, 2, 64).requires_grad_() for _ in range(3))
+    w = torch.ones(64, device=dev, requires_grad=True)
+    for f, ins in ((lambda: ops.cross_attention(q, k, v), (q, k, v)), (lambda: ops.qk_norm_rope(q, None, w, None)[0], (q, w))):
+        plain = torch.autograd.grad(f().pow(2).sum(), ins)
+        rec = torch.autograd.grad(f().pow(2).sum(), ins, create_graph=True)
+        assert all(torch.equal(a, b.detach()) for a, b in zip(plain, rec))
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(rec[0].sum(), ins[0])
+
+
+@gpu
 def test_attention_on_another_stream_and_in_a_graph(dev):
     """A side stream, and forward + backward captured once and replayed on new values with eager work in between: equal to eager each time."""
     from ttdg_mgm_amd import ops

@@ -521,6 +521,16 @@ def _attn_forward(q, k, v, scale, k_lens, key_mask, keep):
     return out, lo, lse
 
 
+def _first_order(backward):
+    """A backward without derivatives of its own.  once_differentiable, whose wrapper costs 6 us, is only needed where somebody records the
+    backward (create_graph); differentiating that record raises."""
+    recorded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 def _dense_grad(g):
     g = g.contiguous()
     return g.clone() if g.data_ptr() & 15 else g
@@ -538,7 +548,7 @@ class CrossAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dout):
         q, k, v, out, lo, lse, k_lens, key_mask = ctx.saved_tensors
         kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
@@ -672,7 +682,7 @@ class QkNormRopeFn(torch.autograd.Function):
             return _qkn_forward(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, eps, interleaved)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, freq, q_pos, k_pos = ctx.saved_tensors
         dq = dk = dwq = dwk = None
