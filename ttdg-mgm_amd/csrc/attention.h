@@ -11,6 +11,7 @@ typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) float f32x8;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 
 struct attn_args {
   const void *q, *k, *v;
@@ -25,15 +26,16 @@ struct attn_args {
   float* lse;                                                       // (problem, row): log2 of the row's sum of exponentials
   const void* dout;
   void *dq, *dk, *dv;
-  float *delta, *part_o, *part_lse;
+  float *delta, *part_o, *part_lse;                                 // delta: minus do . o of every row
 };
 
-__device__ __forceinline__ f32x16 f32x16_zero() {
+__device__ __forceinline__ f32x16 f32x16_all(float x) {
   f32x16 z;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) z[e] = 0.f;
+  for (int e = 0; e < 16; ++e) z[e] = x;
   return z;
 }
+__device__ __forceinline__ f32x16 f32x16_zero() { return f32x16_all(0.f); }
 
 // register e of a 32 x 32 accumulator holds tile row attn_reg_row(e) + 4 (lane >> 5), tile column lane & 31
 __device__ __forceinline__ constexpr int attn_reg_row(int e) { return (e & 3) + 8 * (e >> 2); }
@@ -217,7 +219,16 @@ struct attn_tile {
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = p[8 * kg + e];
         r.x[0][kg] = __builtin_convertvector(y, bf16x8);
-        if constexpr (PARTS == 2) r.x[1][kg] = __builtin_convertvector(y - __builtin_convertvector(r.x[0][kg], f32x8), bf16x8);
+        if constexpr (PARTS == 2) {
+          // (widened as bits: by conversion the compiler would round every value a second time)
+          const u32x4 u = __builtin_bit_cast(u32x4, r.x[0][kg]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[2 * e] -= __uint_as_float(u[e] << 16);
+            y[2 * e + 1] -= __uint_as_float(u[e] & 0xffff0000u);
+          }
+          r.x[1][kg] = __builtin_convertvector(y, bf16x8);
+        }
       }
     }
     return r;

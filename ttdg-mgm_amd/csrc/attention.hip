@@ -305,9 +305,10 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
     __syncthreads();
   }
   float lse = p.lse[(int64_t)prob * p.R + rw.row];
-  if (split == 0 && h == 0 && cs == 0 && row < p.R) p.delta[(int64_t)prob * p.R + row] = delta;
+  if (split == 0 && h == 0 && cs == 0 && row < p.R) p.delta[(int64_t)prob * p.R + row] = -delta;
   if (lse == -INFINITY) lse = INFINITY;       // a row without any key: p = 0
 
+  const f32x16 start = f32x16_all(cs == 0 ? -delta : 0.f);      // the products v . do start from minus delta: no subtraction per score
   f32x16 acc[DC / 32];
 #pragma unroll
   for (int d = 0; d < DC / 32; ++d) acc[d] = f32x16_zero();
@@ -337,7 +338,7 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
 #pragma unroll
     for (int k = 0; k < BN / 32; ++k) {
       s[k][0] = stream_t::start(stage, 32 * k, live, h);
-      dp[k][0] = f32x16_zero();
+      dp[k][0] = start;
     }
     tile_t::template row_product<BN / 32, 1, PRE>(s, stage + cs * DC * tile_t::ES, 0, &qf, l32, h);
     tile_t::template row_product<BN / 32, 1, PRE>(dp, stage + stream_t::TB + cs * DC * tile_t::ES, 0, &gf, l32, h);
@@ -348,7 +349,7 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
 #pragma unroll
     for (int k = 0; k < BN / 32; ++k) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[k][0][e] = fast_exp2(fmaf(s[k][0][e], p.scale_log2, -lse)) * (dp[k][0][e] - delta);
+      for (int e = 0; e < 16; ++e) s[k][0][e] = fast_exp2(fmaf(s[k][0][e], p.scale_log2, -lse)) * dp[k][0][e];
       const auto ds = tile_t::template pack<attn_parts<T>(true)>(s[k][0]);
       tile_t::template col_product<1, attn_parts<T>(true)>(&acc, stage + cs * DC * tile_t::ES, 32 * k, &ds, lane);
     }
@@ -401,22 +402,30 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
 #pragma unroll 1
     for (int qq = 0; qq < BQ / 32; ++qq) {
       constexpr int PRE = DP == 256 && sizeof(T) == 2 ? 4 : 0;
+      const float* st = (const float*)(qt + 2 * rows_t::TB) + 32 * qq + 4 * h;
       f32x16 s[1][1] = {{f32x16_zero()}}, dp[1][1] = {{f32x16_zero()}};
+      if (cs == 0) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 de = *(const f32x4*)(st + 64 + 8 * g);                // the products v . do start from minus delta
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dp[0][0][4 * g + e] = de[e];
+        }
+      }
       tile_t::template row_product<1, 1, PRE>(s, qt + cs * DC * tile_t::ES, 32 * qq, &kf, l32, h);
       tile_t::template row_product<1, 1, PRE>(dp, gt + cs * DC * tile_t::ES, 32 * qq, &vf, l32, h);
       if constexpr (CS > 1) {
         attn_exchange(s[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
         attn_exchange(dp[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
       }
-      const float* st = (const float*)(qt + 2 * rows_t::TB) + 32 * qq + 4 * h;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const f32x4 ls = *(const f32x4*)(st + 8 * g), de = *(const f32x4*)(st + 64 + 8 * g);
+        const f32x4 ls = *(const f32x4*)(st + 8 * g);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float pr = fast_exp2(fmaf(s[0][0][4 * g + e], p.scale_log2, -ls[e]));
           s[0][0][4 * g + e] = pr;
-          dp[0][0][4 * g + e] = pr * (dp[0][0][4 * g + e] - de[e]);
+          dp[0][0][4 * g + e] *= pr;
         }
       }
       const auto pr = tile_t::template pack<PARTS>(s[0][0]);
