@@ -334,24 +334,30 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
     }
     if (live == 0) continue;
     constexpr int PRE = DP == 256 && sizeof(T) == 2 ? 2 : 0;      // one wavefront per SIMD: nobody else hides the LDS
-    f32x16 s[BN / 32][1], dp[BN / 32][1];
+    // blocks of 32 keys at a time: two chains of products with 128 channels; one with 64, where two cost the third wavefront per SIMD its
+    // registers (323 and 296 us)
+    constexpr int KK = DP == 64 && sizeof(T) == 2 ? 1 : BN / 32;
 #pragma unroll
-    for (int k = 0; k < BN / 32; ++k) {
-      s[k][0] = stream_t::start(stage, 32 * k, live, h);
-      dp[k][0] = start;
-    }
-    tile_t::template row_product<BN / 32, 1, PRE>(s, stage + cs * DC * tile_t::ES, 0, &qf, l32, h);
-    tile_t::template row_product<BN / 32, 1, PRE>(dp, stage + stream_t::TB + cs * DC * tile_t::ES, 0, &gf, l32, h);
-    if constexpr (CS > 1) {
-      attn_exchange(s[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
-      attn_exchange(dp[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
-    }
+    for (int k0 = 0; k0 < BN; k0 += 32 * KK) {
+      f32x16 s[KK][1], dp[KK][1];
 #pragma unroll
-    for (int k = 0; k < BN / 32; ++k) {
+      for (int k = 0; k < KK; ++k) {
+        s[k][0] = stream_t::start(stage, k0 + 32 * k, live, h);
+        dp[k][0] = start;
+      }
+      tile_t::template row_product<KK, 1, PRE>(s, stage + cs * DC * tile_t::ES, k0, &qf, l32, h);
+      tile_t::template row_product<KK, 1, PRE>(dp, stage + stream_t::TB + cs * DC * tile_t::ES, k0, &gf, l32, h);
+      if constexpr (CS > 1) {
+        attn_exchange(s[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
+        attn_exchange(dp[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
+      }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[k][0][e] = fast_exp2(fmaf(s[k][0][e], p.scale_log2, -lse)) * dp[k][0][e];
-      const auto ds = tile_t::template pack<attn_parts<T>(true)>(s[k][0]);
-      tile_t::template col_product<1, attn_parts<T>(true)>(&acc, stage + cs * DC * tile_t::ES, 32 * k, &ds, lane);
+      for (int k = 0; k < KK; ++k) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[k][0][e] = fast_exp2(fmaf(s[k][0][e], p.scale_log2, -lse)) * dp[k][0][e];
+        const auto ds = tile_t::template pack<attn_parts<T>(true)>(s[k][0]);
+        tile_t::template col_product<1, attn_parts<T>(true)>(&acc, stage + cs * DC * tile_t::ES, k0 + 32 * k, &ds, lane);
+      }
     }
   }
   if (row >= p.R) return;
