@@ -314,14 +314,19 @@ struct attn_tile {
 };
 
 // Two wavefronts that hold sums over half the channels each add them: `own` and `other` are their 4 KiB of LDS.  Every wavefront of the
-// workgroup takes part in the barriers.
+// workgroup takes part in the barriers; the one behind the reads is left out (LAST) where another follows before the next exchange.
+template <bool LAST>
 __device__ __forceinline__ void attn_exchange(f32x16& x, float* own, const float* other, int lane) {
 #pragma unroll
-  for (int e = 0; e < 16; ++e) own[e * 64 + lane] = x[e];
+  for (int g = 0; g < 4; ++g) ((f32x4*)own)[g * 64 + lane] = f32x4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
   __syncthreads();
 #pragma unroll
-  for (int e = 0; e < 16; ++e) x[e] += other[e * 64 + lane];
-  __syncthreads();
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 y = ((const f32x4*)other)[g * 64 + lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[4 * g + e] += y[e];
+  }
+  if (!LAST) __syncthreads();
 }
 
 // LDS-DMA of ROWS tile rows: instruction i of a wavefront fills 1 KiB; its lanes' offsets repeat every PER instructions (the swizzle has a

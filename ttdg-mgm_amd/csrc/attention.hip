@@ -111,7 +111,7 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
 #pragma unroll
         for (int n = 0; n < NB; ++n) s[k][n] = stream_t::start(stage, k0 + 32 * k, live, h);
       tile_t::template row_product<KK, NB, 0>(s, stage + cs * DC * tile_t::ES, k0, qf, l32, h);
-      if constexpr (CS > 1) attn_exchange(s[0][0], ex + w_ * 1024, ex + (w_ ^ 1) * 1024, lane);
+      if constexpr (CS > 1) attn_exchange<true>(s[0][0], ex + w_ * 1024, ex + (w_ ^ 1) * 1024, lane);
       float mx[NB];
       bool grew = false;
 #pragma unroll
@@ -337,6 +337,7 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
     // blocks of 32 keys at a time: two chains of products with 128 channels; one with 64, where two cost the third wavefront per SIMD its
     // registers (323 and 296 us)
     constexpr int KK = DP == 64 && sizeof(T) == 2 ? 1 : BN / 32;
+    static_assert(CS == 1 || BN == 32, "one pair of exchanges between two barriers");
 #pragma unroll
     for (int k0 = 0; k0 < BN; k0 += 32 * KK) {
       f32x16 s[KK][1], dp[KK][1];
@@ -348,8 +349,8 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
       tile_t::template row_product<KK, 1, PRE>(s, stage + cs * DC * tile_t::ES, k0, &qf, l32, h);
       tile_t::template row_product<KK, 1, PRE>(dp, stage + stream_t::TB + cs * DC * tile_t::ES, k0, &gf, l32, h);
       if constexpr (CS > 1) {
-        attn_exchange(s[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
-        attn_exchange(dp[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
+        attn_exchange<false>(s[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
+        attn_exchange<true>(dp[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
       }
 #pragma unroll
       for (int k = 0; k < KK; ++k) {
@@ -405,6 +406,7 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
     attn_wait_dma();
     __syncthreads();
     if (t + 1 < t1) in.issue(p, attn_smem + ((t + 1 - t0) & 1) * rows_t::STAGE);
+    static_assert(CS == 1 || BQ == 32, "one pair of exchanges between two barriers");
 #pragma unroll 1
     for (int qq = 0; qq < BQ / 32; ++qq) {
       constexpr int PRE = DP == 256 && sizeof(T) == 2 ? 4 : 0;
@@ -421,8 +423,8 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
       tile_t::template row_product<1, 1, PRE>(s, qt + cs * DC * tile_t::ES, 32 * qq, &kf, l32, h);
       tile_t::template row_product<1, 1, PRE>(dp, gt + cs * DC * tile_t::ES, 32 * qq, &vf, l32, h);
       if constexpr (CS > 1) {
-        attn_exchange(s[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
-        attn_exchange(dp[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
+        attn_exchange<false>(s[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
+        attn_exchange<true>(dp[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
       }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
