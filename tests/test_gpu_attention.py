@@ -283,6 +283,51 @@ def test_attention_empty_axes(dev):
 
 
 @gpu
+def test_attention_tensors_that_count_as_contiguous(dev):
+    """Tensors that start off a 16-byte boundary, and odd strides where a size is one or zero: the same results as for plain copies."""
+    from ttdg_mgm_amd import ops
+    g = gen(51, dev)
+    for dtype in (F32, BF16):
+        flat = normal(g, 1 + 2 * 7 * 2 * 64, dtype=dtype)
+        q, k, v = flat[1:1 + 3 * 128].view(1, 3, 2, 64), flat[1:].view(2, 7, 2, 64)[:1], flat[1:].view(2, 7, 2, 64)[1:]
+        assert q.is_contiguous() and q.data_ptr() % 16
+        assert torch.equal(ops.cross_attention(q, k, v), ops.cross_attention(q.clone(), k.clone(), v.clone()))
+        w = torch.ones(64, device=dev)
+        for a, b in zip(ops.qk_norm_rope(q, k, w, w), ops.qk_norm_rope(q.clone(), k.clone(), w, w)):
+            assert torch.equal(a, b)
+        row = normal(g, 67, dtype=dtype)
+        one = row.as_strided((1, 1, 1, 64), (67, 67, 67, 1))             # (is_contiguous(): no stride of a size of one counts)
+        assert one.is_contiguous()
+        leaf = row.clone().requires_grad_()
+        out = ops.cross_attention(leaf.as_strided((1, 1, 1, 64), (67, 67, 67, 1)), one, one)
+        # one key: p / p times v, a few roundings of 32 bits, which bfloat16 rounds away
+        assert float((out.detach() - one).abs().max()) <= 8 * U * float(one.abs().max()) and torch.autograd.grad(out.sum(), leaf)[0].shape == (67,)
+        none = normal(g, 2, 3, 67, dtype=dtype)[:, :0].unsqueeze(2)[..., :64]
+        assert float(ops.cross_attention(q.expand(2, -1, -1, -1), none, none).abs().sum()) == 0
+
+
+@gpu
+def test_long_caches_are_read_in_place(dev):
+    """Keys laid out (batch, heads, positions, channels) may have heads any distance apart: no copy is made of them."""
+    from ttdg_mgm_amd import ops
+    g = gen(52, dev)
+    T = (1 << 27) // 64 // 2 + 64
+    cache = torch.zeros(1, 2, T, 64, device=dev, dtype=BF16)
+    cache[:, :, :100] = normal(g, 1, 2, 100, 64, dtype=BF16)
+    k = cache.transpose(1, 2)
+    assert k.stride(2) * 2 > 1 << 27
+    q, lens = normal(g, 1, 1, 4, 64, dtype=BF16), torch.tensor([100], device=dev, dtype=torch.int32)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    base = torch.cuda.memory_allocated()
+    got = ops.cross_attention(q, k, k, k_lens=lens)
+    assert torch.cuda.max_memory_allocated() - base < cache.numel()
+    short = k[:, :100].contiguous()
+    ref, norm = attention_bounds(q, short, short, None, 64 ** -0.5, torch.ones(1, 100, dtype=torch.bool, device=dev))
+    close("out", got, *ref["out"], norm)
+
+
+@gpu
 def test_attention_gradients_of_some_inputs_only(dev):
     from ttdg_mgm_amd import ops
     g = gen(3, dev)

@@ -455,12 +455,13 @@ def _like(t):
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
-def _dense_rows(t):
+def _dense_rows(t, group=0):
     """``t`` (B, T, H, D) as the kernels read it: dense channels, every other stride a multiple of 16 bytes and short enough for 32-bit
-    offsets inside a tile, 16-byte aligned; anything else is copied once."""
+    offsets inside a tile (tiles of queries span the ``group`` heads of a key head), 16-byte aligned; anything else is copied once.
+    (A clone: contiguous() would return a tensor as it is that starts off a 16-byte boundary, or with any stride where a size is 1.)"""
     sb, st, sh, sd = t.stride()
-    if sd != 1 or (sb | st | sh) * t.element_size() & 15 or t.data_ptr() & 15 or st > 1 << 21 or sh * t.shape[2] > 1 << 27:
-        return t if t.numel() == 0 else t.contiguous()
+    if sd != 1 or (sb | st | sh) * t.element_size() & 15 or t.data_ptr() & 15 or st > 1 << 21 or sh * group > 1 << 27:
+        return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
@@ -579,7 +580,7 @@ def cross_attention(q, k, v, scale=None, k_lens=None, key_mask=None):
         raise ValueError("cross_attention: the scale must be positive and finite, got %r" % scale)
     if k_lens is not None and (k_lens.dtype != torch.int32 or not k_lens.is_contiguous()):
         k_lens = k_lens.to(torch.int32).contiguous()
-    q, k, v = _dense_rows(q), _dense_rows(k), _dense_rows(v)
+    q, k, v = _dense_rows(q, q.shape[2] // k.shape[2]), _dense_rows(k), _dense_rows(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return CrossAttentionFn.apply(q, k, v, scale, k_lens, key_mask)
     with _on_device_of(q):
