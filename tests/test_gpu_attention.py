@@ -307,6 +307,18 @@ def test_attention_tensors_that_count_as_contiguous(dev):
 
 
 @gpu
+def test_lengths_of_either_type_are_clamped(dev):
+    from ttdg_mgm_amd import ops
+    g = gen(53, dev)
+    q, k, v = normal(g, 4, 5, 2, 64), normal(g, 4, 9, 2, 64), normal(g, 4, 9, 2, 64)
+    want = ops.cross_attention(q, k, v, k_lens=torch.tensor([9, 0, 9, 3], device=dev, dtype=torch.int32))
+    for dtype, far in ((torch.int64, 1 << 32), (torch.int64, (1 << 62) + 1), (torch.int32, (1 << 31) - 1)):
+        lens = torch.tensor([far, -far, 9, 3], device=dev, dtype=dtype)
+        assert torch.equal(ops.cross_attention(q, k, v, k_lens=lens), want)
+        assert torch.equal(ops.cross_attention(q, k, v, k_lens=lens.repeat_interleave(2)[::2]), want)
+
+
+@gpu
 def test_long_caches_are_read_in_place(dev):
     """Keys laid out (batch, heads, positions, channels) may have heads any distance apart: no copy is made of them."""
     from ttdg_mgm_amd import ops

@@ -579,7 +579,7 @@ def cross_attention(q, k, v, scale=None, k_lens=None, key_mask=None):
     if not 0.0 < scale < 1e30:
         raise ValueError("cross_attention: the scale must be positive and finite, got %r" % scale)
     if k_lens is not None and (k_lens.dtype != torch.int32 or not k_lens.is_contiguous()):
-        k_lens = k_lens.to(torch.int32).contiguous()
+        k_lens = k_lens.clamp(0, k.shape[1]).to(torch.int32).contiguous()          # (clamped first: int64 values may not fit)
     q, k, v = _dense_rows(q, q.shape[2] // k.shape[2]), _dense_rows(k), _dense_rows(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return CrossAttentionFn.apply(q, k, v, scale, k_lens, key_mask)
