@@ -210,7 +210,8 @@ int ttdg_attention_bwd(const ttdg_attention_t* a, ttdg_stream_t stream);
  * Pair i of R / 2: channels (i, i + R / 2), or (2 i, 2 i + 1) when interleaved; axis i / (R / 2 / axes) of pos (B, T, axes), int32 or
  * (pos64) int64, element strides p_sb / p_st / p_sa; freq (R / 2) fp64 on the device; angles are formed and reduced in 64 bits.
  * R = 0: no rotation (pos / freq may be NULL).  D and R multiples of 8, D <= 256.
- * bwd reads x, w, pos, dy and writes dx and dw of both sides; ws: ttdg_qk_norm_rope_bwd_workspace_bytes(a).  No atomics. */
+ * bwd reads x, w, pos, dy and writes dx and dw of both sides (dw is zeros for a side without rows); ws: at least
+ * ttdg_qk_norm_rope_bwd_workspace_bytes(a), 16-byte aligned.  No atomics. */
 typedef struct {
   const void* x;
   int64_t sb, st, sh;
@@ -234,8 +235,6 @@ typedef struct {
 int ttdg_qk_norm_rope_fwd(const ttdg_qk_norm_rope_t* a, ttdg_stream_t stream);
 size_t ttdg_qk_norm_rope_bwd_workspace_bytes(const ttdg_qk_norm_rope_t* a);
 int ttdg_qk_norm_rope_bwd(const ttdg_qk_norm_rope_t* a, ttdg_stream_t stream);
-
-
 
 /* ---- A6+A7 graduated-assignment multi-graph matching, whole solve on device ------
  * (multi_graph_matching.py:223-244, 300-389 with num_clusters == 1; utils/hungarian.py:8-66 ->

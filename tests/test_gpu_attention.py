@@ -597,6 +597,22 @@ def test_norm_rope_empty_and_unused_outputs(dev):
     assert float(y.abs().sum()) == 0                                    # a row of zeros: eps keeps it zero
 
 
+@gpu
+def test_norm_rope_side_without_heads(dev):
+    """The weight of a side without heads gets zeros, whatever the memory held before."""
+    from ttdg_mgm_amd import ops
+    g = gen(54, dev)
+    q, k = normal(g, 2, 0, 4, 64), normal(g, 2, 5, 2, 64)
+    for lq, lk in ((q, k[:, :, :0]), (k[:, :, :0], k)):
+        wq, wk = (torch.ones(64, device=dev, requires_grad=True) for _ in range(2))
+        junk = torch.full((64,), float("nan"), device=dev)              # (what the allocator hands out next is not zeros)
+        del junk
+        yq, yk = ops.qk_norm_rope(lq, lk, wq, wk)
+        dwq, dwk = torch.autograd.grad(yq.sum() + yk.sum(), [wq, wk])
+        assert float(dwq.abs().sum()) == 0
+        assert (float(dwk.abs().sum()) == 0) == (lk.numel() == 0)
+
+
 # ------------------------------------------------------------------------------------------- together
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -821,3 +837,15 @@ def test_c_entry_points_refuse_without_a_launch():
     a = nr()
     assert lib.ttdg_qk_norm_rope_bwd(C.byref(a), None) == -1
     assert lib.ttdg_qk_norm_rope_fwd(None, None) == -1 and lib.ttdg_qk_norm_rope_bwd(None, None) == -1
+
+
+def test_norm_rope_refuses_a_misaligned_workspace():
+    import ctypes as C
+    from ttdg_mgm_amd import _lib
+    lib, fake, a = _lib.load(), 1 << 20, _lib.QkNormRope()
+    a.q.x = a.q.w = a.q.dy = a.q.dx = a.q.dw = fake
+    a.q.T, a.q.H, a.q.sb, a.q.st, a.q.sh = 4, 2, 512, 128, 64
+    a.B, a.D, a.axes, a.dtype, a.eps = 1, 64, 1, _lib.F32, 1e-6
+    a.ws_bytes = lib.ttdg_qk_norm_rope_bwd_workspace_bytes(C.byref(a))
+    a.ws = fake + 4
+    assert a.ws_bytes > 0 and lib.ttdg_qk_norm_rope_bwd(C.byref(a), None) == -1 and b"workspace" in lib.ttdg_last_error()

@@ -260,6 +260,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_dw_kernel(const float* __res
                                                               float* __restrict__ dwk) {
   __shared__ f32x4 red[4];
   const int side = blockIdx.y, c = blockIdx.x * 4;
+  if (!(side ? dwk : dwq)) return;                               // (a side without heads may come without a gradient)
   const int n = side ? nk : nq;
   const float* p = part + (side ? (int64_t)nq * D : 0) + c;
   f32x4 a = {0.f, 0.f, 0.f, 0.f};
@@ -352,7 +353,7 @@ extern "C" int ttdg_qk_norm_rope_fwd(const ttdg_qk_norm_rope_t* a, ttdg_stream_t
   const int v = qkn_v(a);
   const qkn_args p = qkn_make(a, v, false);
   for (int i = 0; i < 2; ++i) {
-    TTDG_LIMIT(p.s[i].blocks >= 0 && p.s[i].blocks < (1 << 30), "qk_norm_rope_fwd: too many workgroups");
+    TTDG_LIMIT(p.s[i].blocks >= 0 && p.s[i].blocks < (1 << 23), "qk_norm_rope_fwd: too many workgroups");      // (both sides' threads below 2^32)
     TTDG_REQUIRE(p.s[i].blocks == 0 || (p.s[i].y && (uintptr_t)p.s[i].y % 16 == 0), "qk_norm_rope_fwd: outputs must be 16-byte aligned pointers");
   }
   const int grid = p.s[0].blocks + p.s[1].blocks;
@@ -372,10 +373,10 @@ extern "C" int ttdg_qk_norm_rope_bwd(const ttdg_qk_norm_rope_t* a, ttdg_stream_t
     TTDG_REQUIRE(s.blocks == 0 || (s.dy && s.dx && ((uintptr_t)s.dy | (uintptr_t)s.dx) % 16 == 0), "qk_norm_rope_bwd: gradients must be 16-byte aligned pointers");
   }
   TTDG_REQUIRE((a->q.H == 0 || a->q.dw) && (a->k.H == 0 || a->k.dw), "qk_norm_rope_bwd: null pointer");
-  TTDG_REQUIRE(grid == 0 || (a->ws && a->ws_bytes >= (size_t)grid * a->D * 4), "qk_norm_rope_bwd: workspace too small");
+  TTDG_REQUIRE(grid == 0 || (a->ws && (uintptr_t)a->ws % 16 == 0 && a->ws_bytes >= (size_t)grid * a->D * 4), "qk_norm_rope_bwd: workspace too small or misaligned");
   p.part = (float*)a->ws;
   if (grid) QKN_LAUNCH(qk_norm_rope_bwd_kernel, a, v, grid, stream, p);
-  const int sides = a->k.H ? 2 : 1;
+  const int sides = a->k.dw ? 2 : 1;
   hipLaunchKernelGGL(qk_norm_rope_dw_kernel, dim3(a->D / 4, sides), dim3(256), 0, (hipStream_t)stream, p.part, p.s[0].blocks, p.s[1].blocks, a->D,
                      a->q.dw, a->k.dw);
   return ttdg_launch_status("qk_norm_rope_dw");
