@@ -849,3 +849,16 @@ def test_norm_rope_refuses_a_misaligned_workspace():
     a.ws_bytes = lib.ttdg_qk_norm_rope_bwd_workspace_bytes(C.byref(a))
     a.ws = fake + 4
     assert a.ws_bytes > 0 and lib.ttdg_qk_norm_rope_bwd(C.byref(a), None) == -1 and b"workspace" in lib.ttdg_last_error()
+
+
+def test_attention_refuses_launches_beyond_the_limit():
+    """More workgroups than one launch takes: an error before anything is launched."""
+    import ctypes as C
+    from ttdg_mgm_amd import _lib
+    lib, fake, a = _lib.load(), 1 << 20, _lib.Attention()
+    a.q = a.k = a.v = a.out = a.lse = a.dout = a.dq = a.dk = a.dv = a.ws = fake
+    a.B, a.Tq, a.Tk, a.H, a.Hkv, a.D, a.dtype, a.scale = 1 << 20, 1000, 8, 8, 8, 64, _lib.F32, 1.0
+    a.q_sb = a.q_st = a.q_sh = a.k_sb = a.k_st = a.k_sh = a.v_sb = a.v_st = a.v_sh = 64
+    a.ws_bytes = 1 << 62
+    for entry in (lib.ttdg_attention_fwd, lib.ttdg_attention_bwd):
+        assert entry(C.byref(a), None) < 0 and b"too many workgroups" in lib.ttdg_last_error()

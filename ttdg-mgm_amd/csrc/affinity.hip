@@ -25,7 +25,6 @@
 #define LDK (BK + 4)  // 36-word row stride: 16 rows x 4 words hit 64 distinct banks
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// acc + w * |x| in ONE instruction (fma_abs).
 // exact 0/1 step of a pair: 1 where d > 0 (down to the smallest denormal), else 0 -- two multiplies per element whose
 // [0,1] output clamp is a free modifier
 __device__ __forceinline__ f32x2 relu_step2(f32x2 d) {
@@ -41,6 +40,7 @@ __device__ __forceinline__ f32x2 relu_step2(f32x2 d) {
   return t;
 }
 
+// acc + w * |x| in ONE instruction
 __device__ __forceinline__ float fma_abs(float w, float x, float acc) {
   asm("v_fma_f32 %0, %1, |%2|, %0" : "+v"(acc) : "v"(w), "v"(x));
   return acc;

@@ -520,7 +520,7 @@ static attn_args attn_make(const ttdg_attention_t* a) {
   p.B = a->B; p.Tq = a->Tq; p.Tk = a->Tk; p.H = a->H; p.Hk = a->Hkv; p.D = a->D;
   p.G = a->H / a->Hkv; p.R = a->Tq * p.G;
   p.scale = a->scale; p.scale_log2 = a->scale * TTDG_LOG2E;
-  p.out = a->out; p.out_lo = a->out_lo; p.lse = a->lse;
+  p.out = a->out; p.out_lo = a->dtype == TTDG_BF16 ? a->out_lo : nullptr; p.lse = a->lse;
   p.dout = a->dout; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
   p.splits = 1;
   return p;
@@ -608,8 +608,8 @@ template <typename T, int DP, int BN>
 static int attn_fwd_launch(const attn_args& p, const attn_plan& q, ttdg_stream_t stream) {
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int WM = 4, lds = 2 * attn_stream<T, DP, BN, WM>::STAGE + attn_exchange_bytes(DP, F32);
-  const int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;         // (of the forward)
-  TTDG_LIMIT(grid < (1ll << 31), "attention_fwd: too many workgroups");
+  const int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;         // (of the forward; a launch's threads are counted in 32 bits)
+  TTDG_LIMIT(grid < (1ll << 24), "attention_fwd: too many workgroups");
   if constexpr (!(F32 && DP == 256)) {
     constexpr int KW = attn_kw(DP, F32), ldsk = 2 * KW * attn_stream<T, DP, 32, 1>::STAGE;
     if (q.few) ATTN_LAUNCH((attn_fwd_kernel<T, DP, 32, 1, 1, KW, attn_parts<T>(true)>), grid, 64 * KW, ldsk, stream, p);
@@ -632,7 +632,7 @@ static int attn_bwd_launch(attn_args p, const attn_plan& q, ttdg_stream_t stream
   constexpr int WM = 4, lds = 2 * attn_stream<T, DP, BN, WM>::STAGE + attn_exchange_bytes(DP, F32);
   p.splits = q.dq_splits;
   int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;
-  TTDG_LIMIT(grid < (1ll << 31), "attention_bwd: too many workgroups");
+  TTDG_LIMIT(grid < (1ll << 24), "attention_bwd: too many workgroups");
   if constexpr (!(F32 && DP == 256)) {
     if (q.few) ATTN_LAUNCH((attn_bwd_dq_kernel<T, DP, BN, 1>), grid, 64, lds, stream, p);
   }
@@ -646,7 +646,7 @@ static int attn_bwd_launch(attn_args p, const attn_plan& q, ttdg_stream_t stream
   if (p.Tk == 0 || !p.dk) return 0;
   p.splits = q.dkv_splits;
   grid = (int64_t)p.B * p.Hk * p.key_tiles * p.splits;
-  TTDG_LIMIT(grid < (1ll << 31), "attention_bwd: too many workgroups");
+  TTDG_LIMIT(grid < (1ll << 24), "attention_bwd: too many workgroups");
   constexpr int lds2 = 2 * attn_rows<T, DP, BN, WM>::STAGE + attn_exchange_bytes(DP, F32);
   if (2 * grid <= q.slots) ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, WM, attn_parts<T>(true)>), grid, 64 * WM, lds2, stream, p);
   else ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, WM, 1>), grid, 64 * WM, lds2, stream, p);
