@@ -703,6 +703,33 @@ def test_multi_head_layer_over_another_set(dev, num_heads, shared):
         assert float((one - out.detach()[1:2]).abs().max()) <= tol * float(ref.detach().abs().max())
 
 
+@gpu
+@pytest.mark.parametrize("n,m", [(0, 7), (5, 0)])
+def test_multi_head_layer_without_queries_or_states(dev, n, m):
+    from ttdg_mgm_amd.GModule.utils.attentions import MultiHeadAttention
+    torch.manual_seed(6)
+    layer = MultiHeadAttention(256, 4).to(dev)
+    g = gen(32, dev)
+    x, st = normal(g, 2, n, 256).requires_grad_(), normal(g, 2, m, 256).requires_grad_()
+    out = layer.attend(x, st)
+    grads = torch.autograd.grad(out.sum(), [x, st] + list(layer.parameters()))
+    assert out.shape == x.shape and all(bool(torch.isfinite(t).all()) for t in grads)
+    assert grads[0].shape == x.shape and grads[1].shape == st.shape
+    for a, (name, p) in zip(grads[2:], layer.named_parameters()):
+        assert a.shape == p.shape and (float(a.abs().sum()) == 0 or (n > 0 and name.split(".")[0] in ("linear_final", "layer_norm"))), name
+    if n:                                       # nothing attended to: the output projection of zeros is its bias
+        want = layer.layer_norm(x + layer.linear_final.bias)
+        # (the same 32-bit LayerNorm of the same sums: x + (0 + bias))
+        assert float((out - want).abs().max().detach()) <= 8 * U * float(want.abs().max().detach())
+
+
+def test_norm_rope_refuses_learned_frequencies():
+    from ttdg_mgm_amd import ops
+    q, _, _ = _qkv()
+    with pytest.raises(ValueError):
+        ops.qk_norm_rope(q, None, torch.ones(64), None, ops.rope_frequencies(64).requires_grad_(), torch.zeros(2, 3, dtype=torch.int64))
+
+
 def test_multi_head_layer_refuses():
     from ttdg_mgm_amd.GModule.utils.attentions import MultiHeadAttention
     m = MultiHeadAttention(256, 4)

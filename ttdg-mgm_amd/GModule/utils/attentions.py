@@ -56,6 +56,8 @@ class MultiHeadAttention(nn.Module):
             raise ValueError("attend: %d samples of queries, %d of states" % (B, states.shape[0]))
 
         def lin(x, layer):
+            if x.numel() == 0:                                           # (the products take no empty operands)
+                return F.linear(x.float(), layer.weight, layer.bias)
             y = ops.LinearFn.apply(x.float().reshape(-1, x.shape[-1]).contiguous(), layer.weight, layer.bias)
             return y.view(*x.shape[:-1], layer.out_features)
 

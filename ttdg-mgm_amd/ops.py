@@ -625,6 +625,8 @@ def _qkn_check(q, k, q_weight, k_weight, freq, q_pos, k_pos):
     if freq is not None:
         if freq.dtype != torch.float64 or freq.dim() != 1 or freq.device != q.device:
             raise TypeError("qk_norm_rope: frequencies must be a float64 vector on %s" % q.device)
+        if freq.requires_grad:
+            raise ValueError("qk_norm_rope: frequencies have no gradient; detach them")
         if q_pos is None:
             raise ValueError("qk_norm_rope: a rotation needs positions")
         R, dims = 2 * freq.shape[0], 3 if q_pos.dim() == 3 else 2
