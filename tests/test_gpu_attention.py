@@ -665,6 +665,61 @@ def test_norm_rotation_and_attention_together(dev, dtype):
 
 
 @gpu
+def test_layer_step_in_a_graph_and_on_two_streams(dev):
+    """A layer's training step (norms, rotation, attention, all gradients) and a decoding step whose position and lengths live on the device,
+    each captured once and replayed on new values between eager calls; and the same two steps on two streams at once."""
+    from ttdg_mgm_amd import ops
+    g = gen(61, dev)
+    B, T, H, Hk, D, room = 2, 40, 4, 2, 64, 3000
+    freq = ops.rope_frequencies(D, device=dev)
+    steps = torch.arange(T, device=dev)[None]
+    lens = torch.tensor([40, 11], device=dev)
+
+    def train(q, k, v, wq, wk, dout):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, wq, wk)]
+        qn, kn = ops.qk_norm_rope(leaves[0], leaves[1], leaves[3], leaves[4], freq, steps)
+        out = ops.cross_attention(qn, kn, leaves[2], k_lens=lens)
+        return (out.detach(),) + torch.autograd.grad(out, leaves, dout)
+
+    @torch.no_grad()
+    def decode(q, keys, values, wq, at, n):
+        qn, _ = ops.qk_norm_rope(q, None, wq, None, freq, at)
+        return (ops.cross_attention(qn, keys, values, k_lens=n),)
+
+    def inputs():
+        t = [normal(g, B, T, h, D, dtype=BF16) for h in (H, Hk, Hk)] + [1 + 0.1 * normal(g, D) for _ in range(2)] + [normal(g, B, T, H, D, dtype=BF16)]
+        d = [normal(g, B, 1, H, D, dtype=BF16)] + [normal(g, B, room, Hk, D, dtype=BF16) for _ in range(2)] + [1 + 0.1 * normal(g, D)]
+        at = torch.randint(0, room, (B, 1), generator=g, device=dev)
+        return t, d + [at, at[:, 0] + 1]
+
+    side, graphs = [torch.cuda.Stream() for _ in range(2)], []
+    for f, x in zip((train, decode), inputs()):
+        f(*x)
+        static, graph = [t.clone() for t in x], torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = f(*static)
+        graphs.append((graph, static, outs))
+    for turn in range(3):
+        x = inputs()
+        eager = [f(*y) for f, y in zip((train, decode), x)]
+        for (graph, static, _), y in zip(graphs, x):
+            for s, t in zip(static, y):
+                s.copy_(t)
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, outs), want in zip(graphs, eager):
+            assert all(torch.equal(a, b) for a, b in zip(outs, want)), turn
+        got = []
+        for st, f, y in zip(side, (train, decode), x):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                got.append([f(*y) for _ in range(4)][-1])
+        torch.cuda.synchronize()
+        for a, want in zip(got, eager):
+            assert all(torch.equal(c, d) for c, d in zip(a, want)), turn
+
+
+@gpu
 @pytest.mark.parametrize("num_heads,shared", [(4, False), (1, False), (8, True)])
 def test_multi_head_layer_over_another_set(dev, num_heads, shared):
     """MultiHeadAttention.attend: projections, heads, attention over ragged states, output projection, residual, LayerNorm, with gradients of
