@@ -200,6 +200,14 @@ def test_attention_long_axes_are_split_and_joined(dev, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("Tq", [127, 129])
+def test_attention_wide_heads_with_enough_rows_to_fill_the_chip(dev, Tq):
+    """float32, more than 128 channels: from 256 workgroups of 128 rows on, the forward takes another form."""
+    run_attention(dev, F32, 16, Tq, 70, 16, 16, 136, lens=[70, 0, 1, 33] * 4, mask=0.2, train=False)
+    run_attention(dev, F32, 8, 4 * Tq, 45, 8, 8, 256, train=False)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("scale,qscale", [(1.0, 8.0), (1e-3, 1.0), (0.5, 30.0)])
 def test_attention_peaked_and_flat_rows(dev, dtype, scale, qscale):

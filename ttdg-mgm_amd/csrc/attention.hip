@@ -23,8 +23,9 @@
 
 // float32 with 256 channels: the operands and sums of 32 rows times 256 channels overflow a wavefront's registers and take 14 us per tile of
 // 32 keys, so two wavefronts share 32 rows, each with half the channels: half of every score's sum (exchanged through LDS) and half of
-// the output.  dk / dv 85 -> 112 TFLOP/s, 8 x 256 rows over 794 keys forward + backward 198 -> 150 us; the exchange costs the forward of
-// large calls 14 %.  bfloat16 fits without (with the exchange: 640 -> 560 TFLOP/s).
+// the output.  dk / dv of large calls 96 -> 117 TFLOP/s, dq 104 -> 106; 8 x 256 rows over 794 keys, forward + backward, 207 -> 146 us.  The
+// forward holds one set of sums only: there large calls (attn_planned) run at 125 TFLOP/s without the exchange and at 108 with it, few
+// workgroups take 31 us with it and 40 without.  bfloat16 fits without (with the exchange: 640 -> 560 TFLOP/s).
 constexpr int attn_cs(int dp, bool f32) { return dp == 256 && f32 ? 2 : 1; }
 constexpr int attn_rows_wg(int dp, bool f32) { return 128 / attn_cs(dp, f32); }      // rows, or keys, of a workgroup of four wavefronts
 constexpr int attn_exchange_bytes(int dp, bool f32) { return attn_cs(dp, f32) > 1 ? 4 * 4096 : 0; }
@@ -40,18 +41,18 @@ constexpr int attn_waves() {
 // How many bfloat16 operands carry a probability or a score gradient into the second product (PARTS of the kernels, attn_tile::pack).  With
 // one, the rounding of p (or ds) adds an error of the size of the result's own rounding.  ds takes two everywhere: half of its terms
 // cancel in dq and dk, which then had 1.5 times the error of their own rounding (1.04 with two; backward of 4 x 2047 x 2500 x 16 heads x
-// 128: 415 -> 500 us).  p takes two where a launch leaves the chip room - few rows, or workgroups for half of the slots at most: few values are
-// averaged there, and the extra products hide behind the loads (one token over 53294 keys: 21.0 and 21.6 us) - and one in large calls
-// (8 x 1000 x 12 heads x 64 over 1500 keys, forward: 64 and 93 us), where out and dv have 1.2 to 1.45 times their own rounding's error.
+// 128: 532 -> 583 us).  p takes two where a launch leaves the chip room - few rows, or workgroups for half of the slots at most: few values are
+// averaged there, and the extra products hide behind the loads (one token over 53294 keys: 20.8 and 21.3 us) - and one in large calls
+// (8 x 1000 x 12 heads x 64 over 1500 keys: forward 65 and 85 us, dk / dv 111 and 137), where out and dv have 1.2 to 1.45 times their own rounding's error.
 template <typename T>
 constexpr int attn_parts(bool two) { return sizeof(T) == 2 && two ? 2 : 1; }
 
 // ---------------------------------------------------------------------------------------------------------------- forward
 // A wavefront owns 32 NB rows: every chunk that it reads from LDS serves NB products.  WM wavefronts share the key tiles; KW wavefronts
 // (few rows: WM = 1) have key tiles of their own, walk over parts of the keys without a barrier and join their rows at the end.
-template <typename T, int DP, int BN, int WM, int NB, int KW, int PARTS>
+template <typename T, int DP, int BN, int WM, int NB, int KW, int PARTS, int CS>
 __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ? 2 : attn_waves<T, DP, 4>())) void attn_fwd_kernel(attn_args p) {
-  constexpr int CS = WM > 1 ? attn_cs(DP, sizeof(T) == 4) : 1, DC = DP / CS;
+  constexpr int DC = DP / CS;
   typedef attn_tile<T, DC, DP> tile_t;
   typedef typename tile_t::frag frag;
   typedef attn_stream<T, DP, BN, WM> stream_t;
@@ -529,8 +530,8 @@ static attn_args attn_make(const ttdg_attention_t* a) {
 // How many workgroups share one (problem, tile): the long axis (`units` tiles of it) is split into s parts when that shortens the estimated
 // time in microseconds: `tile_us` per tile with all of the chip's `slots` taken (where several workgroups fit on a CU, one alone there runs up to
 // twice as fast, so the rounds are not counted in full), 6 us per workgroup (first loads, last stores), and for the join a launch and the parts written and read once (`part_bytes` each)
-// at 5 TB/s.  Measured both ways: dk / dv of 4 x 2047 x 16 heads over 2500 keys (320 workgroups for 512 slots) 408 us unsplit, 293 in two
-// parts, 362 in three; of 8 x 1000 x 12 heads x 64 over 1500 keys (1152 for 768) 98 us unsplit, 137 in two.
+// at 5 TB/s.  Measured both ways: dk / dv of 4 x 2047 x 16 heads over 2500 keys (320 workgroups for 512 slots) 465 us unsplit, 341 in two
+// parts, 402 in three; of 8 x 1000 x 12 heads x 64 over 1500 keys (1152 for 768) 111 us unsplit, 137 in two.
 static int attn_splits(int64_t blocks, int units, int slots, double tile_us, double part_bytes) {
   int best = 1;
   double least = 0;
@@ -546,7 +547,7 @@ static int attn_splits(int64_t blocks, int units, int slots, double tile_us, dou
 }
 
 struct attn_plan {
-  int dp, slots, few, nb, fwd_tiles, row_tiles, fwd_splits, dq_splits, key_tiles, dkv_splits;
+  int dp, slots, few, nb, fwd_cs, fwd_tiles, row_tiles, fwd_splits, dq_splits, key_tiles, dkv_splits;
   size_t fwd_ws, bwd_ws;
 };
 
@@ -567,13 +568,18 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   q.few = R <= 32 && !(f32 && q.dp == 256);
   q.row_tiles = q.few ? 1 : (int)((R + wg - 1) / wg);
   q.nb = !f32 && q.dp == 128 && !q.few && probs * ((R + 255) / 256) >= 1024 ? 2 : 1;
-  q.fwd_tiles = q.few ? 1 : (int)((R + wg * q.nb - 1) / (wg * q.nb));
+  // float32 with 256 channels: 128 rows per workgroup without the exchange, 64 with it.  A tile takes 1.74 times as long without: worth it where
+  // the workgroups fill the chip and their rounds do not come out longer.
+  const int64_t alone = probs * ((R + 127) / 128), pairs = probs * ((R + 63) / 64);
+  q.fwd_cs = attn_cs(q.dp, f32) > 1 && (alone < 256 || 174 * ((alone + 255) / 256) > 100 * ((pairs + 255) / 256)) ? 2 : 1;
+  const int fwd_wg = 128 / q.fwd_cs * q.nb;
+  q.fwd_tiles = q.few ? 1 : (int)((R + fwd_wg - 1) / fwd_wg);
   const int kt = (a->Tk + bn - 1) / bn, kt32 = (a->Tk + 31) / 32, kw = attn_kw(q.dp, f32);
   // a tile's time at 800 (bf16) / 110 TFLOP/s (fp32) for the products of a full chip; few rows: its bytes at 20 GB/s per CU
   const double es = f32 ? 4 : 2, prod_us = 2.0 * wg * bn * q.dp * shared / (f32 ? 110e6 : 800e6);
   const double q_bytes = (double)probs * R * a->D * 4, kv_bytes = 2.0 * a->B * a->Tk * a->Hkv * a->D * 4;
   q.fwd_splits = q.few ? attn_splits(probs, (kt32 + kw - 1) / kw, 1024 / kw, kw * 2 * 32 * a->D * es / 20e3, q_bytes)
-                           : attn_splits(probs * q.fwd_tiles, kt, shared, 2 * q.nb * prod_us, q_bytes);
+                           : attn_splits(probs * q.fwd_tiles, kt, shared, 2.0 * fwd_wg / wg * prod_us, q_bytes);
   q.dq_splits = attn_splits(probs * q.row_tiles, kt, shared, 3 * prod_us, q_bytes);
   q.key_tiles = (a->Tk + wg - 1) / wg;
   const int qt = (int)((R + bn - 1) / bn);
@@ -612,12 +618,15 @@ static int attn_fwd_launch(const attn_args& p, const attn_plan& q, ttdg_stream_t
   TTDG_LIMIT(grid < (1ll << 24), "attention_fwd: too many workgroups");
   if constexpr (!(F32 && DP == 256)) {
     constexpr int KW = attn_kw(DP, F32), ldsk = 2 * KW * attn_stream<T, DP, 32, 1>::STAGE;
-    if (q.few) ATTN_LAUNCH((attn_fwd_kernel<T, DP, 32, 1, 1, KW, attn_parts<T>(true)>), grid, 64 * KW, ldsk, stream, p);
+    if (q.few) ATTN_LAUNCH((attn_fwd_kernel<T, DP, 32, 1, 1, KW, attn_parts<T>(true), 1>), grid, 64 * KW, ldsk, stream, p);
   }
-  if (q.few) {
-  } else if (q.nb == 1 && 2 * grid <= q.slots) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 1, 1, attn_parts<T>(true)>), grid, 64 * WM, lds, stream, p);
-  else if (q.nb == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 1, 1, 1>), grid, 64 * WM, lds, stream, p);
-  else if constexpr (sizeof(T) == 2 && DP == 128) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 2, 1, 1>), grid, 64 * WM, lds, stream, p);
+  if constexpr (attn_cs(DP, F32) > 1) {
+    if (q.fwd_cs > 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 1, 1, 1, attn_cs(DP, F32)>), grid, 64 * WM, lds, stream, p);
+  }
+  if (q.few || q.fwd_cs > 1) {
+  } else if (q.nb == 1 && 2 * grid <= q.slots) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 1, 1, attn_parts<T>(true), 1>), grid, 64 * WM, lds, stream, p);
+  else if (q.nb == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 1, 1, 1, 1>), grid, 64 * WM, lds, stream, p);
+  else if constexpr (sizeof(T) == 2 && DP == 128) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 2, 1, 1, 1>), grid, 64 * WM, lds, stream, p);
   if (p.splits > 1) {
     const int64_t rows = (int64_t)p.B * p.Hk * p.R;
     if (p.splits > 32) ATTN_LAUNCH((attn_combine_kernel<T, 4>), rows, 256, 0, stream, p);
