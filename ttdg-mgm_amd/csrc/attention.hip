@@ -24,8 +24,8 @@
 // float32 with 256 channels: the operands and sums of 32 rows times 256 channels overflow a wavefront's registers and take 14 us per tile of
 // 32 keys, so two wavefronts share 32 rows, each with half the channels: half of every score's sum (exchanged through LDS) and half of
 // the output.  dk / dv of large calls 96 -> 117 TFLOP/s, dq 104 -> 106; 8 x 256 rows over 794 keys, forward + backward, 207 -> 146 us.  The
-// forward holds one set of sums only: there large calls (attn_planned) run at 125 TFLOP/s without the exchange and at 108 with it, few
-// workgroups take 31 us with it and 40 without.  bfloat16 fits without (with the exchange: 640 -> 560 TFLOP/s).
+// forward holds one set of sums only: there large calls run at 125 TFLOP/s without the exchange and at 108 with it, while 8 x 256 rows take
+// 31 us with it and 40 without; attn_planned compares the two.  bfloat16 fits without (with the exchange: 640 -> 560 TFLOP/s).
 constexpr int attn_cs(int dp, bool f32) { return dp == 256 && f32 ? 2 : 1; }
 constexpr int attn_rows_wg(int dp, bool f32) { return 128 / attn_cs(dp, f32); }      // rows, or keys, of a workgroup of four wavefronts
 constexpr int attn_exchange_bytes(int dp, bool f32) { return attn_cs(dp, f32) > 1 ? 4 * 4096 : 0; }
@@ -532,10 +532,11 @@ static attn_args attn_make(const ttdg_attention_t* a) {
 // twice as fast, so the rounds are not counted in full), 6 us per workgroup (first loads, last stores), and for the join a launch and the parts written and read once (`part_bytes` each)
 // at 5 TB/s.  Measured both ways: dk / dv of 4 x 2047 x 16 heads over 2500 keys (320 workgroups for 512 slots) 465 us unsplit, 341 in two
 // parts, 402 in three; of 8 x 1000 x 12 heads x 64 over 1500 keys (1152 for 768) 111 us unsplit, 137 in two.
-static int attn_splits(int64_t blocks, int units, int slots, double tile_us, double part_bytes) {
+static int attn_splits(int64_t blocks, int units, int slots, double tile_us, double part_bytes, double* estimate = nullptr) {
   int best = 1;
   double least = 0;
-  if (units < 2 || blocks < 1) return 1;
+  if (estimate) *estimate = 0;
+  if (units < 1 || blocks < 1) return 1;
   for (int s = 1; s <= 256 && (s == 1 || 2 * s <= units) && (s == 1 || blocks * s <= 8 * (int64_t)slots); ++s) {
     const int per = (units + s - 1) / s;
     const double full = (double)blocks * s / slots, rounds = (double)((blocks * s + slots - 1) / slots);
@@ -543,6 +544,7 @@ static int attn_splits(int64_t blocks, int units, int slots, double tile_us, dou
     const double us = taken * (per * tile_us + 6) + (s > 1 ? 3 + 2 * s * part_bytes / 5e6 : 0);
     if (s == 1 || us < 0.97 * least) { least = us; best = (units + per - 1) / per; }
   }
+  if (estimate) *estimate = least;
   return best;
 }
 
@@ -568,18 +570,21 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   q.few = R <= 32 && !(f32 && q.dp == 256);
   q.row_tiles = q.few ? 1 : (int)((R + wg - 1) / wg);
   q.nb = !f32 && q.dp == 128 && !q.few && probs * ((R + 255) / 256) >= 1024 ? 2 : 1;
-  // float32 with 256 channels: 128 rows per workgroup without the exchange, 64 with it.  A tile takes 1.74 times as long without: worth it where
-  // the workgroups fill the chip and their rounds do not come out longer.
-  const int64_t alone = probs * ((R + 127) / 128), pairs = probs * ((R + 63) / 64);
-  q.fwd_cs = attn_cs(q.dp, f32) > 1 && (alone < 256 || 174 * ((alone + 255) / 256) > 100 * ((pairs + 255) / 256)) ? 2 : 1;
-  const int fwd_wg = 128 / q.fwd_cs * q.nb;
-  q.fwd_tiles = q.few ? 1 : (int)((R + fwd_wg - 1) / fwd_wg);
   const int kt = (a->Tk + bn - 1) / bn, kt32 = (a->Tk + 31) / 32, kw = attn_kw(q.dp, f32);
   // a tile's time at 800 (bf16) / 110 TFLOP/s (fp32) for the products of a full chip; few rows: its bytes at 20 GB/s per CU
   const double es = f32 ? 4 : 2, prod_us = 2.0 * wg * bn * q.dp * shared / (f32 ? 110e6 : 800e6);
   const double q_bytes = (double)probs * R * a->D * 4, kv_bytes = 2.0 * a->B * a->Tk * a->Hkv * a->D * 4;
+  const int fwd_wg = 128 * q.nb;
+  const bool pairs = attn_cs(q.dp, f32) > 1;          // (prod_us is the time of 64 rows with the exchange; 128 without take 1.74 times as long)
+  q.fwd_cs = 1;
+  q.fwd_tiles = q.few ? 1 : (int)((R + fwd_wg - 1) / fwd_wg);
+  double us = 0, us2 = 0;
   q.fwd_splits = q.few ? attn_splits(probs, (kt32 + kw - 1) / kw, 1024 / kw, kw * 2 * 32 * a->D * es / 20e3, q_bytes)
-                           : attn_splits(probs * q.fwd_tiles, kt, shared, 2.0 * fwd_wg / wg * prod_us, q_bytes);
+                           : attn_splits(probs * q.fwd_tiles, kt, shared, (pairs ? 2 * 1.74 : 2.0 * q.nb) * prod_us, q_bytes, &us);
+  if (pairs) {                       // 64 rows per workgroup where that fills the chip better
+    const int splits = attn_splits(probs * q.row_tiles, kt, shared, 2 * prod_us, q_bytes, &us2);
+    if (us2 < us) { q.fwd_cs = 2; q.fwd_tiles = q.row_tiles; q.fwd_splits = splits; }
+  }
   q.dq_splits = attn_splits(probs * q.row_tiles, kt, shared, 3 * prod_us, q_bytes);
   q.key_tiles = (a->Tk + wg - 1) / wg;
   const int qt = (int)((R + bn - 1) / bn);
