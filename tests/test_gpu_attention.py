@@ -200,6 +200,23 @@ def test_attention_long_axes_are_split_and_joined(dev, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[1500, 90, 0, 1, 64, 700], [1500] * 6, [0] * 5 + [33], [0] * 6, [1, 1500] + [65] * 4])
+def test_attention_ragged_samples_share_the_parts(dev, dtype, D, lens):
+    """Few rows per sample and many keys: the parts of the key axis (and, for dk and dv, of the rows) go to the samples by their lengths."""
+    run_attention(dev, dtype, 6, 70, 1500, 2, 1, D, lens=lens)
+
+
+@gpu
+def test_attention_ragged_batches_of_any_size(dev):
+    """Up to 64 samples the lengths decide about the parts, beyond all samples get the same number."""
+    for B in (2, 63, 64, 65, 100):
+        run_attention(dev, F32, B, 33, 400, 1, 1, 256, lens=[(37 * i + 400) % 401 for i in range(B)])
+        run_attention(dev, BF16, B, 1, 400, 4, 1, 64, lens=[(37 * i + 400) % 401 for i in range(B)], mask=0.1)
+
+
+@gpu
 @pytest.mark.parametrize("Tq", [127, 129])
 def test_attention_wide_heads_with_enough_rows_to_fill_the_chip(dev, Tq):
     """float32, more than 128 channels: from 256 workgroups of 128 rows on, the forward takes another form."""

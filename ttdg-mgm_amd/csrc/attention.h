@@ -20,13 +20,14 @@ struct attn_args {
   const uint8_t* key_mask;
   int64_t m_sb, m_st;
   int B, Tq, Tk, H, Hk, D, G, R;                                    // G = H / Hk query heads per key head, R = Tq G rows per problem
-  int row_tiles, key_tiles, splits;
+  int row_tiles, key_tiles, splits, slots;                          // slots: workgroups of dk / dv that the chip runs at once
   float scale, scale_log2;                                          // scale, scale * log2(e)
   void *out, *out_lo;
   float* lse;                                                       // (problem, row): log2 of the row's sum of exponentials
   const void* dout;
   void *dq, *dk, *dv;
   float *delta, *part_o, *part_lse;                                 // delta: minus do . o of every row
+  int32_t* share;                                                   // (first part or tile, how many) of every sample; null: all alike
 };
 
 __device__ __forceinline__ f32x16 f32x16_all(float x) {
@@ -72,13 +73,130 @@ __device__ __forceinline__ void attn_dma4(__amdgpu_buffer_rsrc_t r, char* lds_wa
 __device__ __forceinline__ void attn_store4(float* out, f32x4 x) { *(f32x4*)out = x; }
 __device__ __forceinline__ void attn_store4(__bf16* out, f32x4 x) { *(bf16x4*)out = __builtin_convertvector(x, bf16x4); }
 
-// workgroup -> (problem, tile, split), tiles of one split next to each other
-__device__ __forceinline__ void attn_block(const attn_args& p, int tiles, int& prob, int& tile, int& split) {
-  const int L = blockIdx.x, per = tiles * p.splits;
-  prob = L / per;
-  const int rem = L - prob * per;
-  split = rem / tiles;
-  tile = rem - split * tiles;
+// sum over the lanes up to the own one
+__device__ __forceinline__ uint32_t attn_scan(uint32_t x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);      // from 1, 2, 4, 8 lanes before, inside rows of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);     // the last lane of a row, to the next one
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);     // lane 31, to the upper half
+  return x;
+}
+__device__ __forceinline__ uint32_t attn_ceil(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
+
+// keys of sample b
+__device__ __forceinline__ int attn_length(const attn_args& p, int b) { return p.k_lens ? max(0, min(p.k_lens[b], p.Tk)) : p.Tk; }
+
+// workgroup -> (sample, its keys, key head, tile, split of how many, first part of the sample)
+struct attn_item {
+  int b, keys, hk, prob, tile, split, splits, base;
+  __device__ __forceinline__ void uniform() {      // (they are; said to the compiler, which otherwise keeps them in vector registers)
+    b = __builtin_amdgcn_readfirstlane(b);
+    keys = __builtin_amdgcn_readfirstlane(keys);
+    hk = __builtin_amdgcn_readfirstlane(hk);
+    prob = __builtin_amdgcn_readfirstlane(prob);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    split = __builtin_amdgcn_readfirstlane(split);
+    splits = __builtin_amdgcn_readfirstlane(splits);
+    base = __builtin_amdgcn_readfirstlane(base);
+  }
+};
+
+// The long axis is in parts: all samples alike, or (RAGGED and p.share, at most 64 samples, one per lane) as many for each as its own length
+// gives: the B splits parts there are go round in units of `unit` keys, as few units per part as possible.  False: a part too many.
+template <bool RAGGED>
+__device__ __forceinline__ bool attn_place(const attn_args& p, int tiles, int unit, attn_item& w) {
+  const int L = blockIdx.x;
+  if (!RAGGED || !p.share) {
+    const int per = tiles * p.splits;
+    w.prob = L / per;
+    const int rem = L - w.prob * per;
+    w.splits = p.splits;
+    w.split = rem / tiles;
+    w.tile = rem - w.split * tiles;
+    w.b = w.prob / p.Hk;
+    w.hk = w.prob - w.b * p.Hk;
+    w.base = w.b * p.splits;
+    w.keys = attn_length(p, w.b);
+  } else {
+    const int per = p.Hk * tiles, j = L / per, rem = L - j * per;
+    w.hk = rem / tiles;
+    w.tile = rem - w.hk * tiles;
+    const int lane = threadIdx.x & 63;
+    const bool on = lane < p.B;
+    const int len = on ? attn_length(p, lane) : 0;
+    const uint32_t n = attn_ceil(len, unit), room = p.B * p.splits, total = __builtin_amdgcn_readlane(attn_scan(n), 63);
+    uint32_t each = max(1u, attn_ceil(total, room)), mine = on ? max(1u, attn_ceil(n, each)) : 0, end = attn_scan(mine);
+    if ((uint32_t)__builtin_amdgcn_readlane(end, 63) > room) {
+      uint32_t lo = each + 1;
+      each = max(lo, attn_ceil(total, room - p.B));            // (with this many they fit: at most total / each + B parts)
+      while (lo < each) {
+        const uint32_t mid = (lo + each) / 2;
+        if ((uint32_t)__builtin_amdgcn_readlane(attn_scan(on ? max(1u, attn_ceil(n, mid)) : 0), 63) <= room) each = mid;
+        else lo = mid + 1;
+      }
+      mine = on ? max(1u, attn_ceil(n, each)) : 0;
+      end = attn_scan(mine);
+    }
+    if (L == 0 && threadIdx.x < p.B) {
+      p.share[2 * lane] = end - mine;
+      p.share[2 * lane + 1] = mine;
+    }
+    if (j >= __builtin_amdgcn_readlane(end, 63)) return false;
+    w.b = __popcll(__ballot(end <= (uint32_t)j));
+    w.splits = __builtin_amdgcn_readlane(mine, w.b);
+    w.base = __builtin_amdgcn_readlane(end, w.b) - w.splits;
+    w.keys = __builtin_amdgcn_readlane(len, w.b);
+    w.split = j - w.base;
+    w.prob = w.b * p.Hk + w.hk;
+  }
+  w.uniform();
+  return true;
+}
+
+// The same for dk / dv: (sample, key head, key tile, split of the rows).  With p.share the workgroups go to the key tiles that have keys, every
+// one of them in as many parts as there is room for; base: number of the key tile among these.
+__device__ __forceinline__ bool attn_place_keys(const attn_args& p, int unit, int row_units, attn_item& w) {
+  const int L = blockIdx.x;
+  if (!p.share) {
+    const int per = p.key_tiles * p.splits;
+    w.prob = L / per;
+    const int rem = L - w.prob * per;
+    w.splits = p.splits;
+    w.split = rem / p.key_tiles;
+    w.tile = rem - w.split * p.key_tiles;
+    w.b = w.prob / p.Hk;
+    w.hk = w.prob - w.b * p.Hk;
+    w.base = w.b * p.key_tiles + w.tile;
+    w.keys = attn_length(p, w.b);
+    w.uniform();
+    return true;
+  }
+  const int lane = threadIdx.x & 63;
+  const int len = lane < p.B ? attn_length(p, lane) : 0;
+  const uint32_t mine = attn_ceil(len, unit), end = attn_scan(mine);
+  const int tiles = __builtin_amdgcn_readlane(end, 63);
+  // (of the host's splits there is always room, of more only what the chip runs at once)
+  const int most = min(row_units, max(p.splits, p.slots / (p.Hk * max(tiles, 1))));
+  w.splits = attn_ceil(row_units, attn_ceil(row_units, most));
+  if (L == 0 && threadIdx.x < p.B) {
+    p.share[2 * lane] = end - mine;
+    p.share[2 * lane + 1] = mine;
+    p.share[2 * 64] = w.splits;
+  }
+  const int per = tiles * w.splits;
+  if (L >= per * p.Hk) return false;
+  w.hk = L / per;
+  const int rem = L - w.hk * per;
+  w.split = rem / tiles;
+  w.base = rem - w.split * tiles;
+  w.b = __popcll(__ballot(end <= (uint32_t)w.base));
+  w.tile = w.base - (__builtin_amdgcn_readlane(end, w.b) - __builtin_amdgcn_readlane(mine, w.b));
+  w.keys = __builtin_amdgcn_readlane(len, w.b);
+  w.prob = w.b * p.Hk + w.hk;
+  w.uniform();
+  return true;
 }
 
 // the part [t0, t1) of n tiles that falls to one of the splits
@@ -102,8 +220,8 @@ struct attn_keys {
   int n;
   const uint8_t* mask;
   int64_t m_st;
-  __device__ __forceinline__ attn_keys(const attn_args& p, int b) {
-    n = p.k_lens ? max(0, min(p.k_lens[b], p.Tk)) : p.Tk;
+  __device__ __forceinline__ attn_keys(const attn_args& p, int b, int keys) {
+    n = keys;
     mask = p.key_mask ? p.key_mask + b * p.m_sb : nullptr;
     m_st = p.m_st;
   }
@@ -381,7 +499,7 @@ struct attn_stream {
   uint32_t ahead;                    // the mask byte of this lane's key of the next tile, asked for a tile earlier (kept as it comes: a
                                      // comparison here would wait for it)
 
-  __device__ __forceinline__ attn_stream(const attn_args& p, int b, int hk, int wave_, int lane_) : keys(p, b), next(0), wave(wave_), lane(lane_) {
+  __device__ __forceinline__ attn_stream(const attn_args& p, int b, int hk, int n, int wave_, int lane_) : keys(p, b, n), next(0), wave(wave_), lane(lane_) {
     k = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh;
     v = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh;
     k_tile = BN * p.k_st;

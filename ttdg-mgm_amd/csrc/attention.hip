@@ -65,9 +65,9 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
   const int cs = CS > 1 ? w_ % CS : 0;                        // which part of the channels
   char* const smem = attn_smem + kw * 2 * stream_t::STAGE;
   float* const ex = (float*)(attn_smem + 2 * stream_t::STAGE);
-  int prob, tile, split;
-  attn_block(p, p.row_tiles, prob, tile, split);
-  const int b = prob / p.Hk, hk = prob - b * p.Hk;
+  attn_item at;
+  if (!attn_place<(WM > 1)>(p, p.row_tiles, BN, at)) return;
+  const int b = at.b, hk = at.hk, prob = at.prob, tile = at.tile, split = at.split;
 
   const int row0 = (tile * (WM / CS) + wave / CS) * 32 * NB + l32;      // block n of this lane: row0 + 32 n
   frag qf[NB][tile_t::NP];
@@ -83,9 +83,9 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
     l[n] = 0.f;
   }
 
-  stream_t in(p, b, hk, wave, lane);
+  stream_t in(p, b, hk, at.keys, wave, lane);
   int t0, t1;
-  attn_part(in.tiles(), split * KW + kw, p.splits * KW, t0, t1);
+  attn_part(in.tiles(), split * KW + kw, at.splits * KW, t0, t1);
   in.seek(t0);
   uint64_t live_next = 0;
   if (t0 < t1) {
@@ -201,7 +201,7 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
     const int row = row0 + 32 * n;
     if (row >= p.R) continue;
     if (p.splits > 1) {
-      const int64_t pr = ((int64_t)prob * p.R + row) * p.splits + split;
+      const int64_t pr = (int64_t)at.base * p.Hk * p.R + ((int64_t)hk * p.R + row) * at.splits + split;
       if (h == 0 && cs == 0) p.part_lse[pr] = lse;
       tile_t::store_row(o[n], inv, p.part_o + pr * p.D + cs * DC, (float*)nullptr, p.D - cs * DC, h);
     } else {
@@ -224,21 +224,23 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(attn_args p) {
   if (id >= (int64_t)p.B * p.Hk * p.R) return;                     // (W > 1: the whole workgroup)
   const int prob = (int)(id / p.R), row = (int)(id - (int64_t)prob * p.R);
   const int b = prob / p.Hk, hk = prob - b * p.Hk;
-  const float* lse = p.part_lse + id * p.splits;
-  const float* part = p.part_o + id * p.splits * p.D;
+  const int base = p.share ? p.share[2 * b] : b * p.splits, splits = p.share ? p.share[2 * b + 1] : p.splits;
+  const int64_t first_part = (int64_t)base * p.Hk * p.R + ((int64_t)hk * p.R + row) * splits;
+  const float* lse = p.part_lse + first_part;
+  const float* part = p.part_o + first_part * p.D;
   float mx = -INFINITY;
-  for (int s = lane; s < p.splits; s += 64) mx = fmaxf(mx, lse[s]);
+  for (int s = lane; s < splits; s += 64) mx = fmaxf(mx, lse[s]);
   mx = wave_max(mx);
   const bool any = mx > -INFINITY || mx != mx;
-  const float base = any ? mx : 0.f;
+  const float top = any ? mx : 0.f;
   const int per = p.D <= 64 ? 16 : p.D <= 128 ? 32 : 64;           // lanes per row
   const int c = 4 * (lane & (per - 1)), first = (W > 1 ? wave * (64 / per) : 0) + lane / per, step = W * (64 / per);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   float z = 0.f;
   if (c < p.D) {
 #pragma unroll 4
-    for (int s = first; s < p.splits; s += step) {
-      const float w = fast_exp2(lse[s] - base);
+    for (int s = first; s < splits; s += step) {
+      const float w = fast_exp2(lse[s] - top);
       z += w;
       o += *(const f32x4*)(part + (int64_t)s * p.D + c) * w;
     }
@@ -285,9 +287,9 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
   extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = lane >> 5, l32 = lane & 31;
-  int prob, tile, split;
-  attn_block(p, p.row_tiles, prob, tile, split);
-  const int b = prob / p.Hk, hk = prob - b * p.Hk;
+  attn_item at;
+  if (!attn_place<(WM > 1)>(p, p.row_tiles, BN, at)) return;
+  const int b = at.b, hk = at.hk, prob = at.prob, tile = at.tile, split = at.split;
 
   const int cs = CS > 1 ? wave % CS : 0;                      // which part of the channels
   float* const ex = (float*)(attn_smem + 2 * stream_t::STAGE);
@@ -314,9 +316,9 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
 #pragma unroll
   for (int d = 0; d < DC / 32; ++d) acc[d] = f32x16_zero();
 
-  stream_t in(p, b, hk, wave, lane);
+  stream_t in(p, b, hk, at.keys, wave, lane);
   int t0, t1;
-  attn_part(in.tiles(), split, p.splits, t0, t1);
+  attn_part(in.tiles(), split, at.splits, t0, t1);
   in.seek(t0);
   uint64_t live_next = 0;
   if (t0 < t1) {
@@ -363,7 +365,8 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
     }
   }
   if (row >= p.R) return;
-  if (p.splits > 1) tile_t::store_row(acc, 1.f, p.part_o + (int64_t)split * p.B * p.Tq * p.H * p.D + off, (float*)nullptr, p.D - cs * DC, h);
+  const int64_t sample = (int64_t)p.Tq * p.H * p.D;
+  if (p.splits > 1) tile_t::store_row(acc, 1.f, p.part_o + (at.base + split - b) * sample + off, (float*)nullptr, p.D - cs * DC, h);
   else tile_t::store_row(acc, p.scale, (T*)p.dq + off, (T*)nullptr, p.D - cs * DC, h);
 }
 
@@ -378,14 +381,14 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
   extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = lane >> 5, l32 = lane & 31;
-  int prob, tile, split;
-  attn_block(p, p.key_tiles, prob, tile, split);
-  const int b = prob / p.Hk, hk = prob - b * p.Hk;
+  attn_item at;
+  if (!attn_place_keys(p, 32 * WM / CS, (p.R + BQ - 1) / BQ, at)) return;
+  const int b = at.b, hk = at.hk, prob = at.prob, tile = at.tile, split = at.split;
 
   const int cs = CS > 1 ? wave % CS : 0;                      // which part of the channels
   float* const ex = (float*)(attn_smem + 2 * rows_t::STAGE);
   const int key = (tile * (WM / CS) + wave / CS) * 32 + l32;
-  const attn_keys keys(p, b);
+  const attn_keys keys(p, b, at.keys);
   const bool mine = keys.alive(key);
   const int64_t kr = min(key, p.Tk - 1);
   const T* kp = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh + kr * p.k_st + cs * DC;
@@ -398,7 +401,7 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
   for (int d = 0; d < DC / 32; ++d) { dk[d] = f32x16_zero(); dv[d] = f32x16_zero(); }
 
   int t0, t1;
-  attn_part(__syncthreads_or(mine) ? (p.R + BQ - 1) / BQ : 0, split, p.splits, t0, t1);      // no key of this workgroup exists: zeros
+  attn_part(__syncthreads_or(mine) ? (p.R + BQ - 1) / BQ : 0, split, at.splits, t0, t1);      // no key of this workgroup exists: zeros
   rows_t in(p, b, hk, prob, t0, wave, lane);
   if (t0 < t1) in.issue(p, attn_smem);
   for (int t = t0; t < t1; ++t) {
@@ -450,28 +453,47 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
     for (int d = 0; d < DC / 32; ++d) { dk[d] = f32x16_zero(); dv[d] = f32x16_zero(); }
   }
   if (p.splits > 1) {
-    const int64_t plane = (int64_t)p.B * p.Tk * p.Hk * p.D;
-    tile_t::store_row(dk, 1.f, p.part_o + 2 * split * plane + off, (float*)nullptr, p.D - cs * DC, h);
-    tile_t::store_row(dv, 1.f, p.part_o + (2 * split + 1) * plane + off, (float*)nullptr, p.D - cs * DC, h);
+    constexpr int KEYS = 32 * WM / CS;
+    float* part = p.part_o + ((((int64_t)at.base * at.splits + split) * p.Hk + hk) * 2 * KEYS + key - tile * KEYS) * p.D + cs * DC;
+    tile_t::store_row(dk, 1.f, part, (float*)nullptr, p.D - cs * DC, h);
+    tile_t::store_row(dv, 1.f, part + KEYS * p.D, (float*)nullptr, p.D - cs * DC, h);
   } else {
     tile_t::store_row(dk, p.scale, (T*)p.dk + off, (T*)nullptr, p.D - cs * DC, h);
     tile_t::store_row(dv, 1.f, (T*)p.dv + off, (T*)nullptr, p.D - cs * DC, h);
   }
 }
 
-// adds the planes of a split in their order: out[i] = factor * sum_s part[s * stride + i], four values per thread (n % 4 == 0: D is);
-// blockIdx.y = 1: the second tensor, whose planes follow the first one's
+// adds the parts of dq in their order: dq[i] = scale * sum_s part_s[i], four values per thread (D % 4 == 0; with parts dq has less than 2^31 values)
 template <typename T>
-__global__ __launch_bounds__(256) void attn_reduce_kernel(const float* __restrict__ part, int64_t stride, int splits, float factor, T* __restrict__ out,
-                                                          T* __restrict__ out2, int64_t n) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= n) return;
-  const float* at = part + i + (blockIdx.y ? n : 0);
+__global__ __launch_bounds__(256) void attn_reduce_q_kernel(attn_args p) {
+  const uint32_t sample = (uint32_t)(p.Tq * p.H * p.D), i = (blockIdx.x * 256 + threadIdx.x) * 4, b = i / sample;
+  if (b >= (uint32_t)p.B) return;
+  const int base = p.share ? p.share[2 * b] : b * p.splits, splits = p.share ? p.share[2 * b + 1] : p.splits;
+  const float* at = p.part_o + (int64_t)base * sample + (i - b * sample);
   f32x4 a = *(const f32x4*)at;
 #pragma unroll 4
-  for (int s = 1; s < splits; ++s) a += *(const f32x4*)(at + s * stride);
-  if (blockIdx.y) attn_store4(out2 + i, a);
-  else attn_store4(out + i, a * factor);
+  for (int s = 1; s < splits; ++s) a += *(const f32x4*)(at + (int64_t)s * sample);
+  attn_store4((T*)p.dq + i, a * p.scale);
+}
+
+// the same for dk (blockIdx.y = 0) and dv, whose parts lie in tiles of `keys` keys; tiles without keys have no parts
+template <typename T>
+__global__ __launch_bounds__(256) void attn_reduce_kv_kernel(attn_args p, int keys) {
+  const uint32_t head = (blockIdx.x * 256 + threadIdx.x) * 4 / p.D, d = (blockIdx.x * 256 + threadIdx.x) * 4 - head * p.D;
+  const uint32_t row = head / p.Hk, hk = head - row * p.Hk, b = row / p.Tk, key = row - b * p.Tk, tile = key / keys;
+  if (b >= (uint32_t)p.B) return;
+  const int base = p.share ? p.share[2 * b] : b * p.key_tiles, tiles = p.share ? p.share[2 * b + 1] : p.key_tiles;
+  const int splits = p.share ? p.share[2 * 64] : p.splits;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+  if (tile < (uint32_t)tiles) {
+    const int64_t step = (int64_t)p.Hk * 2 * keys * p.D;
+    const float* at = p.part_o + (base + tile) * splits * step + ((hk * 2 + blockIdx.y) * keys + key - tile * keys) * p.D + d;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) a += *(const f32x4*)(at + s * step);
+  }
+  const int64_t i = (int64_t)head * p.D + d;
+  if (blockIdx.y) attn_store4((T*)p.dv + i, a);
+  else attn_store4((T*)p.dk + i, a * p.scale);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -549,12 +571,15 @@ static int attn_splits(int64_t blocks, int units, int slots, double tile_us, dou
 }
 
 struct attn_plan {
-  int dp, slots, few, nb, fwd_cs, fwd_tiles, row_tiles, fwd_splits, dq_splits, key_tiles, dkv_splits;
+  int dp, slots, few, nb, fwd_cs, fwd_tiles, row_tiles, fwd_splits, dq_splits, key_tiles, dkv_splits, fwd_share, dq_share, dkv_share, fwd_two, dkv_two;
+  int64_t dkv_grid;
   size_t fwd_ws, bwd_ws;
 };
 
 // keys per tile of the kernels that share tiles between wavefronts; 32 where wavefronts have their own
 static int attn_bn(int dp, bool f32) { return dp == 64 || (dp == 128 && !f32) ? 64 : 32; }
+
+#define ATTN_SHARE_BYTES ((2 * 64 + 4) * 4)
 
 static attn_plan attn_planned(const ttdg_attention_t* a) {
   attn_plan q;
@@ -589,12 +614,28 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   q.key_tiles = (a->Tk + wg - 1) / wg;
   const int qt = (int)((R + bn - 1) / bn);
   q.dkv_splits = attn_splits(probs * q.key_tiles, qt, shared, 4 * prod_us, kv_bytes);
+  q.fwd_two = q.few || (q.nb == 1 && 2 * probs * q.fwd_tiles * q.fwd_splits <= shared);        // (see attn_parts)
+  q.dkv_two = 2 * probs * q.key_tiles * q.dkv_splits <= shared;
+  // Ragged samples: only the device knows their lengths, and the kernels divide by them (attn_place) where the workgroups run all at once.  What
+  // the host says is how many parts there may be: as many as the chip has slots for.  Forward and backward of 8 x 256 rows over
+  // up to 794 keys, float32, 256 channels: 147 -> 135 us with 447 to 794 keys, 137 -> 86 us with one sample of 794 and seven of 40 to 200; what
+  // the division costs when all are alike: 2 us of 78 (8 x 64 rows over 128 keys).
+  const bool ragged = a->k_lens && a->B > 1 && a->B <= 64;
+  const auto share = [&](int& splits, int64_t blocks) {
+    if (!ragged || q.few || splits < 2 || blocks * splits > shared) return 0;
+    const int64_t most = shared / blocks < kt / 2 ? shared / blocks : kt / 2;
+    if (most > splits) splits = (int)most;
+    return 1;
+  };
+  q.fwd_share = share(q.fwd_splits, probs * q.fwd_tiles);
+  q.dq_share = share(q.dq_splits, probs * q.row_tiles);
+  q.dkv_grid = probs * q.key_tiles * q.dkv_splits;
+  q.dkv_share = ragged && q.dkv_splits > 1;
+  if (q.dkv_share && q.dkv_grid < shared) q.dkv_grid = shared / a->Hkv * a->Hkv;
   const size_t rows = (size_t)probs * R;
-  q.fwd_ws = q.fwd_splits > 1 ? (size_t)q.fwd_splits * rows * (a->D + 1) * 4 : 0;
-  const size_t kv = (size_t)a->B * a->Tk * a->Hkv * a->D * 4;
-  size_t w = q.dq_splits > 1 ? (size_t)q.dq_splits * rows * a->D * 4 : 0;
-  if (q.dkv_splits > 1 && 2 * kv * q.dkv_splits > w) w = 2 * kv * q.dkv_splits;
-  q.bwd_ws = rows * 4 + 16 + w;
+  q.fwd_ws = q.fwd_splits > 1 ? (size_t)q.fwd_splits * rows * (a->D + 1) * 4 + ATTN_SHARE_BYTES : 0;
+  const size_t dq = q.dq_splits > 1 ? (size_t)q.dq_splits * rows * a->D * 4 : 0, dkv = q.dkv_splits > 1 ? (size_t)q.dkv_grid * 2 * wg * a->D * 4 : 0;
+  q.bwd_ws = rows * 4 + 16 + ATTN_SHARE_BYTES + (dq > dkv ? dq : dkv);
   return q;
 }
 
@@ -629,12 +670,14 @@ static int attn_fwd_launch(const attn_args& p, const attn_plan& q, ttdg_stream_t
     if (q.fwd_cs > 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 1, 1, 1, attn_cs(DP, F32)>), grid, 64 * WM, lds, stream, p);
   }
   if (q.few || q.fwd_cs > 1) {
-  } else if (q.nb == 1 && 2 * grid <= q.slots) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 1, 1, attn_parts<T>(true), 1>), grid, 64 * WM, lds, stream, p);
+  } else if (q.fwd_two) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 1, 1, attn_parts<T>(true), 1>), grid, 64 * WM, lds, stream, p);
   else if (q.nb == 1) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 1, 1, 1, 1>), grid, 64 * WM, lds, stream, p);
   else if constexpr (sizeof(T) == 2 && DP == 128) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 2, 1, 1, 1>), grid, 64 * WM, lds, stream, p);
   if (p.splits > 1) {
     const int64_t rows = (int64_t)p.B * p.Hk * p.R;
-    if (p.splits > 32) ATTN_LAUNCH((attn_combine_kernel<T, 4>), rows, 256, 0, stream, p);
+    // four wavefronts per row from 32 parts on; with ragged samples, the longest of which may have several times the parts there are on average,
+    // from 12 on while the rows are few (1024 rows of 256 channels: 8.5 -> 5.1 us; 4096 rows of 64: 5.7 -> 8.6)
+    if (p.splits > (p.share && rows <= 2048 ? 12 : 32)) ATTN_LAUNCH((attn_combine_kernel<T, 4>), rows, 256, 0, stream, p);
     else ATTN_LAUNCH((attn_combine_kernel<T, 1>), (rows + 3) / 4, 256, 0, stream, p);
   }
   return 0;
@@ -645,6 +688,8 @@ static int attn_bwd_launch(attn_args p, const attn_plan& q, ttdg_stream_t stream
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int WM = 4, lds = 2 * attn_stream<T, DP, BN, WM>::STAGE + attn_exchange_bytes(DP, F32);
   p.splits = q.dq_splits;
+  int32_t* const share = p.share;
+  if (!q.dq_share) p.share = nullptr;
   int64_t grid = (int64_t)p.B * p.Hk * p.row_tiles * p.splits;
   TTDG_LIMIT(grid < (1ll << 24), "attention_bwd: too many workgroups");
   if constexpr (!(F32 && DP == 256)) {
@@ -653,20 +698,20 @@ static int attn_bwd_launch(attn_args p, const attn_plan& q, ttdg_stream_t stream
   if (!q.few) ATTN_LAUNCH((attn_bwd_dq_kernel<T, DP, BN, WM>), grid, 64 * WM, lds, stream, p);
   const int64_t nq = (int64_t)p.B * p.Tq * p.H * p.D, nk = (int64_t)p.B * p.Tk * p.Hk * p.D;
   if (p.splits > 1) {
-    hipLaunchKernelGGL(attn_reduce_kernel<T>, dim3((unsigned)((nq / 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p.part_o, nq, p.splits, p.scale,
-                       (T*)p.dq, (T*)nullptr, nq);
+    hipLaunchKernelGGL(attn_reduce_q_kernel<T>, dim3((unsigned)((nq / 4 + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p);
     if (int e = ttdg_launch_status("attn_reduce")) return e;
   }
   if (p.Tk == 0 || !p.dk) return 0;
   p.splits = q.dkv_splits;
-  grid = (int64_t)p.B * p.Hk * p.key_tiles * p.splits;
+  p.share = q.dkv_share ? share : nullptr;
+  grid = q.dkv_grid;
   TTDG_LIMIT(grid < (1ll << 24), "attention_bwd: too many workgroups");
   constexpr int lds2 = 2 * attn_rows<T, DP, BN, WM>::STAGE + attn_exchange_bytes(DP, F32);
-  if (2 * grid <= q.slots) ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, WM, attn_parts<T>(true)>), grid, 64 * WM, lds2, stream, p);
+  if (q.dkv_two) ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, WM, attn_parts<T>(true)>), grid, 64 * WM, lds2, stream, p);
   else ATTN_LAUNCH((attn_bwd_dkv_kernel<T, DP, BN, WM, 1>), grid, 64 * WM, lds2, stream, p);
   if (p.splits > 1) {
-    hipLaunchKernelGGL(attn_reduce_kernel<T>, dim3((unsigned)((nk / 4 + 255) / 256), 2), dim3(256), 0, (hipStream_t)stream, p.part_o, 2 * nk, p.splits,
-                       p.scale, (T*)p.dk, (T*)p.dv, nk);
+    hipLaunchKernelGGL(attn_reduce_kv_kernel<T>, dim3((unsigned)((nk / 4 + 255) / 256), 2), dim3(256), 0, (hipStream_t)stream, p,
+                       attn_rows_wg(DP, F32));
     if (int e = ttdg_launch_status("attn_reduce")) return e;
   }
   return 0;
@@ -695,7 +740,8 @@ extern "C" int ttdg_attention_fwd(const ttdg_attention_t* a, ttdg_stream_t strea
   p.row_tiles = q.fwd_tiles;
   p.splits = q.fwd_splits;
   p.part_o = (float*)a->ws;
-  p.part_lse = (float*)a->ws + (size_t)q.fwd_splits * p.B * p.Hk * p.R * p.D;
+  p.part_lse = p.part_o + (size_t)q.fwd_splits * p.B * p.Hk * p.R * p.D;
+  p.share = q.fwd_share ? (int32_t*)(p.part_lse + (size_t)q.fwd_splits * p.B * p.Hk * p.R) : nullptr;
   ATTN_DISPATCH(attn_fwd_launch, a, p, q, stream);
 }
 
@@ -714,7 +760,9 @@ extern "C" int ttdg_attention_bwd(const ttdg_attention_t* a, ttdg_stream_t strea
   attn_args p = attn_make(a);
   p.row_tiles = q.row_tiles;
   p.key_tiles = q.key_tiles;
+  p.slots = q.slots;
   p.delta = (float*)a->ws;
-  p.part_o = (float*)a->ws + (((size_t)p.B * p.Hk * p.R + 3) & ~(size_t)3);
+  p.share = (int32_t*)(p.delta + (((size_t)p.B * p.Hk * p.R + 3) & ~(size_t)3));
+  p.part_o = (float*)p.share + ATTN_SHARE_BYTES / 4;
   ATTN_DISPATCH(attn_bwd_launch, a, p, q, stream);
 }
