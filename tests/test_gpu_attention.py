@@ -745,6 +745,33 @@ def test_layer_step_in_a_graph_and_on_two_streams(dev):
 
 
 @gpu
+def test_ragged_step_in_a_graph_follows_its_lengths(dev):
+    """Forward and backward of ragged samples captured once: the lengths are read at every replay, and so is how the work is divided by them."""
+    from ttdg_mgm_amd import ops
+    g = gen(71, dev)
+    for dtype, D in ((F32, 256), (BF16, 64)):
+        x = [normal(g, 5, n, 2, D, dtype=dtype) for n in (90, 1100, 1100, 90)]
+        lens = torch.full((5,), 1100, device=dev, dtype=torch.int32)
+
+        def step(q, k, v, dout, n):
+            leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+            out = ops.cross_attention(*leaves, k_lens=n)
+            return (out.detach(),) + torch.autograd.grad(out, leaves, dout)
+
+        step(*x, lens)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step(*x, lens)
+        for now in ([1100, 3, 40, 0, 900], [0, 0, 0, 0, 1], [1100] * 5, [0] * 5, [64, 1100, 1, 1099, 65]):
+            lens.copy_(torch.tensor(now))
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in outs]
+            want = step(*x, lens.clone())
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), now
+
+
+@gpu
 @pytest.mark.parametrize("num_heads,shared", [(4, False), (1, False), (8, True)])
 def test_multi_head_layer_over_another_set(dev, num_heads, shared):
     """MultiHeadAttention.attend: projections, heads, attention over ragged states, output projection, residual, LayerNorm, with gradients of
