@@ -51,7 +51,13 @@ __device__ __forceinline__ float attn_half_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-__device__ __forceinline__ void attn_wait_dma() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// waits for every load and LDS-DMA of this wavefront (0xf70: vmcnt 0, the other counters as they are).  The builtin, not assembly text: the
+// compiler then knows that nothing is outstanding and adds no waits of its own behind the next tile's LDS-DMA.
+__device__ __forceinline__ void attn_wait_dma() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xf70);
+  asm volatile("" ::: "memory");
+}
 
 // Transposing LDS read: of the 4 x 16 block that 16 neighbouring lanes address (lane i: row i / 4, columns 4 (i % 4) ...) lane i gets column i.
 // (restrict: without alias information the compiler would wait here for every LDS-DMA in flight, that is for the next tile.)
@@ -431,20 +437,27 @@ struct attn_tile {
   }
 };
 
+// A barrier for what the wavefronts wrote to LDS themselves.  (__syncthreads waits for LDS-DMA in flight as well, that is for the next tile.)
+__device__ __forceinline__ void attn_lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // Two wavefronts that hold sums over half the channels each add them: `own` and `other` are their 4 KiB of LDS.  Every wavefront of the
 // workgroup takes part in the barriers; the one behind the reads is left out (LAST) where another follows before the next exchange.
 template <bool LAST>
 __device__ __forceinline__ void attn_exchange(f32x16& x, float* own, const float* other, int lane) {
 #pragma unroll
   for (int g = 0; g < 4; ++g) ((f32x4*)own)[g * 64 + lane] = f32x4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
-  __syncthreads();
+  attn_lds_barrier();
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const f32x4 y = ((const f32x4*)other)[g * 64 + lane];
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[4 * g + e] += y[e];
   }
-  if (!LAST) __syncthreads();
+  if (!LAST) attn_lds_barrier();
 }
 
 // LDS-DMA of ROWS tile rows: instruction i of a wavefront fills 1 KiB; its lanes' offsets repeat every PER instructions (the swizzle has a
