@@ -55,7 +55,7 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
   constexpr int DC = DP / CS;
   typedef attn_tile<T, DC, DP> tile_t;
   typedef typename tile_t::frag frag;
-  typedef attn_stream<T, DP, BN, WM> stream_t;
+  typedef attn_stream<T, DP, BN, WM, (NB > 1)> stream_t;
   static_assert(WM == 1 || KW == 1, "wavefronts along rows or along keys");
   static_assert(CS == 1 || (NB == 1 && BN == 32), "one sum at a time to exchange");
   extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
