@@ -51,7 +51,7 @@ __device__ __forceinline__ float attn_half_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// waits for every load and LDS-DMA of this wavefront (0xf70: vmcnt 0, the other counters as they are).  The builtin, not assembly text: the
+// Waits for every load and LDS-DMA of this wavefront (0xf70: vmcnt 0, the other counters as they are).  The builtin, not assembly text: the
 // compiler then knows that nothing is outstanding and adds no waits of its own behind the next tile's LDS-DMA.
 __device__ __forceinline__ void attn_wait_dma() {
   asm volatile("" ::: "memory");
@@ -515,7 +515,7 @@ struct attn_stream {
   uint32_t ahead;                    // the mask byte of this lane's key of the next tile, asked for a tile earlier (kept as it comes: a
                                      // comparison here would wait for it)
 
-  __device__ __forceinline__ attn_stream(const attn_args& p, int b, int hk, int n, int wave_, int lane_) : keys(p, b, n), next(0), wave(wave_), lane(lane_), D(p.D) {
+  __device__ __forceinline__ attn_stream(const attn_args& p, int b, int hk, int n, int wave_, int lane_) : keys(p, b, n), next(0), wave(wave_), lane(lane_), D(p.D), ahead(0) {
     k = (const T*)p.k + b * p.k_sb + (int64_t)hk * p.k_sh;
     v = (const T*)p.v + b * p.v_sb + (int64_t)hk * p.v_sh;
     k_tile = BN * p.k_st;
@@ -535,13 +535,18 @@ struct attn_stream {
   }
   __device__ __forceinline__ void peek() {
     const int key = next * BN + lane;
-    ahead = 1;
-    if (keys.mask && key < keys.n) ahead = keys.mask[key * keys.m_st];
+    if (keys.mask) ahead = key < keys.n ? keys.mask[key * keys.m_st] : 0;
   }
-  // starts the next tile's way into `stage` and returns which of its keys exist (none: nothing is loaded)
+  // starts the next tile's way into `stage` and returns which of its keys exist (none: nothing is loaded); asks for the mask of the tile after it
   __device__ __forceinline__ uint64_t issue(char* stage) {
-    const bool mine = lane < BN && next * BN + lane < keys.n && ahead;
+    bool mine = lane < BN && next * BN + lane < keys.n;
+    if (keys.mask) {
+      asm volatile("" : "+v"(ahead));                   // (awaited in here: without a mask there is nothing to wait for)
+      mine = mine && ahead;
+    }
     const uint64_t live = __ballot(mine);
+    ++next;
+    peek();
     if (live) {
       const bool all = live == ALL;
       if (LEAN) {
@@ -558,7 +563,6 @@ struct attn_stream {
     }
     k += k_tile;
     v += v_tile;
-    ++next;
     return live;
   }
   // starting values of the scores

@@ -91,7 +91,6 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
   if (t0 < t1) {
     in.peek();
     live_next = in.issue(smem);
-    in.peek();
   }
   constexpr int KK = NB == 1 ? BN / 32 : 1;                // blocks of 32 keys at a time: as many sums as the registers hold
   for (int t = t0; t < t1; ++t) {
@@ -99,10 +98,7 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
     const uint64_t live = live_next;
     attn_wait_dma();                 // this wavefront's share of tile t has landed
     if (WM > 1) __syncthreads();     // ... everybody's has, and nobody still reads the other stage
-    if (t + 1 < t1) {
-      live_next = in.issue(smem + ((t + 1 - t0) & 1) * stream_t::STAGE);
-      in.peek();
-    }
+    if (t + 1 < t1) live_next = in.issue(smem + ((t + 1 - t0) & 1) * stream_t::STAGE);
     if (live == 0) continue;         // (the same for every wavefront of the workgroup)
 #pragma unroll 1
     for (int k0 = 0; k0 < BN; k0 += 32 * KK) {
@@ -324,17 +320,13 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
   if (t0 < t1) {
     in.peek();
     live_next = in.issue(attn_smem);
-    in.peek();
   }
   for (int t = t0; t < t1; ++t) {
     char* stage = attn_smem + ((t - t0) & 1) * stream_t::STAGE;
     const uint64_t live = live_next;
     attn_wait_dma();
     __syncthreads();
-    if (t + 1 < t1) {
-      live_next = in.issue(attn_smem + ((t + 1 - t0) & 1) * stream_t::STAGE);
-      in.peek();
-    }
+    if (t + 1 < t1) live_next = in.issue(attn_smem + ((t + 1 - t0) & 1) * stream_t::STAGE);
     if (live == 0) continue;
     constexpr int PRE = DP == 256 && sizeof(T) == 2 ? 2 : 0;      // one wavefront per SIMD: nobody else hides the LDS
     // blocks of 32 keys at a time: two chains of products with 128 channels; one with 64, where two cost the third wavefront per SIMD its
