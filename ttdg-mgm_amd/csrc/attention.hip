@@ -23,7 +23,7 @@
 
 // float32 with 256 channels: the operands and sums of 32 rows times 256 channels overflow a wavefront's registers and take 14 us per tile of
 // 32 keys, so two wavefronts share 32 rows, each with half the channels: half of every score's sum (exchanged through LDS) and half of
-// the output.  dk / dv of large calls 96 -> 117 TFLOP/s, dq 104 -> 106; 8 x 256 rows over 794 keys, forward + backward, 207 -> 146 us.  The
+// the output.  dk / dv of large calls 96 -> 118 TFLOP/s, dq 104 -> 111; 8 x 256 rows over 794 keys, forward + backward, 207 -> 143 us.  The
 // forward holds one set of sums only: there large calls run at 125 TFLOP/s without the exchange and at 108 with it, while 8 x 256 rows take
 // 31 us with it and 40 without; attn_planned compares the two.  bfloat16 fits without (with the exchange: 640 -> 560 TFLOP/s).
 constexpr int attn_cs(int dp, bool f32) { return dp == 256 && f32 ? 2 : 1; }
@@ -586,6 +586,8 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   const int wg = attn_rows_wg(q.dp, f32);
   q.few = R <= 32 && !(f32 && q.dp == 256);
   q.row_tiles = q.few ? 1 : (int)((R + wg - 1) / wg);
+  // 64 rows per wavefront where the workgroups still go round twice: 16 x 2048 rows over 4096 keys, 8 heads, 632 -> 596 us; with fewer workgroups
+  // the rounds decide (batch 4: 163 -> 202 us, 8: 318 -> 304, 9: 395 -> 431).  With 64 channels 361 -> 378 us.
   q.nb = !f32 && q.dp == 128 && !q.few && probs * ((R + 255) / 256) >= 1024 ? 2 : 1;
   const int kt = (a->Tk + bn - 1) / bn, kt32 = (a->Tk + 31) / 32, kw = attn_kw(q.dp, f32);
   // a tile's time at 800 (bf16) / 110 TFLOP/s (fp32) for the products of a full chip; few rows: its bytes at 20 GB/s per CU
