@@ -175,7 +175,8 @@ int ttdg_mha_adjacency(const float* q, const float* k, int d, ttdg_graphs_t gr, 
  *     out[b,i,h,:] = sum_j softmax_j(scale * q[b,i,h,:] . k[b,j,h',:]) v[b,j,h',:]        out (B, Tq, H, D) contiguous
  * dtype TTDG_F32: products in fp32 on the matrix unit; TTDG_BF16: products of bf16 with fp32 sums, probabilities (and, backward, the
  * score gradients) rounded to bf16 between the two products.  Softmax statistics are fp32.
- * For a backward pass later: lse (B, Hkv, Tq * H / Hkv) fp32 (log2 of the sums) and, bf16 only, out_lo (like out: what the rounding of
+ * Scores may be of any finite size; the sums before their division - the keys' number times 2^8 times the largest |v| - have to be finite.
+ * For a backward pass later: lse (2, B, Hkv, Tq * H / Hkv) fp32 (log2 of the sums, and the score they are relative to) and, bf16 only, out_lo (like out: what the rounding of
  * out dropped) are written when not NULL, and the backward reads q, k, v, out, out_lo, lse, dout (contiguous like out) and writes dq like
  * out, dk / dv (B, Tk, Hkv, D) contiguous (zeros at keys that do not exist; both NULL: not wanted).  No atomics: results do not change from run to run.
  * ws / ws_bytes: at least ttdg_attention_{fwd,bwd}_workspace_bytes(a), 16-byte aligned (0 bytes: NULL is fine); nothing in it outlives the call.

@@ -23,7 +23,7 @@ struct attn_args {
   int row_tiles, key_tiles, splits, slots;                          // slots: workgroups of dk / dv that the chip runs at once
   float scale, scale_log2;                                          // scale, scale * log2(e)
   void *out, *out_lo;
-  float* lse;                                                       // (problem, row): log2 of the row's sum of exponentials
+  float *lse, *far;                                                 // (problem, row): log2 of the row's sum of exponentials, see attn_ref
   const void* dout;
   void *dq, *dk, *dv;
   float *delta, *part_o, *part_lse;                                 // delta: minus do . o of every row
@@ -78,6 +78,30 @@ __device__ __forceinline__ void attn_dma4(__amdgpu_buffer_rsrc_t r, char* lds_wa
 
 __device__ __forceinline__ void attn_store4(float* out, f32x4 x) { *(f32x4*)out = x; }
 __device__ __forceinline__ void attn_store4(__bf16* out, f32x4 x) { *(bf16x4*)out = __builtin_convertvector(x, bf16x4); }
+
+// A row's reference point: its terms are 2^((s - far) k - ref), k = scale log2(e).  Up to ATTN_FAR (in powers of two) far is 0 and ref the
+// scaled score, so that a term costs one fma and its exponential; the rounding of ref, up to 2^-17, is the same for all terms.  A larger scaled
+// score has no 32-bit number near enough (half a step of 10^9 is 2^5), there far is the score itself, which the subtraction cancels
+// exactly, and ref 0.  A row's log of the sum is kept as the same two numbers: far, and lse = ref + log2(sum).
+// A wavefront asks once whether any of its rows is far and leaves the subtraction out if none is.
+#define ATTN_FAR 256.f
+struct attn_ref {
+  float at;                          // far or ref, whichever is not 0 (one register less than both); -infinity: no key yet
+  bool is_far;
+  __device__ __forceinline__ float far() const { return is_far ? at : 0.f; }
+  __device__ __forceinline__ float ref() const { return is_far ? 0.f : at; }
+  __device__ __forceinline__ bool any() const { return is_far || at > -INFINITY; }
+  // how far this point lies above the other one, in powers of two
+  __device__ __forceinline__ float above(const attn_ref& o, float k) const { return fmaf(far() - o.far(), k, ref() - o.ref()); }
+  // the same for a score
+  __device__ __forceinline__ float below(float s, float k) const { return fmaf(s - far(), k, -ref()); }
+};
+// the reference point of score s
+__device__ __forceinline__ attn_ref attn_ref_at(float s, float k) {
+  const float c = s * k;
+  const bool far = !(fabsf(c) <= ATTN_FAR);
+  return attn_ref{far ? s : c, far};
+}
 
 // sum over the lanes up to the own one
 __device__ __forceinline__ uint32_t attn_scan(uint32_t x) {
@@ -580,18 +604,20 @@ struct attn_stream {
   }
 };
 
-// The row tiles of the dk / dv kernel, in stages of LDS: q tile, do tile, lse and delta of the rows
+// The row tiles of the dk / dv kernel, in stages of LDS: q tile, do tile, lse, delta and far of the rows
 template <typename T, int DP, int BQ, int WM>
 struct attn_rows {
   typedef attn_tile<T, DP> tile_t;
-  static constexpr int TB = tile_t::bytes(BQ), STAGE = 2 * TB + 512;
+  static constexpr int TB = tile_t::bytes(BQ), STAGE = 2 * TB + 768;
   attn_loader<T, DP, BQ, WM> lq, lg;
   const T *q, *g;
-  const float *lse, *delta;
+  const float *lse, *delta, *far;
   int next, wave, lane;
-  __device__ __forceinline__ attn_rows(const attn_args& p, int b, int hk, int prob, int first, int wave_, int lane_) : next(first), wave(wave_), lane(lane_) {
+  float ahead;                       // far of this lane's row of the next tile
+  __device__ __forceinline__ attn_rows(const attn_args& p, int b, int hk, int prob, int first, int wave_, int lane_) : next(first), wave(wave_), lane(lane_), ahead(0.f) {
     lse = p.lse + (int64_t)prob * p.R;
     delta = p.delta + (int64_t)prob * p.R;
+    far = p.far + (int64_t)prob * p.R;
     q = (const T*)p.q + b * p.q_sb + (int64_t)hk * p.G * p.q_sh;
     g = (const T*)p.dout + ((int64_t)b * p.Tq * p.H + (int64_t)hk * p.G) * p.D;
     lq.init(p.D, wave, lane);
@@ -615,7 +641,11 @@ struct attn_rows {
       const uint32_t off = lane < BQ && lane < left ? lane * 4 : ATTN_OOB;
       attn_dma4(attn_rsrc(lse + r0), stage + 2 * TB, off);
       attn_dma4(attn_rsrc(delta + r0), stage + 2 * TB + 256, off);
+      attn_dma4(attn_rsrc(far + r0), stage + 2 * TB + 512, off);
     }
+    ahead = lane < BQ && lane < left ? far[r0 + lane] : 0.f;
     ++next;
   }
+  // whether a row of the tile that has landed has a far reference point (asked before the next one is started)
+  __device__ __forceinline__ bool some_far() const { return __any(ahead != 0.f); }
 };

@@ -56,6 +56,11 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
   typedef attn_tile<T, DC, DP> tile_t;
   typedef typename tile_t::frag frag;
   typedef attn_stream<T, DP, BN, WM, (NB > 1)> stream_t;
+  // Scores are added up in the same order here and in the backward kernels, bit for bit: s - far must be zero there where it was here.  What
+  // two wavefronts add there in halves, one adds here in two sums.
+  constexpr int HN = CS == 1 ? attn_cs(DP, sizeof(T) == 4) : 1;
+  typedef attn_tile<T, DC / HN, DP> score_t;
+  static_assert(HN == 1 || (NB == 1 && BN == 32), "two sums of one block of scores");
   static_assert(WM == 1 || KW == 1, "wavefronts along rows or along keys");
   static_assert(CS == 1 || (NB == 1 && BN == 32), "one sum at a time to exchange");
   extern __shared__ __attribute__((aligned(1024))) char attn_smem[];
@@ -70,16 +75,20 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
   const int b = at.b, hk = at.hk, prob = at.prob, tile = at.tile, split = at.split;
 
   const int row0 = (tile * (WM / CS) + wave / CS) * 32 * NB + l32;      // block n of this lane: row0 + 32 n
-  frag qf[NB][tile_t::NP];
+  frag qf[NB * HN][score_t::NP];
   f32x16 o[NB][DC / 32];
-  float m[NB], l[NB];
+  attn_ref m[NB];
+  float l[NB];
+  bool far = false;                  // some row of this wavefront has a far reference point
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     const attn_row rw(p, hk, row0 + 32 * n);
-    tile_t::load_row(qf[n], (const T*)p.q + b * p.q_sb + (int64_t)rw.t * p.q_st + (int64_t)rw.head * p.q_sh + cs * DC, p.D - cs * DC, h);
+    const T* row = (const T*)p.q + b * p.q_sb + (int64_t)rw.t * p.q_st + (int64_t)rw.head * p.q_sh + cs * DC;
+#pragma unroll
+    for (int i = 0; i < HN; ++i) score_t::load_row(qf[n * HN + i], row + i * (DC / HN), p.D - cs * DC - i * (DC / HN), h);
 #pragma unroll
     for (int d = 0; d < DC / 32; ++d) o[n][d] = f32x16_zero();
-    m[n] = -INFINITY;
+    m[n] = attn_ref{-INFINITY, false};
     l[n] = 0.f;
   }
 
@@ -107,7 +116,13 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
       for (int k = 0; k < KK; ++k)
 #pragma unroll
         for (int n = 0; n < NB; ++n) s[k][n] = stream_t::start(stage, k0 + 32 * k, live, h);
-      tile_t::template row_product<KK, NB, 0>(s, stage + cs * DC * tile_t::ES, k0, qf, l32, h);
+      score_t::template row_product<KK, NB, 0>(s, stage + cs * DC * tile_t::ES, k0, qf, l32, h);
+      if constexpr (HN > 1) {
+        f32x16 s1[1][1] = {{f32x16_zero()}};
+        score_t::template row_product<1, 1, 0>(s1, stage + DC / HN * tile_t::ES, k0, qf + 1, l32, h);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[0][0][e] += s1[0][0][e];
+      }
       if constexpr (CS > 1) attn_exchange<true>(s[0][0], ex + w_ * 1024, ex + (w_ ^ 1) * 1024, lane);
       float mx[NB];
       bool grew = false;
@@ -118,27 +133,41 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
         for (int k = 0; k < KK; ++k)
 #pragma unroll
           for (int e = 0; e < 16; ++e) mx[n] = fmaxf(mx[n], s[k][n][e]);
-        mx[n] = attn_half_max(mx[n]) * p.scale_log2;
-        grew |= mx[n] > m[n] + 8.f;
+        mx[n] = attn_half_max(mx[n]);
+        grew |= m[n].below(mx[n], p.scale_log2) > 8.f;
       }
-      // The reference point m follows the running maximum only when that has grown by more than 2^8: terms up to 2^8 round no worse than
-      // terms up to 1 and their sums are far from any limit, and with m at every new maximum most tiles would rescale the sums.
+      // A row's reference point m follows its running maximum only when that has grown by more than 2^8: terms up to 2^8 round no worse than
+      // terms up to 1 and their sums are far from any limit, and with m at every new maximum most tiles would rescale the sums.  (Row by
+      // row: what a row comes to does not depend on the rows beside it.)
       if (__any(grew)) {
+        far = false;
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          const float mn = fmaxf(m[n], mx[n]), a = mn > -INFINITY ? fast_exp2(m[n] - mn) : 1.f;
+          const bool up = m[n].below(mx[n], p.scale_log2) > 8.f;
+          const attn_ref at_max = attn_ref_at(mx[n], p.scale_log2), mn = {up ? at_max.at : m[n].at, up ? at_max.is_far : m[n].is_far};
+          const float a = up ? (m[n].any() ? fast_exp2(m[n].above(mn, p.scale_log2)) : 0.f) : 1.f;
           l[n] *= a;
 #pragma unroll
           for (int d = 0; d < DC / 32; ++d) o[n][d] *= a;
           m[n] = mn;
+          far |= mn.is_far;
         }
+        far = __any(far);
+      }
+      if (far) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int k = 0; k < KK; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[k][n][e] -= m[n].far();
       }
 #pragma unroll
       for (int k = 0; k < KK; ++k) {
         typename tile_t::template operand<PARTS> pr[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-          const float ref = m[n] > -INFINITY ? m[n] : 0.f;      // (no key yet in this row: every term is 2^-infinity = 0)
+          const float ref = m[n].any() ? m[n].ref() : 0.f;      // (no key yet in this row: every term is 2^-infinity = 0)
 #pragma unroll
           for (int e = 0; e < 16; ++e) s[k][n][e] = fast_exp2(fmaf(s[k][n][e], p.scale_log2, -ref));
           pr[n] = tile_t::template pack<PARTS>(s[k][n]);
@@ -149,43 +178,48 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
     }
   }
   if constexpr (KW > 1) {              // the wavefronts' rows meet in LDS, wavefront 0 goes on with them
-    static_assert(NB == 1 && KW * 32 * (DP + 2) * 4 <= KW * 2 * stream_t::STAGE, "the rows fit where the tiles were");
+    static_assert(NB == 1 && KW * 32 * (DP + 3) * 4 <= KW * 2 * stream_t::STAGE, "the rows fit where the tiles were");
     l[0] = attn_half_sum(l[0]);
     __syncthreads();
-    float* mine = (float*)attn_smem + kw * 32 * (DP + 2);
+    constexpr int PART = 32 * (DP + 3);
+    float* mine = (float*)attn_smem + kw * PART;
     if (kw > 0) {
 #pragma unroll
       for (int d = 0; d < DC / 32; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) mine[(32 * d + attn_reg_row(e) + 4 * h) * 32 + l32] = o[0][d][e];
       if (h == 0) {
-        mine[DP * 32 + l32] = m[0];
+        mine[DP * 32 + l32] = m[0].at;
         mine[DP * 32 + 32 + l32] = l[0];
+        mine[DP * 32 + 64 + l32] = m[0].is_far ? 1.f : 0.f;
       }
     }
     __syncthreads();
     if (kw > 0) return;
-    float mx = m[0], f[KW];
-#pragma unroll
-    for (int w = 1; w < KW; ++w) mx = fmaxf(mx, mine[w * 32 * (DP + 2) + DP * 32 + l32]);
-    const float ref = mx > -INFINITY ? mx : 0.f;
-    f[0] = fast_exp2(m[0] - ref);
-    l[0] *= f[0];
+    attn_ref mw[KW], top = m[0];
+    float f[KW];
+    mw[0] = m[0];
 #pragma unroll
     for (int w = 1; w < KW; ++w) {
-      f[w] = fast_exp2(mine[w * 32 * (DP + 2) + DP * 32 + l32] - ref);
-      l[0] = fmaf(f[w], mine[w * 32 * (DP + 2) + DP * 32 + 32 + l32], l[0]);
+      mw[w] = attn_ref{mine[w * PART + DP * 32 + l32], mine[w * PART + DP * 32 + 64 + l32] != 0.f};
+      const bool up = mw[w].any() && (!top.any() || mw[w].above(top, p.scale_log2) > 0.f);
+      top = attn_ref{up ? mw[w].at : top.at, up ? mw[w].is_far : top.is_far};
     }
+#pragma unroll
+    for (int w = 0; w < KW; ++w) f[w] = mw[w].any() ? fast_exp2(mw[w].above(top, p.scale_log2)) : 0.f;
+    l[0] *= f[0];
+#pragma unroll
+    for (int w = 1; w < KW; ++w) l[0] = fmaf(f[w], mine[w * PART + DP * 32 + 32 + l32], l[0]);
 #pragma unroll
     for (int d = 0; d < DC / 32; ++d)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         float x = o[0][d][e] * f[0];
 #pragma unroll
-        for (int w = 1; w < KW; ++w) x = fmaf(f[w], mine[w * 32 * (DP + 2) + (32 * d + attn_reg_row(e) + 4 * h) * 32 + l32], x);
+        for (int w = 1; w < KW; ++w) x = fmaf(f[w], mine[w * PART + (32 * d + attn_reg_row(e) + 4 * h) * 32 + l32], x);
         o[0][d][e] = x;
       }
-    m[0] = mx;
+    m[0] = top;
     l[0] *= 0.5f;                      // (both halves hold the whole sum; they are added below)
   }
 #pragma unroll
@@ -193,23 +227,30 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
     const float sum = attn_half_sum(l[n]);
     const bool any = sum > 0.f || sum != sum;
     const float inv = any ? 1.f / sum : 0.f;                // no key at all: zeros
-    const float lse = any ? m[n] + fast_log2(sum) : -INFINITY;
+    const float lse = any ? (m[n].any() ? m[n].ref() : 0.f) + fast_log2(sum) : -INFINITY;
     const int row = row0 + 32 * n;
     if (row >= p.R) continue;
     if (p.splits > 1) {
       const int64_t pr = (int64_t)at.base * p.Hk * p.R + ((int64_t)hk * p.R + row) * at.splits + split;
-      if (h == 0 && cs == 0) p.part_lse[pr] = lse;
+      if (h == 0 && cs == 0) {
+        p.part_lse[2 * pr] = lse;
+        p.part_lse[2 * pr + 1] = m[n].far();
+      }
       tile_t::store_row(o[n], inv, p.part_o + pr * p.D + cs * DC, (float*)nullptr, p.D - cs * DC, h);
     } else {
       const attn_row rw(p, hk, row);
-      if (h == 0 && cs == 0 && p.lse) p.lse[(int64_t)prob * p.R + row] = lse;
+      if (h == 0 && cs == 0 && p.lse) {
+        p.lse[(int64_t)prob * p.R + row] = lse;
+        p.far[(int64_t)prob * p.R + row] = m[n].far();
+      }
       const int64_t off = (((int64_t)b * p.Tq + rw.t) * p.H + rw.head) * p.D + cs * DC;
       tile_t::store_row(o[n], inv, (T*)p.out + off, p.out_lo ? (T*)p.out_lo + off : (T*)nullptr, p.D - cs * DC, h);
     }
   }
 }
 
-// Joins the splits of a row: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max).  W wavefronts per row: a lane owns four channels and
+// Joins the splits of a row: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max), the logs taken from the largest far of the parts on (a part
+// with a smaller far is exactly as far below as the difference says, or has no weight at all).  W wavefronts per row: a lane owns four channels and
 // every n-th split (n = 64 W / lanes per row), loads several splits ahead, and the lanes' sums meet by shuffles and, for W > 1, in LDS.
 // Bound by latency: with one wavefront walking over 256 splits a row took 186 us, with four 8 us (16 heads, 53294 keys, 128 channels).
 template <typename T, int W>
@@ -222,13 +263,26 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(attn_args p) {
   const int b = prob / p.Hk, hk = prob - b * p.Hk;
   const int base = p.share ? p.share[2 * b] : b * p.splits, splits = p.share ? p.share[2 * b + 1] : p.splits;
   const int64_t first_part = (int64_t)base * p.Hk * p.R + ((int64_t)hk * p.R + row) * splits;
-  const float* lse = p.part_lse + first_part;
+  const f32x2* lse = (const f32x2*)p.part_lse + first_part;       // (lse, far)
   const float* part = p.part_o + first_part * p.D;
-  float mx = -INFINITY;
-  for (int s = lane; s < splits; s += 64) mx = fmaxf(mx, lse[s]);
+  float mx = -INFINITY, far = 0.f;
+  bool any = false, some_far = false;
+  for (int s = lane; s < splits; s += 64) {
+    const f32x2 x = lse[s];
+    any |= x.x != -INFINITY;
+    some_far |= x.y != 0.f;
+    mx = fmaxf(mx, x.x);
+  }
+  any = __any(any);
+  const auto log_at = [&](f32x2 x) { return x.x == -INFINITY ? -INFINITY : fmaf(x.y - far, p.scale_log2, x.x); };
+  if (__any(some_far)) {
+    far = mx = -INFINITY;
+    for (int s = lane; s < splits; s += 64) far = fmaxf(far, lse[s].x == -INFINITY ? -INFINITY : lse[s].y);      // (a part without keys has none)
+    far = wave_max(far);
+    for (int s = lane; s < splits; s += 64) mx = fmaxf(mx, log_at(lse[s]));
+  }
   mx = wave_max(mx);
-  const bool any = mx > -INFINITY || mx != mx;
-  const float top = any ? mx : 0.f;
+  const float top = mx > -INFINITY ? mx : 0.f;
   const int per = p.D <= 64 ? 16 : p.D <= 128 ? 32 : 64;           // lanes per row
   const int c = 4 * (lane & (per - 1)), first = (W > 1 ? wave * (64 / per) : 0) + lane / per, step = W * (64 / per);
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -236,7 +290,7 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(attn_args p) {
   if (c < p.D) {
 #pragma unroll 4
     for (int s = first; s < splits; s += step) {
-      const float w = fast_exp2(lse[s] - top);
+      const float w = fast_exp2(log_at(lse[s]) - top);
       z += w;
       o += *(const f32x4*)(part + (int64_t)s * p.D + c) * w;
     }
@@ -268,7 +322,10 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(attn_args p) {
   o *= any ? 1.f / z : 0.f;
   attn_store4((T*)p.out + off, o);
   if (sizeof(T) == 2 && p.out_lo) attn_store4((T*)p.out_lo + off, o - __builtin_convertvector(__builtin_convertvector(o, bf16x4), f32x4));
-  if (lane == 0 && p.lse) p.lse[id] = any ? mx + fast_log2(z) : -INFINITY;
+  if (lane == 0 && p.lse) {
+    p.lse[id] = any ? top + fast_log2(z) : -INFINITY;
+    p.far[id] = far;
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------- backward
@@ -304,6 +361,8 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
     __syncthreads();
   }
   float lse = p.lse[(int64_t)prob * p.R + rw.row];
+  const float far = p.far[(int64_t)prob * p.R + rw.row];
+  const bool some_far = __any(far != 0.f);
   if (split == 0 && h == 0 && cs == 0 && row < p.R) p.delta[(int64_t)prob * p.R + row] = -delta;
   if (lse == -INFINITY) lse = INFINITY;       // a row without any key: p = 0
 
@@ -346,6 +405,12 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
       if constexpr (CS > 1) {
         attn_exchange<false>(s[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
         attn_exchange<true>(dp[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
+      }
+      if (some_far) {
+#pragma unroll
+        for (int k = 0; k < KK; ++k)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[k][0][e] -= far;
       }
 #pragma unroll
       for (int k = 0; k < KK; ++k) {
@@ -401,6 +466,7 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
     const char* gt = qt + rows_t::TB;
     attn_wait_dma();
     __syncthreads();
+    const bool some_far = in.some_far();
     if (t + 1 < t1) in.issue(p, attn_smem + ((t + 1 - t0) & 1) * rows_t::STAGE);
     static_assert(CS == 1 || BQ == 32, "one pair of exchanges between two barriers");
 #pragma unroll 1
@@ -421,6 +487,14 @@ __global__ ATTN_WAVES(64 * WM, (attn_waves<T, DP, 3>())) void attn_bwd_dkv_kerne
       if constexpr (CS > 1) {
         attn_exchange<false>(s[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
         attn_exchange<true>(dp[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
+      }
+      if (some_far) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 far = *(const f32x4*)(st + 128 + 8 * g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[0][0][4 * g + e] -= far[e];
+        }
       }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -535,7 +609,7 @@ static attn_args attn_make(const ttdg_attention_t* a) {
   p.B = a->B; p.Tq = a->Tq; p.Tk = a->Tk; p.H = a->H; p.Hk = a->Hkv; p.D = a->D;
   p.G = a->H / a->Hkv; p.R = a->Tq * p.G;
   p.scale = a->scale; p.scale_log2 = a->scale * TTDG_LOG2E;
-  p.out = a->out; p.out_lo = a->dtype == TTDG_BF16 ? a->out_lo : nullptr; p.lse = a->lse;
+  p.out = a->out; p.out_lo = a->dtype == TTDG_BF16 ? a->out_lo : nullptr; p.lse = a->lse; p.far = a->lse ? a->lse + (size_t)a->B * a->Hkv * a->Tq * (a->H / a->Hkv) : nullptr;
   p.dout = a->dout; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
   p.splits = 1;
   return p;
@@ -627,7 +701,7 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   q.dkv_share = ragged && q.dkv_splits > 1;
   if (q.dkv_share && q.dkv_grid < shared) q.dkv_grid = shared / a->Hkv * a->Hkv;
   const size_t rows = (size_t)probs * R;
-  q.fwd_ws = q.fwd_splits > 1 ? (size_t)q.fwd_splits * rows * (a->D + 1) * 4 + ATTN_SHARE_BYTES : 0;
+  q.fwd_ws = q.fwd_splits > 1 ? (size_t)q.fwd_splits * rows * (a->D + 2) * 4 + ATTN_SHARE_BYTES : 0;
   const size_t dq = q.dq_splits > 1 ? (size_t)q.dq_splits * rows * a->D * 4 : 0, dkv = q.dkv_splits > 1 ? (size_t)q.dkv_grid * 2 * wg * a->D * 4 : 0;
   q.bwd_ws = rows * 4 + 16 + ATTN_SHARE_BYTES + (dq > dkv ? dq : dkv);
   return q;
@@ -735,7 +809,7 @@ extern "C" int ttdg_attention_fwd(const ttdg_attention_t* a, ttdg_stream_t strea
   p.splits = q.fwd_splits;
   p.part_o = (float*)a->ws;
   p.part_lse = p.part_o + (size_t)q.fwd_splits * p.B * p.Hk * p.R * p.D;
-  p.share = q.fwd_share ? (int32_t*)(p.part_lse + (size_t)q.fwd_splits * p.B * p.Hk * p.R) : nullptr;
+  p.share = q.fwd_share ? (int32_t*)(p.part_lse + 2 * (size_t)q.fwd_splits * p.B * p.Hk * p.R) : nullptr;
   ATTN_DISPATCH(attn_fwd_launch, a, p, q, stream);
 }
 

@@ -515,7 +515,7 @@ def _attn_forward(q, k, v, scale, k_lens, key_mask, keep):
     if q.numel() == 0:
         return out, lo, lse
     if keep:
-        lse = torch.empty(q.shape[0] * q.shape[1] * q.shape[2], device=q.device, dtype=torch.float32)
+        lse = torch.empty(2 * q.shape[0] * q.shape[1] * q.shape[2], device=q.device, dtype=torch.float32)
         lo = None if q.dtype == torch.float32 else _like(q)
     _packed_call("ttdg_attention_fwd", _lib.ATTENTION, _attn_fields(q, k, v, scale, k_lens, key_mask, out, lo, lse),
                  _lib.load().ttdg_attention_fwd_workspace_bytes, q.device, q.shape + k.shape[1:3])
@@ -538,7 +538,7 @@ def _dense_grad(g):
 
 
 class CrossAttentionFn(torch.autograd.Function):
-    """cross_attention with gradients.  Saved: the inputs, the output (with what its rounding dropped) and one float per row."""
+    """cross_attention with gradients.  Saved: the inputs, the output (with what its rounding dropped) and two floats per row."""
 
     @staticmethod
     def forward(ctx, q, k, v, scale, k_lens, key_mask):
