@@ -8,6 +8,7 @@ import ctypes as C
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import call, check_f32, graphs, ptr, stream
@@ -537,6 +538,18 @@ def _dense_grad(g):
     return g.clone() if g.data_ptr() & 15 else g
 
 
+def _derived(*tensors):
+    """Whether autograd has to see a call: a gradient is asked for, or forward mode is on (a tensor with a tangent does not require a gradient;
+    the function then raises, as it has no forward-mode derivative, where the direct call would drop the tangent)."""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 class CrossAttentionFn(torch.autograd.Function):
     """cross_attention with gradients.  Saved: the inputs, the output (with what its rounding dropped) and two floats per row."""
 
@@ -573,7 +586,7 @@ def cross_attention(q, k, v, scale=None, k_lens=None, key_mask=None):
     ``k_lens`` (B,) int32 / int64: the keys j < k_lens[b] exist (values are clamped to 0 .. Tk); ``key_mask`` (B or 1, Tk) bool: the keys with
     True exist.  What stands at other keys - padding, infinities, NaN - never reaches a result; they get zero gradients, and a sample
     without any key gives zeros.  Returns (B, Tq, H, D), contiguous.  One query per sample (a decoding step) and few queries over many keys
-    take the same call: the keys are then split over the chip and joined.  No second derivatives."""
+    take the same call: the keys are then split over the chip and joined.  No second and no forward-mode derivatives."""
     _attn_check(q, k, v, k_lens, key_mask)
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
@@ -581,7 +594,7 @@ def cross_attention(q, k, v, scale=None, k_lens=None, key_mask=None):
     if k_lens is not None and (k_lens.dtype != torch.int32 or not k_lens.is_contiguous()):
         k_lens = k_lens.clamp(0, k.shape[1]).to(torch.int32).contiguous()          # (clamped first: int64 values may not fit)
     q, k, v = _dense_rows(q, q.shape[2] // k.shape[2]), _dense_rows(k), _dense_rows(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _derived(q, k, v):
         return CrossAttentionFn.apply(q, k, v, scale, k_lens, key_mask)
     with _on_device_of(q):
         return _attn_forward(q, k, v, scale, k_lens, key_mask, False)[0]
@@ -708,7 +721,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, freq=None, q_pos=None, k_pos=None, ep
     any strides (see cross_attention); weights (D,) float32.  ``freq`` (R / 2,) float64, see ``rope_frequencies``: the pairs of the first R
     channels - (i, i + R / 2), or (2 i, 2 i + 1) with ``interleaved`` - turn by position * freq[i]; None: no rotation.  Positions
     (B or 1, T) int32 / int64, or (B or 1, T, 2) for two coordinates: the first half of the pairs turns by the first one.  ``k_pos`` defaults
-    to ``q_pos``.  D and R are multiples of 8, D up to 256.  Returns (q', k'), contiguous; k' is None without k.  No second derivatives."""
+    to ``q_pos``.  D and R are multiples of 8, D up to 256.  Returns (q', k'), contiguous; k' is None without k.  No second and no
+    forward-mode derivatives."""
     if freq is not None and k is not None and k_pos is None:
         k_pos = q_pos
     axes = _qkn_check(q, k, q_weight, k_weight, freq, q_pos, k_pos)
@@ -721,7 +735,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, freq=None, q_pos=None, k_pos=None, ep
     q, k = _dense_rows(q), None if k is None else _dense_rows(k)
     q_weight, k_weight = _dense_weight(q_weight), None if k is None else _dense_weight(k_weight)
     args = (q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, float(eps), int(bool(interleaved)))
-    if torch.is_grad_enabled() and (q.requires_grad or q_weight.requires_grad or (k is not None and (k.requires_grad or k_weight.requires_grad))):
+    if _derived(q, k, q_weight, k_weight):
         return QkNormRopeFn.apply(*args)
     with _on_device_of(q):
         return _qkn_forward(*args)
