@@ -170,7 +170,7 @@ class TestLoader:
             slot = dicts.get("slot")
             items_ = disk.expand(dicts, self._disk.ring)
             stacked, masks, dicts = dicts["images"], dicts["masks"], items_
-        direct = slot is not None and self._disk.ring is not None and self._disk.ring.pinned      # the slot is page-locked: DMA straight from it
+        direct = slot is not None and self._disk.ring is not None and self._disk.ring.pinned      # the slot's twin is page-locked: DMA straight from it
         if dicts is None:
             dicts = dataset_dicts(self.name, lo, hi)
         items = [map_for_test(d, self.min_size, self.max_size, resize=not self.device_resize) for d in dicts]
@@ -200,8 +200,8 @@ class TestLoader:
                         n = len(it["dataset_dict"]["annotations"])
                         if n:
                             it["dataset_dict"]["device_masks"] = dm[k:k + n]
-                            if direct:       # the host masks are VIEWS of the ring slot, which goes back to a worker once this upload
-                                # has completed: nobody may read them later (evaluator fallbacks) - hand out the device copy instead
+                            if slot is not None:       # the host masks are VIEWS of the ring slot or its twin, which take another batch
+                                # once this upload has completed: nobody may read them later (evaluator fallbacks) - hand out the device copy
                                 for j, a in enumerate(it["dataset_dict"]["annotations"]):
                                     a["mask"] = dm[k + j]
                         k += n
@@ -210,7 +210,7 @@ class TestLoader:
                         anns = it["dataset_dict"]["annotations"]
                         if anns and "device_masks" not in it["dataset_dict"]:
                             it["dataset_dict"]["device_masks"] = torch.stack([a["mask"] for a in anns]).pin_memory().to(self.device, non_blocking=True)
-                if direct:
+                if slot is not None:
                     for it in items:
                         it["dataset_dict"].pop("image", None)      # a view of the ring slot as well; the batch carries the device image
                 ev = torch.cuda.Event()

@@ -65,18 +65,23 @@ class _Ring:
     """A ring of batch slots in SHARED memory: worker processes write a decoded batch straight into its slot - no per-batch
     shared-memory segment.  For the GPU every slot has a page-locked twin of the main process (allocated as such: registering the
     shared memory itself is refused on some hosts): ``expand`` copies an arrived slot there once and the DMA starts from it.
+    Where page-locked memory is refused the slots themselves are handed out (``pinned`` False) and uploaded through staging buffers.
     Allocated before the workers are forked, so they inherit the mapping.  Slot s is handed to a worker again only after the
-    upload that read its twin has completed (``wait``)."""
+    upload that read it or its twin has completed (``wait``)."""
 
     def __init__(self, slots, batch, image_shape, masks_per_image, mask_shape, register):
         self.slots, self.batch, self.mpi = slots, batch, masks_per_image
         self.images = torch.empty((slots, batch) + tuple(image_shape), dtype=torch.uint8).share_memory_()
         self.masks = torch.empty((slots, batch * max(1, masks_per_image)) + tuple(mask_shape), dtype=torch.bool).share_memory_()
         self.events = [None] * slots
-        self.pinned = bool(register and torch.cuda.is_available())
-        if self.pinned:
-            self.pin_images = torch.empty(self.images.shape, dtype=self.images.dtype, pin_memory=True)
-            self.pin_masks = torch.empty(self.masks.shape, dtype=self.masks.dtype, pin_memory=True)
+        self.pinned = False
+        if register and torch.cuda.is_available():
+            try:
+                self.pin_images = torch.empty(self.images.shape, dtype=self.images.dtype, pin_memory=True)
+                self.pin_masks = torch.empty(self.masks.shape, dtype=self.masks.dtype, pin_memory=True)
+                self.pinned = True
+            except RuntimeError:
+                self.pin_images = self.pin_masks = None          # both or none
 
     def batch_views(self, slot, nb):
         """Images and masks (None without any) of the ``nb`` items that have arrived in a slot."""
