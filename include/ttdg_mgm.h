@@ -202,6 +202,15 @@ size_t ttdg_attention_fwd_workspace_bytes(const ttdg_attention_t* a);
 size_t ttdg_attention_bwd_workspace_bytes(const ttdg_attention_t* a);
 int ttdg_attention_fwd(const ttdg_attention_t* a, ttdg_stream_t stream);
 int ttdg_attention_bwd(const ttdg_attention_t* a, ttdg_stream_t stream);
+/* The forms that the kernels of this call take (its sizes, types and whether k_lens is there decide; nothing is launched): */
+typedef struct {
+  int32_t few_rows;              /* one tile of rows per key head: wavefronts along the keys */
+  int32_t rows_per_wavefront;    /* of the forward: 32 or 64 */
+  int32_t shared_channels;       /* of the forward: wavefronts that share a row's channels */
+  int32_t fwd_parts, dq_parts, dkv_parts;              /* of the long axis */
+  int32_t fwd_operands, dkv_operands;                  /* bf16 operands that carry a probability into the second product */
+} ttdg_attention_forms_t;
+int ttdg_attention_forms(const ttdg_attention_t* a, ttdg_attention_forms_t* forms);
 
 /* ---- norm of queries and keys for each head with the position rotation in the same pass (the step between the projections of an
  *      attention layer, utils/attentions.py:72-74, and its scores) ---------------------------------------------------------------

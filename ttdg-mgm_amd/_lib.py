@@ -92,6 +92,11 @@ class Attention(C.Structure):
                 ("dq", C.c_void_p), ("dk", C.c_void_p), ("dv", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_size_t)]
 
 
+class AttentionForms(C.Structure):
+    """ttdg_attention_forms_t: the forms that the kernels of an attention call take."""
+    _fields_ = [(n, C.c_int32) for n in ("few_rows", "rows_per_wavefront", "shared_channels", "fwd_parts", "dq_parts", "dkv_parts", "fwd_operands", "dkv_operands")]
+
+
 class NormRopeSide(C.Structure):
     """ttdg_norm_rope_side_t: the queries or the keys of ttdg_qk_norm_rope_t."""
     _fields_ = [("x", C.c_void_p), ("sb", C.c_int64), ("st", C.c_int64), ("sh", C.c_int64), ("T", C.c_int32), ("H", C.c_int32), ("w", C.c_void_p),
@@ -143,6 +148,7 @@ SIGNATURES = {
     "ttdg_attention_bwd_workspace_bytes": (C.c_size_t, [_P]),
     "ttdg_attention_fwd": (C.c_int, [_P, _S]),
     "ttdg_attention_bwd": (C.c_int, [_P, _S]),
+    "ttdg_attention_forms": (C.c_int, [_P, _P]),
     "ttdg_qk_norm_rope_fwd": (C.c_int, [_P, _S]),
     "ttdg_qk_norm_rope_bwd_workspace_bytes": (C.c_size_t, [_P]),
     "ttdg_qk_norm_rope_bwd": (C.c_int, [_P, _S]),

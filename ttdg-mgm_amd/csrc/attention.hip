@@ -717,6 +717,17 @@ extern "C" size_t ttdg_attention_bwd_workspace_bytes(const ttdg_attention_t* a) 
   return a->B && a->Tq ? attn_planned(a).bwd_ws : 0;
 }
 
+extern "C" int ttdg_attention_forms(const ttdg_attention_t* a, ttdg_attention_forms_t* forms) {
+  TTDG_REQUIRE(a && forms, "attention_forms: null pointer");
+  if (int e = attn_check(a, "attention_forms")) return e;
+  *forms = ttdg_attention_forms_t{};
+  if (a->B == 0 || a->Tq == 0) return 0;
+  const attn_plan q = attn_planned(a);
+  const bool bf16 = a->dtype == TTDG_BF16;
+  *forms = {q.few, 32 * q.nb, q.fwd_cs, q.fwd_splits, q.dq_splits, q.dkv_splits, bf16 && q.fwd_two ? 2 : 1, bf16 && q.dkv_two ? 2 : 1};
+  return 0;
+}
+
 #define ATTN_LAUNCH(kernel, grid, threads, lds, stream, args)                              \
   do {                                                                                     \
     TTDG_ALLOW_LDS((kernel), (lds));                                                       \
