@@ -1,4 +1,5 @@
-"""Cross attention (csrc/attention.hip): every form of its bfloat16 kernels that a large call takes, at sizes with remainders in every axis.
+"""Cross attention (csrc/attention.hip): every form of its bfloat16 kernels that a large call takes, at sizes with remainders in every axis, and the
+accuracy that the second bfloat16 operand buys.
 
 The cases are many small problems, so that the call counts as large; that each of them takes the form it stands for is asked of the library
 without a GPU, and the results are held to the bounds of the other attention tests."""
@@ -62,3 +63,29 @@ def test_forms_of_other_calls():
 def test_large_calls(dev, name):
     shape, args, _ = LARGE[name]
     run_attention(dev, BF16, *shape, **args)
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_two_operands_leave_the_rounding_of_the_result(dev, D):
+    """dq and dk carry the score gradients in two bfloat16 operands (16 bits of significand), out and dv of small calls the probabilities too: beside
+    the rounding of the result, of mean square r^2, nothing of its order is left.  One operand would add a rounding of the same relative
+    size, independent of the first: (1 + 1)^(1/2) = 1.41 r.  Held is 1.2 r, 0.44 r^2 of such a rounding."""
+    from ttdg_mgm_amd import ops
+    B, Tq, Tk, H = 2, 120, 200, 2
+    assert forms_of(B, Tq, Tk, H, H, D, BF16, False)["fwd_operands"] == 2 and forms_of(B, Tq, Tk, H, H, D, BF16, False)["dkv_operands"] == 2
+    g = gen(7 + D, dev)
+    q, k, v, dout = normal(g, B, Tq, H, D, dtype=BF16, scale=2.0), normal(g, B, Tk, H, D, dtype=BF16), normal(g, B, Tk, H, D, dtype=BF16), normal(g, B, Tq, H, D, dtype=BF16)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = ops.cross_attention(*leaves)
+    got = (out.detach(),) + torch.autograd.grad(out, leaves, dout)
+    Q, K, V, dO = (t.detach().double().transpose(1, 2).contiguous() for t in (q, k, v, dout))
+    s = D ** -0.5
+    P = torch.softmax(s * torch.matmul(Q, K.transpose(2, 3).contiguous()), -1)
+    O = torch.matmul(P, V)
+    dS = P * (torch.matmul(dO, V.transpose(2, 3).contiguous()) - (dO * O).sum(-1, keepdim=True))
+    want = (O, s * torch.matmul(dS, K), s * torch.matmul(dS.transpose(2, 3).contiguous(), Q), torch.matmul(P.transpose(2, 3).contiguous(), dO))
+    for name, a, b in zip(("out", "dq", "dk", "dv"), got, want):
+        b = b.transpose(1, 2)
+        own = float((b.to(BF16).double() - b).norm())
+        assert float((a.double() - b).norm()) <= 1.2 * own, (name, float((a.double() - b).norm()) / own)
