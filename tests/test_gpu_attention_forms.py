@@ -89,3 +89,12 @@ def test_two_operands_leave_the_rounding_of_the_result(dev, D):
         b = b.transpose(1, 2)
         own = float((b.to(BF16).double() - b).norm())
         assert float((a.double() - b).norm()) <= 1.2 * own, (name, float((a.double() - b).norm()) / own)
+
+
+@gpu
+@pytest.mark.parametrize("eps", [-1.0, -1e-30, float("nan")])
+def test_norm_rope_refuses_eps(dev, eps):
+    from ttdg_mgm_amd import ops
+    q, w = torch.zeros(2, 3, 4, 64, device=dev), torch.ones(64, device=dev)
+    with pytest.raises(ValueError, match="eps"):
+        ops.qk_norm_rope(q, q, w, w, eps=eps)
