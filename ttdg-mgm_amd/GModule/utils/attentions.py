@@ -52,6 +52,8 @@ class MultiHeadAttention(nn.Module):
             raise ValueError("attend: query (B, n, %d) and states (B, m, %d) or (m, %d), got %s and %s" %
                              (self.linear_q.in_features, self.linear_k.in_features, self.linear_k.in_features, tuple(query.shape), tuple(states.shape)))
         B, H, D = query.shape[0], self.num_heads, self.dim_per_head
+        if H * D != self.linear_final.in_features:                       # (as in the reference, whose output projection refuses it)
+            raise ValueError("attend: %d channels are no %d heads" % (self.linear_final.in_features, H))
         if states.dim() == 3 and states.shape[0] != B:
             raise ValueError("attend: %d samples of queries, %d of states" % (B, states.shape[0]))
 
