@@ -56,6 +56,13 @@ class MultiHeadAttention(nn.Module):
             raise ValueError("attend: %d channels are no %d heads" % (self.linear_final.in_features, H))
         if states.dim() == 3 and states.shape[0] != B:
             raise ValueError("attend: %d samples of queries, %d of states" % (B, states.shape[0]))
+        if not query.device == states.device == self.linear_q.weight.device:
+            raise ValueError("attend: queries on %s, states on %s, the layer on %s" % (query.device, states.device, self.linear_q.weight.device))
+        with ops.on_device_of(query):                                    # (the projections' kernels too, whatever device is current)
+            return self._attend(query, states, state_lens, state_mask)
+
+    def _attend(self, query, states, state_lens, state_mask):
+        B, H, D = query.shape[0], self.num_heads, self.dim_per_head
 
         def lin(x, layer):
             if x.numel() == 0:                                           # (the products take no empty operands)

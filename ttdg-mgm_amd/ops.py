@@ -426,9 +426,9 @@ class _NoDevice:
 _NO_DEVICE = _NoDevice()
 
 
-def _on_device_of(t):
+def on_device_of(t):
     """The kernels run on the current stream of the device the tensors live on, whatever device is current."""
-    return _NO_DEVICE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+    return _NO_DEVICE if not t.is_cuda or t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def _packed_call(name, packer, fields, ws_query, device, meta):
@@ -555,7 +555,7 @@ class CrossAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, scale, k_lens, key_mask):
-        with _on_device_of(q):
+        with on_device_of(q):
             out, lo, lse = _attn_forward(q, k, v, scale, k_lens, key_mask, True)
         ctx.save_for_backward(q, k, v, out, lo, lse, k_lens, key_mask)
         ctx.scale = scale
@@ -568,7 +568,7 @@ class CrossAttentionFn(torch.autograd.Function):
         kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         if q.numel() == 0:
             return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), None, None, None
-        with _on_device_of(q):
+        with on_device_of(q):
             dq = _like(q)
             dk, dv = (_like(k), _like(k)) if kv else (None, None)
             dout = _dense_grad(dout)
@@ -596,7 +596,7 @@ def cross_attention(q, k, v, scale=None, k_lens=None, key_mask=None):
     q, k, v = _dense_rows(q, q.shape[2] // k.shape[2]), _dense_rows(k), _dense_rows(v)
     if _derived(q, k, v):
         return CrossAttentionFn.apply(q, k, v, scale, k_lens, key_mask)
-    with _on_device_of(q):
+    with on_device_of(q):
         return _attn_forward(q, k, v, scale, k_lens, key_mask, False)[0]
 
 
@@ -694,7 +694,7 @@ class QkNormRopeFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(q, k, q_weight, k_weight, freq, q_pos, k_pos)
         ctx.args = (axes, eps, interleaved)
-        with _on_device_of(q):
+        with on_device_of(q):
             return _qkn_forward(q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, eps, interleaved)
 
     @staticmethod
@@ -702,7 +702,7 @@ class QkNormRopeFn(torch.autograd.Function):
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, freq, q_pos, k_pos = ctx.saved_tensors
         dq = dk = dwq = dwk = None
-        with _on_device_of(q):
+        with on_device_of(q):
             gq = _dense_grad(gq) if gq is not None else torch.zeros(q.shape, device=q.device, dtype=q.dtype)     # (an output nobody used)
             dq, dwq = _like(q), _like(q_weight)
             if k is not None:
@@ -737,7 +737,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, freq=None, q_pos=None, k_pos=None, ep
     args = (q, k, q_weight, k_weight, freq, q_pos, k_pos, axes, float(eps), int(bool(interleaved)))
     if _derived(q, k, q_weight, k_weight):
         return QkNormRopeFn.apply(*args)
-    with _on_device_of(q):
+    with on_device_of(q):
         return _qkn_forward(*args)
 
 
