@@ -44,3 +44,14 @@ def test_a_batch_is_copied_to_the_twin_of_its_slot(monkeypatch):
     r.images[2].fill_(9)
     r.masks[2].fill_(False)
     assert int(images.min()) == int(images.max()) == 7 and bool(masks.all())
+
+
+def test_a_slot_is_copied_without_waking_other_threads(monkeypatch):
+    """torch's copy_ shares 3 MB out to a thread per CPU; beside busy workers that took milliseconds a batch, and the streamed rate a quarter."""
+    r, _ = ring_of(monkeypatch)
+
+    def refused(*a, **k):
+        raise AssertionError("a copy over several threads")
+
+    monkeypatch.setattr(torch.Tensor, "copy_", refused)
+    assert r.batch_views(0, 2)[0].shape == (2, 3, 4, 5)

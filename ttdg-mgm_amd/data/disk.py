@@ -61,6 +61,14 @@ class DiskDataset(torch.utils.data.Dataset):
         return d
 
 
+def _copy(to, of):
+    """Host memory to host memory on the calling thread alone : 0.1 ms for 3 MB.  torch's copy_ wakes a thread
+    per CPU, which beside the busy workers took 1.2 ms a tensor in the loader and more in the adaptation loop: with it the streamed input ran at
+    84 of 112.6 images/s, with this at 104.6 (20 batches of four 512 x 512 images, two runs each in turn)."""
+    np.copyto(to.numpy(), of.numpy())
+    return to
+
+
 class _Ring:
     """A ring of batch slots in SHARED memory: worker processes write a decoded batch straight into its slot - no per-batch
     shared-memory segment.  For the GPU every slot has a page-locked twin of the main process (allocated as such: registering the
@@ -87,8 +95,8 @@ class _Ring:
         """Images and masks (None without any) of the ``nb`` items that have arrived in a slot."""
         images, masks = self.images[slot, :nb], self.masks[slot, :nb * self.mpi] if self.mpi else None
         if self.pinned:
-            images = self.pin_images[slot, :nb].copy_(images)
-            masks = None if masks is None else self.pin_masks[slot, :nb * self.mpi].copy_(masks)
+            images = _copy(self.pin_images[slot, :nb], images)
+            masks = None if masks is None else _copy(self.pin_masks[slot, :nb * self.mpi], masks)
         return images, masks
 
     def wait(self, slot):
