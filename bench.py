@@ -705,8 +705,9 @@ def gpu_main(args, rank, world, local):
     device = torch.device("cuda", local)
     if args.miopen_search:
         torch.backends.cudnn.benchmark = True
-    import __graft_entry__
-    if rank == 0:
+    from ttdg_mgm_amd import _lib
+    if rank == 0 and not os.path.exists(_lib.LIB_PATH):
+        import __graft_entry__
         __graft_entry__.build()
     if world > 1:
         dist.barrier()

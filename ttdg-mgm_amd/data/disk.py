@@ -62,7 +62,7 @@ class DiskDataset(torch.utils.data.Dataset):
 
 
 def _copy(to, of):
-    """Host memory to host memory on the calling thread alone : 0.1 ms for 3 MB.  torch's copy_ wakes a thread
+    """Host memory to host memory on the calling thread alone: 0.1 ms for 3 MB.  torch's copy_ wakes a thread
     per CPU, which beside the busy workers took 1.2 ms a tensor in the loader and more in the adaptation loop: with it the streamed input ran at
     84 of 112.6 images/s, with this at 104.6 (20 batches of four 512 x 512 images, two runs each in turn)."""
     np.copyto(to.numpy(), of.numpy())
