@@ -64,6 +64,16 @@ def test_large_calls(dev, name):
     shape, args, _ = LARGE[name]
     run_attention(dev, BF16, *shape, **args)
 
+@gpu
+@pytest.mark.parametrize("dtype,shape", [(F32, (2, 1, 9001, 8, 2, 128)), (BF16, (1, 1, 9001, 8, 4, 256)), (BF16, (2, 2, 5000, 8, 8, 64)), (F32, (2, 3, 7000, 4, 4, 40))])
+def test_gradients_of_few_rows_over_many_keys(dev, dtype, shape):
+    """A workgroup of dq is one wavefront there; two (four with up to 64 bfloat16 channels) of them fit on a CU, and the parts of the key axis fill
+    these places."""
+    B, Hk = shape[0], shape[4]
+    assert B * Hk * forms_of(*shape, dtype, False)["dq_parts"] > 256
+    run_attention(dev, dtype, *shape)
+    run_attention(dev, dtype, *shape, lens=[shape[2] - 900 * b for b in range(B)], mask=0.1)
+
 
 @gpu
 @pytest.mark.parametrize("D", [64, 128, 256])

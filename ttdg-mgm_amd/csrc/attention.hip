@@ -678,7 +678,11 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
     const int splits = attn_splits(probs * q.row_tiles, kt, shared, 2 * prod_us, q_bytes, &us2);
     if (us2 < us) { q.fwd_cs = 2; q.fwd_tiles = q.row_tiles; q.fwd_splits = splits; }
   }
-  q.dq_splits = attn_splits(probs * q.row_tiles, kt, shared, 3 * prod_us, q_bytes);
+  // few rows: workgroups of one wavefront, as many per CU as their two stages of LDS leave room for (one token of 4 x 16 heads x 128 over 20000
+  // keys, float32: 16 parts 272 us, 32 parts 148, 64 parts 155; 8 heads x 256 over 30000, bfloat16: 31 parts 88, 62 parts 55, 124 parts 67;
+  // + 4, 6 and 9 us for the sums.  Elsewhere the estimate's parts are the best of half, twice and four times as many, or within 2 us)
+  const int dq_slots = q.few ? (q.dp == 64 && !f32 ? 1024 : 512) : shared;
+  q.dq_splits = attn_splits(probs * q.row_tiles, kt, dq_slots, 3 * prod_us, q_bytes);
   q.key_tiles = (a->Tk + wg - 1) / wg;
   const int qt = (int)((R + bn - 1) / bn);
   q.dkv_splits = attn_splits(probs * q.key_tiles, qt, shared, 4 * prod_us, kv_bytes);
