@@ -758,9 +758,10 @@ static int attn_fwd_launch(const attn_args& p, const attn_plan& q, ttdg_stream_t
   else if constexpr (sizeof(T) == 2 && DP == 128) ATTN_LAUNCH((attn_fwd_kernel<T, DP, BN, WM, 2, 1, 1, 1>), grid, 64 * WM, lds, stream, p);
   if (p.splits > 1) {
     const int64_t rows = (int64_t)p.B * p.Hk * p.R;
-    // four wavefronts per row from 32 parts on; with ragged samples, the longest of which may have several times the parts there are on average,
-    // from 12 on while the rows are few (1024 rows of 256 channels: 8.5 -> 5.1 us; 4096 rows of 64: 5.7 -> 8.6)
-    if (p.splits > (p.share && rows <= 2048 ? 12 : 32)) ATTN_LAUNCH((attn_combine_kernel<T, 4>), rows, 256, 0, stream, p);
+    // Four wavefronts per row where the rows alone do not fill the chip and the parts are many (one and four wavefronts, us: 32 rows of 105 parts
+    // 9.2 / 5.5, 256 of 125 10.8 / 6.5, 512 of 63 6.1 / 5.1, 128 of 21 5.6 / 4.1, 1024 of 48 5.5 / 5.2; up to 16 parts the same within 0.1;
+    // 2048 rows 5.4 / 6.0, 4096 5.9 / 9.4, 8192 6.2 / 14.1, whatever the parts, channels and lengths)
+    if (rows <= 1024 && p.splits > 16) ATTN_LAUNCH((attn_combine_kernel<T, 4>), rows, 256, 0, stream, p);
     else ATTN_LAUNCH((attn_combine_kernel<T, 1>), (rows + 3) / 4, 256, 0, stream, p);
   }
   return 0;
