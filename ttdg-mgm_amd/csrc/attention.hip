@@ -388,37 +388,32 @@ __global__ ATTN_WAVES(64 * WM, (WM == 1 ? 1 : attn_waves<T, DP, 3>())) void attn
     if (t + 1 < t1) live_next = in.issue(attn_smem + ((t + 1 - t0) & 1) * stream_t::STAGE);
     if (live == 0) continue;
     constexpr int PRE = DP == 256 && sizeof(T) == 2 ? 2 : 0;      // one wavefront per SIMD: nobody else hides the LDS
-    // blocks of 32 keys at a time: two chains of products with 128 channels; one with 64, where two cost the third wavefront per SIMD its
-    // registers (323 and 296 us)
-    constexpr int KK = DP == 64 && sizeof(T) == 2 ? 1 : BN / 32;
+    constexpr int KK = BN / 32;          // blocks of 32 keys, all at a time: so many independent chains of products
     static_assert(CS == 1 || BN == 32, "one pair of exchanges between two barriers");
+    f32x16 s[KK][1], dp[KK][1];
 #pragma unroll
-    for (int k0 = 0; k0 < BN; k0 += 32 * KK) {
-      f32x16 s[KK][1], dp[KK][1];
+    for (int k = 0; k < KK; ++k) {
+      s[k][0] = stream_t::start(stage, 32 * k, live, h);
+      dp[k][0] = start;
+    }
+    tile_t::template row_product<KK, 1, PRE>(s, stage + cs * DC * tile_t::ES, 0, &qf, l32, h);
+    tile_t::template row_product<KK, 1, PRE>(dp, stage + stream_t::TB + cs * DC * tile_t::ES, 0, &gf, l32, h);
+    if constexpr (CS > 1) {
+      attn_exchange<false>(s[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
+      attn_exchange<true>(dp[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
+    }
+    if (some_far) {
 #pragma unroll
-      for (int k = 0; k < KK; ++k) {
-        s[k][0] = stream_t::start(stage, k0 + 32 * k, live, h);
-        dp[k][0] = start;
-      }
-      tile_t::template row_product<KK, 1, PRE>(s, stage + cs * DC * tile_t::ES, k0, &qf, l32, h);
-      tile_t::template row_product<KK, 1, PRE>(dp, stage + stream_t::TB + cs * DC * tile_t::ES, k0, &gf, l32, h);
-      if constexpr (CS > 1) {
-        attn_exchange<false>(s[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
-        attn_exchange<true>(dp[0][0], ex + wave * 1024, ex + (wave ^ 1) * 1024, lane);
-      }
-      if (some_far) {
+      for (int k = 0; k < KK; ++k)
 #pragma unroll
-        for (int k = 0; k < KK; ++k)
+        for (int e = 0; e < 16; ++e) s[k][0][e] -= far;
+    }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[k][0][e] -= far;
-      }
+    for (int k = 0; k < KK; ++k) {
 #pragma unroll
-      for (int k = 0; k < KK; ++k) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[k][0][e] = fast_exp2(fmaf(s[k][0][e], p.scale_log2, -lse)) * dp[k][0][e];
-        const auto ds = tile_t::template pack<attn_parts<T>(true)>(s[k][0]);
-        tile_t::template col_product<1, attn_parts<T>(true)>(&acc, stage + cs * DC * tile_t::ES, k0 + 32 * k, &ds, lane);
-      }
+      for (int e = 0; e < 16; ++e) s[k][0][e] = fast_exp2(fmaf(s[k][0][e], p.scale_log2, -lse)) * dp[k][0][e];
+      const auto ds = tile_t::template pack<attn_parts<T>(true)>(s[k][0]);
+      tile_t::template col_product<1, attn_parts<T>(true)>(&acc, stage + cs * DC * tile_t::ES, 32 * k, &ds, lane);
     }
   }
   if (row >= p.R) return;
