@@ -902,8 +902,8 @@ def gpu_main(args, rank, world, local):
             return sloader
         ab["loader_inclusive"] = short(
             timed_pass(cfg, model, init_state, batches, local_dicts, name, K, W, args, world, device, tf, loader_factory=stream),
-            "timed batches stream from local storage through %d worker processes that write each batch into a shared page-locked ring; DMA of the "
-            "raw %dx%d uint8 batch and its ground-truth masks from the ring slot, resize to the test size ON THE DEVICE, staged one batch ahead; "
+            "timed batches stream from local storage through %d worker processes that write each batch into a shared ring; one host copy into the "
+            "slot's page-locked twin, DMA of the raw %dx%d uint8 batch and its ground-truth masks from there, resize to the test size ON THE DEVICE, staged one batch ahead; "
             "in both passes (rendering the stream to disk and starting the workers are outside the timed region)"
             % (cfg.DATALOADER.NUM_WORKERS, args.size, args.size))
         ab["loader_inclusive"]["fraction_of_resident"] = ab["loader_inclusive"]["value"] / (K * B / main["elapsed"])

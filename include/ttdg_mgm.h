@@ -173,8 +173,9 @@ int ttdg_mha_adjacency(const float* q, const float* k, int d, ttdg_graphs_t gr, 
  * != 0 (bytes; NULL: all).  What stands at keys that do not exist never reaches a result, infinities and NaN included; a sample without
  * any key gives zeros and no gradient.
  *     out[b,i,h,:] = sum_j softmax_j(scale * q[b,i,h,:] . k[b,j,h',:]) v[b,j,h',:]        out (B, Tq, H, D) contiguous
- * dtype TTDG_F32: products in fp32 on the matrix unit; TTDG_BF16: products of bf16 with fp32 sums, probabilities (and, backward, the
- * score gradients) rounded to bf16 between the two products.  Softmax statistics are fp32.
+ * dtype TTDG_F32: products in fp32 on the matrix unit; TTDG_BF16: products of bf16 with fp32 sums; between the two products the score gradients
+ * are carried in two bf16 operands (16 bits of significand), the probabilities in two in small calls and in one in large ones, where out and
+ * dv have up to 1.45 times the error of their own rounding (ttdg_attention_forms says which).  Softmax statistics are fp32.
  * Scores may be of any finite size; the sums before their division - the keys' number times 2^8 times the largest |v| - have to be finite.
  * For a backward pass later: lse (2, B, Hkv, Tq * H / Hkv) fp32 (log2 of the sums, and the score they are relative to) and, bf16 only, out_lo (like out: what the rounding of
  * out dropped) are written when not NULL, and the backward reads q, k, v, out, out_lo, lse, dout (contiguous like out) and writes dq like
@@ -219,7 +220,7 @@ int ttdg_attention_forms(const ttdg_attention_t* a, ttdg_attention_forms_t* form
  *     n = x / sqrt(mean(x^2) + eps),  u = n * w,  y = u with the pairs of its first R channels turned by pos[axis] * freq[pair]
  * Pair i of R / 2: channels (i, i + R / 2), or (2 i, 2 i + 1) when interleaved; axis i / (R / 2 / axes) of pos (B, T, axes), int32 or
  * (pos64) int64, element strides p_sb / p_st / p_sa; freq (R / 2) fp64 on the device; angles are formed and reduced in 64 bits.
- * R = 0: no rotation (pos / freq may be NULL).  D and R multiples of 8, D <= 256.
+ * R = 0: no rotation (pos / freq may be NULL).  D and R multiples of 8, D <= 256.  Squares are summed in fp32: |x| up to 1e18.
  * bwd reads x, w, pos, dy and writes dx and dw of both sides (dw is zeros for a side without rows); ws: at least
  * ttdg_qk_norm_rope_bwd_workspace_bytes(a), 16-byte aligned.  No atomics. */
 typedef struct {

@@ -329,8 +329,8 @@ __device__ __forceinline__ void affinity_bwd_body(const float* __restrict__ X, c
       for (int a = 0; a < 4; ++a) {
         // relu'(x + y) = [x > -y] as an exact 0/1 step WITHOUT a compare (no VCC round trip between v_cmp and
         // v_cndmask): step = clamp(clamp((x - (-y)) * 2^126) * 2^126), the clamps being the free [0,1] output modifier
-        // of the packed multiply; positive differences down to the smallest denormal saturate to 1, the rest to 0.
-        // acc += step * d is then bit-identical to the select-add, in 4 packed instructions per two k.
+        // of the multiplies; positive differences down to the smallest denormal saturate to 1, the rest to 0.
+        // acc += step * d is then bit-identical to the select-add, in four instructions per (i, j, k).
         acc2[a][0] = __builtin_elementwise_fma(relu_step2(x2[a][0] - y01), (f32x2){dv[a], dv[a]}, acc2[a][0]);
         acc2[a][1] = __builtin_elementwise_fma(relu_step2(x2[a][1] - y23), (f32x2){dv[a], dv[a]}, acc2[a][1]);
       }

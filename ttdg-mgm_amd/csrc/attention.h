@@ -260,6 +260,8 @@ struct attn_keys {
 
 // position of 16-byte chunk c of a tile row.  Eight consecutive rows XOR with eight different numbers (row reads: eight lanes of
 // consecutive rows read the same c), and the four rows of a transposing read's 16-lane group land in four different 32-byte windows.
+// (The counters still call 25 % of the LDS' busy cycles conflicts with rows of 128 bytes, 40 to 50 % with longer ones; it is busy 25 to 45 % of
+// the time in large calls.)
 __device__ __forceinline__ int attn_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
 
 // DP channels of tiles whose rows have RD (a wavefront may work on a part of the channels)
@@ -523,8 +525,8 @@ struct attn_loader {
 // The key / value tiles of a problem, in stages of LDS: k tile, v tile, and for tiles with absent keys the scores' starting values (0, or
 // -infinity where no key exists: the scores' sums start from them, so masking costs no vector instruction).
 // LEAN: the lanes' offsets are made anew for every tile; kept, they are the registers that the kernel with 64 rows per wavefront lacks, and
-// reloading one of them from scratch waits for the LDS-DMA just started (16 x 2048 rows
-// over 4096 keys, 8 heads, with 64 rows per wavefront: 632 -> 596 us).
+// reloading one of them from scratch waits for the LDS-DMA just started (both in one run: 16 x 2048 rows over 4096 keys, 8 heads, with 64
+// rows per wavefront 754 -> 712 us; 4 x 4096 rows over 8191 keys, 16 heads, 1188 -> 1131).
 template <typename T, int DP, int BN, int WM, bool LEAN = false>
 struct attn_stream {
   typedef attn_tile<T, DP> tile_t;

@@ -15,7 +15,7 @@
 // (32-bit).  One body serves both types: bfloat16 through v_mfma_f32_32x32x16_bf16, float32 through v_mfma_f32_32x32x2_f32 (exact products).
 //
 // Tiles go memory -> LDS by LDS-DMA, double-buffered, in 16-byte chunks whose position in the row is XORed with a function of the row
-// (conflict-free for row reads and for the transposing reads).  A chunk that must not be read - a row behind the last key, a masked
+// (attn_swz: neighbouring rows in different places, for row reads and for the transposing reads).  A chunk that must not be read - a row behind the last key, a masked
 // key, a channel behind D - gets an offset behind the end of the buffer resource: the hardware then stores zeros, so whatever stands in
 // masked places (infinities, NaN) never reaches a product.  The resource starts at the tile, so 32-bit offsets are relative to the tile
 // and a cache may be longer than 4 GiB.
@@ -23,9 +23,10 @@
 
 // float32 with 256 channels: the operands and sums of 32 rows times 256 channels overflow a wavefront's registers and take 14 us per tile of
 // 32 keys, so two wavefronts share 32 rows, each with half the channels: half of every score's sum (exchanged through LDS) and half of
-// the output.  dk / dv of large calls 96 -> 118 TFLOP/s, dq 104 -> 111; 8 x 256 rows over 794 keys, forward + backward, 207 -> 143 us.  The
-// forward holds one set of sums only: there large calls run at 125 TFLOP/s without the exchange and at 108 with it, while 8 x 256 rows take
-// 31 us with it and 40 without; attn_planned compares the two.  bfloat16 fits without (with the exchange: 640 -> 560 TFLOP/s).
+// the output (both sides in one run: dq of 8 x 2048 rows over 4096 keys, 8 heads, 8400 -> 7500 us, dk / dv 9450 -> 9546; 8 x 256 rows over 794
+// ragged keys, forward + backward, 184 -> 134 us).  The forward holds one set of sums only: the large call takes 4330 us without the exchange and
+// 5180 with it, 2048 rows over 4096 keys 644 and 724, 8 x 256 rows 45 and 36 (with the join); attn_planned compares the two.  bfloat16 fits
+// without (with the exchange: 640 -> 560 TFLOP/s).
 constexpr int attn_cs(int dp, bool f32) { return dp == 256 && f32 ? 2 : 1; }
 constexpr int attn_rows_wg(int dp, bool f32) { return 128 / attn_cs(dp, f32); }      // rows, or keys, of a workgroup of four wavefronts
 constexpr int attn_exchange_bytes(int dp, bool f32) { return attn_cs(dp, f32) > 1 ? 4 * 4096 : 0; }
@@ -40,10 +41,11 @@ constexpr int attn_waves() {
 
 // How many bfloat16 operands carry a probability or a score gradient into the second product (PARTS of the kernels, attn_tile::pack).  With
 // one, the rounding of p (or ds) adds an error of the size of the result's own rounding.  ds takes two everywhere: half of its terms
-// cancel in dq and dk, which then had 1.5 times the error of their own rounding (1.04 with two; backward of 4 x 2047 x 2500 x 16 heads x
-// 128: 532 -> 583 us).  p takes two where a launch leaves the chip room - few rows, or workgroups for half of the slots at most: few values are
-// averaged there, and the extra products hide behind the loads (one token over 53294 keys: 20.8 and 21.3 us) - and one in large calls
-// (8 x 1000 x 12 heads x 64 over 1500 keys: forward 65 and 85 us, dk / dv 111 and 137), where out and dv have 1.2 to 1.45 times their own rounding's error.
+// cancel in dq and dk, which then had 1.5 times the error of their own rounding (1.04 with two; dq and dk / dv of 4 x 2047 rows over 2500 keys, 16
+// heads x 128: 268 + 473 us with one, 324 + 535 with two; of 8 x 1000 over 1500, 12 heads x 64: 79 + 104 and 97 + 122).  p takes two where a
+// launch leaves the chip room - few rows, or workgroups for half of the slots at most: few values are averaged there, and the extra products
+// hide behind the loads (one token over 53294 keys: 15.2 and 15.6 us) - and one in large calls (the two above: forward 217 and 283 us, dk / dv
+// 534 and 608; 69 and 91, 122 and 140), where out and dv have 1.2 to 1.45 times their own rounding's error.
 template <typename T>
 constexpr int attn_parts(bool two) { return sizeof(T) == 2 && two ? 2 : 1; }
 
@@ -252,7 +254,7 @@ __global__ ATTN_WAVES(64 * WM * KW, (WM == 1 ? 1 : DP == 256 && sizeof(T) == 2 ?
 // Joins the splits of a row: o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max), the logs taken from the largest far of the parts on (a part
 // with a smaller far is exactly as far below as the difference says, or has no weight at all).  W wavefronts per row: a lane owns four channels and
 // every n-th split (n = 64 W / lanes per row), loads several splits ahead, and the lanes' sums meet by shuffles and, for W > 1, in LDS.
-// Bound by latency: with one wavefront walking over 256 splits a row took 186 us, with four 8 us (16 heads, 53294 keys, 128 channels).
+// Bound by latency: 32 rows of 105 parts and 128 channels take 9.2 us with one wavefront per row and 5.5 with four.
 template <typename T, int W>
 __global__ __launch_bounds__(256) void attn_combine_kernel(attn_args p) {
   __shared__ float red[W > 1 ? W * 260 : 1];
@@ -613,8 +615,9 @@ static attn_args attn_make(const ttdg_attention_t* a) {
 // How many workgroups share one (problem, tile): the long axis (`units` tiles of it) is split into s parts when that shortens the estimated
 // time in microseconds: `tile_us` per tile with all of the chip's `slots` taken (where several workgroups fit on a CU, one alone there runs up to
 // twice as fast, so the rounds are not counted in full), 6 us per workgroup (first loads, last stores), and for the join a launch and the parts written and read once (`part_bytes` each)
-// at 5 TB/s.  Measured both ways: dk / dv of 4 x 2047 x 16 heads over 2500 keys (320 workgroups for 512 slots) 465 us unsplit, 341 in two
-// parts, 402 in three; of 8 x 1000 x 12 heads x 64 over 1500 keys (1152 for 768) 111 us unsplit, 137 in two.
+// at 5 TB/s.  Measured both ways: dk / dv of 8 x 256 rows over 794 ragged keys, float32, 256 channels (104 workgroups for 256 slots) 83 us
+// unsplit, 43 + 9 for the sums in two parts; of 8 x 1000 x 12 heads x 64 over 1500 keys (1152 for 768) 122 unsplit, 144 + 34 in two; of 4 x 2047
+// rows x 16 heads over 4 x 2500 keys (320 for 512) 570 unsplit, 539 + 18 in two, 449 + 24 in three, where the estimate says two.
 static int attn_splits(int64_t blocks, int units, int slots, double tile_us, double part_bytes, double* estimate = nullptr) {
   int best = 1;
   double least = 0;
@@ -653,10 +656,12 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   const int shared = q.dp == 256 || (q.dp == 128 && f32) ? 256 : q.dp == 128 || f32 ? 512 : 768;
   q.slots = shared;
   const int wg = attn_rows_wg(q.dp, f32);
+  // One wavefront's 32 rows hold all.  Two such tiles of 33 to 64 rows would read the keys twice: 2 x 48 rows over 53294 keys, one key head x 128,
+  // bfloat16, take 19 us in the form for many rows (32 rows: 16), float32 with 64 channels 43 (20), with 128 channels 64 rows 77 (64).
   q.few = R <= 32 && !(f32 && q.dp == 256);
   q.row_tiles = q.few ? 1 : (int)((R + wg - 1) / wg);
-  // 64 rows per wavefront where the workgroups still go round twice: 16 x 2048 rows over 4096 keys, 8 heads, 632 -> 596 us; with fewer workgroups
-  // the rounds decide (batch 4: 163 -> 202 us, 8: 318 -> 304, 9: 395 -> 431).  With 64 channels 361 -> 378 us.
+  // 64 rows per wavefront where the workgroups still go round twice: 16 x 2048 rows over 4096 keys, 8 heads, 654 -> 618 us; with fewer workgroups
+  // the rounds decide (batch 4: 167 -> 173 us and a join of 32, 8: 360 -> 348, 9: 406 -> 443).  With 64 channels 361 -> 378 us.
   q.nb = !f32 && q.dp == 128 && !q.few && probs * ((R + 255) / 256) >= 1024 ? 2 : 1;
   const int kt = (a->Tk + bn - 1) / bn, kt32 = (a->Tk + 31) / 32, kw = attn_kw(q.dp, f32);
   // a tile's time at 800 (bf16) / 110 TFLOP/s (fp32) for the products of a full chip; few rows: its bytes at 20 GB/s per CU
@@ -685,8 +690,8 @@ static attn_plan attn_planned(const ttdg_attention_t* a) {
   q.dkv_two = 2 * probs * q.key_tiles * q.dkv_splits <= shared;
   // Ragged samples: only the device knows their lengths, and the kernels divide by them (attn_place) where the workgroups run all at once.  What
   // the host says is how many parts there may be: as many as the chip has slots for.  Forward and backward of 8 x 256 rows over
-  // up to 794 keys, float32, 256 channels: 147 -> 135 us with 447 to 794 keys, 137 -> 86 us with one sample of 794 and seven of 40 to 200; what
-  // the division costs when all are alike: 2 us of 78 (8 x 64 rows over 128 keys).
+  // up to 794 keys, float32, 256 channels: 152 -> 134 us with 447 to 794 keys, 140 -> 88 us with one sample of 794 and seven of 40 to 160; what
+  // the division costs when all are alike: 1.6 us of 79 (8 x 64 rows over 128 keys).
   const bool ragged = a->k_lens && a->B > 1 && a->B <= 64;
   const auto share = [&](int& splits, int64_t blocks) {
     if (!ragged || q.few || splits < 2 || blocks * splits > shared) return 0;

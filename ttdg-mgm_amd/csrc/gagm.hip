@@ -139,7 +139,7 @@ __device__ __forceinline__ void sk_wave_project(const float* Vb, int n, float sc
 // 32 x 32 problem after dummy rows; every lane owns 16 entries in BOTH layouts (row = lane & 31, half = lane >> 5), the
 // dummy row lives in the free row slot n (its column-layout copy carries +log2(multiplicity)), so both sweeps are the
 // same 16-element loop with no special cases.  A single wavefront issues ~1 instruction per 4-5 cycles, so the loop is
-// written for instruction count: packed fp32 subtracts/adds, and NO max pass - after any sweep y = L - f - g <= 0, so
+// written for instruction count: pairs without a dependence between them, and NO max pass - after any sweep y = L - f - g <= 0, so
 // the previous potential is a valid stabiliser (exp2 arguments <= 0, sums in (0, 32]); the exact two-pass form is used
 // for the first sweep and whenever a sum underflows (< 2^-60).
 typedef float f32x2 __attribute__((ext_vector_type(2)));

@@ -7,8 +7,8 @@
 // lines one at a time through LDS (two passes and two dependent shuffle reductions per line, a barrier per sweep): 10 + 104 us
 // for the ten 20..40-node pairs of a TTA step.  Here ONE workgroup per pair keeps the block on the CU from the P / Q rows to the
 // doubly-stochastic result:
-//   phase 1  M_ij = sum_k w2_k relu(P_ik + Q_jk) + b2 over the whole hidden dimension (same 1.5-instruction inner loop as
-//            affinity.hip: packed add + fma with the |.| modifier, the linear half as two row sums), 4x4 register tiles,
+//   phase 1  M_ij = sum_k w2_k relu(P_ik + Q_jk) + b2 over the whole hidden dimension (same two-instruction inner loop as
+//            affinity.hip: add + fma with the |.| modifier, the linear half as two row sums), 4x4 register tiles,
 //            16-row sub-tiles beyond the block's edge skipped;  (M - b2) goes to `aff` once (the backward's input, 1x bytes),
 //            L = (M) * log2(e) / tau goes to LDS in the oriented frame (rows = the smaller graph);
 //   phase 2  the block moves into REGISTERS: lane = column, wavefront w owns rows w, w+4, ... (<= 16 per lane).  A row sweep is

@@ -150,7 +150,7 @@ class _RingDataset(DiskDataset):
 
 def _collate(items):
     """Runs in the WORKER process.  A batch crosses the process boundary as plain Python metadata plus EITHER a ring slot
-    number (the pixels are already in shared page-locked memory) OR two shared-memory tensors - the stacked uint8 images and the
+    number (the pixels are already in shared memory) OR two shared-memory tensors - the stacked uint8 images and the
     stacked ground-truth masks: every tensor costs the receiving process a connection to the worker's resource sharer (~1 ms with
     its authentication handshake; 14 tensors per batch were 15 ms), Python numbers cost nothing.  ``expand`` rebuilds the
     per-image dicts as views.  Images of different sizes travel as they are."""

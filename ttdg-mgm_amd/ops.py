@@ -586,7 +586,11 @@ def cross_attention(q, k, v, scale=None, k_lens=None, key_mask=None):
     ``k_lens`` (B,) int32 / int64: the keys j < k_lens[b] exist (values are clamped to 0 .. Tk); ``key_mask`` (B or 1, Tk) bool: the keys with
     True exist.  What stands at other keys - padding, infinities, NaN - never reaches a result; they get zero gradients, and a sample
     without any key gives zeros.  Returns (B, Tq, H, D), contiguous.  One query per sample (a decoding step) and few queries over many keys
-    take the same call: the keys are then split over the chip and joined.  No second and no forward-mode derivatives."""
+    take the same call: the keys are then split over the chip and joined.  No second and no forward-mode derivatives.
+    Sums and softmax statistics are 32 bits; bfloat16 carries score gradients, and in small calls probabilities, in two operands between the two
+    products, in large calls probabilities in one: out and v's gradient are then within 1.45 times their own rounding.  Which form a call takes, and in
+    which order parts are joined, goes by the whole call's size, so a sample may come out one rounding different in another batch; the
+    same call always gives the same bits.  Scores may be of any finite size."""
     _attn_check(q, k, v, k_lens, key_mask)
     scale = q.shape[3] ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
